@@ -284,6 +284,176 @@ PB_API uint32_t pb_rope_table(float *table_host);
  * routine the top-k/top-p weights use: fp32_sse2.rs:378-469 (scalbnf, expf). */
 PB_API uint32_t pb_expf_device(const uint32_t *x_device, uint64_t n, uint32_t *y_device, void *stream);
 
+/* --------------------------------------------------- paged serving operators
+ * Rotary positions, attention over packed prompts and over a paged cache, and
+ * the cache's page operations, for callers that keep their keys and values in
+ * pages instead of an engine's slots (no counterpart in the reference, whose
+ * rotary table, attention and cache serve one sequence of one model:
+ * fp32_sse2.rs:1413-1672, inference.rs:2035-2052).
+ *
+ * All are asynchronous on `stream`, whose device must be the current one and
+ * hold every pointer; none allocates device memory, waits or keeps state, so
+ * they may be captured into a graph and called from any thread.  Arguments that
+ * the host can see are checked first: PB_CAPACITY (a size, count or type that is
+ * not supported), PB_ALIGNMENT (a pointer or stride), each with its text in
+ * pb_last_error_string, and nothing is launched.  What device arrays hold
+ * (positions, offsets, page ids, slots, counts) cannot be checked there: values
+ * that point outside the buffers described here are ignored as each entry says,
+ * never followed.  Operands may not overlap the outputs unless said so. */
+enum { PB_TYPE_F32 = 0, PB_TYPE_F16 = 1, PB_TYPE_BF16 = 2 };
+/* A position, slot or page id that stands for none. */
+#define PB_NONE 0xffffffffu
+/* Sequences of one attention call. */
+#define PB_MAX_SEQS 2048u
+
+/* Rows of heads on the device: element c of head h of row r is data[r *
+ * row_stride + h * head_stride + c], strides in elements.  data is 16-byte
+ * aligned and both strides are multiples of 16 bytes. */
+typedef struct pb_rows {
+    void *data;
+    uint64_t row_stride, head_stride;
+} pb_rows;
+
+/* A paged key/value cache on the device: element c of slot s of head h of page p
+ * of layer n is k[n * layer_stride + ((p * kv_heads + h) * page_size + s) *
+ * head_dim + c], v alike; layer_stride in elements, a multiple of 16 bytes.
+ * page_size is 16, 32, 64, 128 or 256; head_dim a multiple of 16 up to 256 (64
+ * or 128 for attention); pages * page_size below 2^31. */
+typedef struct pb_cache {
+    void *k, *v;
+    uint64_t layer_stride;
+    uint32_t type, layers, pages, page_size, kv_heads, head_dim;
+} pb_cache;
+
+/* Rotary positions.  Pair i of the first rotary_dim elements of a head turns by
+ * the angle position * f_i, f_i = theta^(-2i / rotary_dim), formed in 64 bits:
+ *   a' = m (a cos - b sin), b' = m (b cos + a sin),
+ * (a, b) the elements (i, i + rotary_dim / 2) in PB_ROTARY_HALF and (2i, 2i + 1)
+ * in PB_ROTARY_INTERLEAVED; the rest of the head stays.  For contexts longer
+ * than `original` positions by `factor` (>= 1) the f_i are scaled:
+ *   PB_SCALING_LINEAR  f_i / factor;
+ *   PB_SCALING_BANDS   with t = original f_i / (2 pi) turns over the original
+ *     context: f_i / factor where t <= low, f_i where t >= high, and between
+ *     them the mix of both in proportion to t;
+ *   PB_SCALING_YARN    the same two ends, mixed in proportion to i between
+ *     i0 = floor(d(high)) and i1 = ceil(d(low)), clamped to 0 .. rotary_dim - 1
+ *     (i1 = i0 + 0.001 where not above i0), with
+ *     d(t) = rotary_dim ln(original / (2 pi t)) / (2 ln theta).
+ * m = magnitude; 0 stands for 1, for PB_SCALING_YARN 0.1 ln(factor) + 1.
+ * low and high both 0 stand for 1 and 4 (bands) or 1 and 32 (yarn). */
+enum { PB_ROTARY_HALF = 0, PB_ROTARY_INTERLEAVED = 1 };
+enum { PB_SCALING_NONE = 0, PB_SCALING_LINEAR = 1, PB_SCALING_BANDS = 2, PB_SCALING_YARN = 3 };
+typedef struct pb_rotary_config {
+    uint32_t head_dim, rotary_dim; /* both multiples of 16, rotary_dim <= head_dim <= 256 */
+    uint32_t layout, scaling;
+    double theta, factor, original, low, high, magnitude;
+} pb_rotary_config;
+typedef struct pb_rotary pb_rotary;
+/* The frequencies of a configuration, kept on the host: serves any device. */
+PB_API uint32_t pb_rotary_create(const pb_rotary_config *config, pb_rotary **out);
+PB_API void pb_rotary_destroy(pb_rotary *rotary);
+/* q and k [rows] turned by positions_device[row] into q_out and k_out, which may
+ * be q and k themselves (the same data and strides).  k_heads 0: no k.  A row
+ * whose position is PB_NONE is left out: its outputs stay as they were. */
+PB_API uint32_t pb_rotary_device(const pb_rotary *rotary, uint32_t type, uint32_t rows,
+                                 const uint32_t *positions_device, uint32_t q_heads,
+                                 const pb_rows *q, const pb_rows *q_out, uint32_t k_heads,
+                                 const pb_rows *k, const pb_rows *k_out, void *stream);
+/* The same, with k turned and v as it is written to `layer` of the cache, whose
+ * type, heads and head_dim they have, at slots_device[row] = page * page_size +
+ * slot in the page.  A slot outside the cache (PB_NONE) writes no k and v; the
+ * same slot twice holds either row. */
+PB_API uint32_t pb_rotary_cache_device(const pb_rotary *rotary, uint32_t rows,
+                                       const uint32_t *positions_device, uint32_t q_heads,
+                                       const pb_rows *q, const pb_rows *q_out, const pb_rows *k,
+                                       const pb_rows *v, const pb_cache *cache, uint32_t layer,
+                                       const uint32_t *slots_device, void *stream);
+
+/* Causal attention of packed prompts, out = softmax(scale q k^T) v per head, q
+ * head h reading key head h / (q_heads / kv_heads).  Sequence s has the q rows
+ * [q_offsets[s], q_offsets[s + 1]) and the key rows [kv_offsets[s], kv_offsets
+ * [s + 1]) (kv_offsets NULL: the same), both aligned at their ends: row i of t
+ * sees the first n - t + i + 1 of n keys.  A row that sees none is zero; rows
+ * behind q_offsets[seqs] stay as they were.  Offsets ascend; they are cut at
+ * q_rows and kv_rows.  Keys that a row does not see have no part in it whatever
+ * they hold.  head_dim 64 or 128, seqs up to PB_MAX_SEQS. */
+PB_API uint32_t pb_prompt_attention_device(uint32_t type, uint32_t head_dim, uint32_t q_heads,
+                                           uint32_t kv_heads, uint32_t seqs, uint32_t q_rows,
+                                           uint32_t kv_rows, const pb_rows *q, const pb_rows *k,
+                                           const pb_rows *v, const pb_rows *out,
+                                           const uint32_t *q_offsets_device,
+                                           const uint32_t *kv_offsets_device, float scale,
+                                           void *stream);
+
+/* Attention of drafted token trees over `layer` of a paged cache.  Sequence s
+ * has contexts[s] positions and the rows [offsets[s], offsets[s + 1]) of q, its
+ * drafted nodes, whose keys and values stand in the cache behind the context, at
+ * position contexts[s] + node.  A node sees the whole context and node j of its
+ * sequence where bit j of visible[row] is set (its own bit among them; nodes
+ * past 63 are seen by none).  One node with visible 1 is plain decode.  Position
+ * p of sequence s is slot p % page_size of page tables[s * table_width + p /
+ * page_size]; positions past the table are not seen, a page id outside the cache
+ * reads as zeros.  A row that sees nothing is zero; rows behind offsets[seqs]
+ * stay as they were.
+ * The keys are split over the GPU and joined through `workspace` (16-byte
+ * aligned, pb_tree_attention_workspace bytes for the same type, head_dim, heads,
+ * seqs and rows); calls that can overlap on the GPU need workspaces of their own. */
+PB_API uint64_t pb_tree_attention_workspace(uint32_t type, uint32_t head_dim, uint32_t q_heads,
+                                            uint32_t kv_heads, uint32_t seqs, uint32_t rows);
+PB_API uint32_t pb_tree_attention_device(const pb_cache *cache, uint32_t layer, uint32_t q_heads,
+                                         uint32_t seqs, uint32_t rows, const pb_rows *q,
+                                         const pb_rows *out, const uint32_t *tables_device,
+                                         uint32_t table_width, const uint32_t *contexts_device,
+                                         const uint32_t *offsets_device,
+                                         const uint64_t *visible_device, float scale,
+                                         void *workspace, uint64_t workspace_bytes, void *stream);
+
+/* Copies page pairs[2 i] to page pairs[2 i + 1] for i < n, keys and values of
+ * every layer.  No page may be the target of two pairs or the target of one and
+ * the source of another.  Pairs with a page outside the cache are left out. */
+PB_API uint32_t pb_cache_copy_pages_device(const pb_cache *cache, uint32_t n,
+                                           const uint32_t *pairs_device, void *stream);
+/* Keeps the accepted nodes of drafted trees: for every layer, position contexts
+ * [s] + nodes[s * nodes_width + i] moves to contexts[s] + i, for i < counts[s]
+ * (cut at nodes_width).  nodes ascend within a sequence; an entry below its own
+ * index, below the one before it, or past the table, and a page id outside the
+ * cache, is left out.  The pages that are written belong to one sequence each. */
+PB_API uint32_t pb_cache_keep_device(const pb_cache *cache, uint32_t seqs,
+                                     const uint32_t *tables_device, uint32_t table_width,
+                                     const uint32_t *contexts_device,
+                                     const uint32_t *counts_device, const uint32_t *nodes_device,
+                                     uint32_t nodes_width, void *stream);
+
+/* The host's book of a cache's pages: which pages each sequence holds, counted,
+ * so that forked sequences share them.  Host memory only; one thread at a time.
+ * A call that fails (PB_CAPACITY: too few free pages or sequences, or an array
+ * too short, with the number needed in *needed; PB_STATE: a sequence that is not
+ * open) changes nothing. */
+typedef struct pb_pool pb_pool;
+PB_API uint32_t pb_pool_create(uint32_t pages, uint32_t page_size, uint32_t max_seqs, pb_pool **out);
+PB_API void pb_pool_destroy(pb_pool *pool);
+/* Opens a sequence without tokens. */
+PB_API uint32_t pb_pool_open(pb_pool *pool, uint32_t *seq);
+/* Opens a sequence that shares every page of `seq`. */
+PB_API uint32_t pb_pool_fork(pb_pool *pool, uint32_t seq, uint32_t *child);
+/* Makes room for `tokens` more.  Where the last page is partly filled and
+ * shared, the sequence gets a page of its own in its place and pair[0] = the old
+ * page, pair[1] = the new one for pb_cache_copy_pages_device, to be run before
+ * anything is written; else both are PB_NONE. */
+PB_API uint32_t pb_pool_extend(pb_pool *pool, uint32_t seq, uint32_t tokens, uint32_t *pair,
+                               uint32_t *needed);
+/* Cuts a sequence to `length` tokens and frees the pages behind them. */
+PB_API uint32_t pb_pool_truncate(pb_pool *pool, uint32_t seq, uint32_t length);
+PB_API uint32_t pb_pool_free(pb_pool *pool, uint32_t seq);
+/* Moves the pages in use to the lowest ids: writes n <= capacity pairs (from,
+ * to) for pb_cache_copy_pages_device, after which no page past *used is held. */
+PB_API uint32_t pb_pool_compact(pb_pool *pool, uint32_t *pairs, uint32_t capacity, uint32_t *n,
+                                uint32_t *used, uint32_t *needed);
+/* The length of a sequence and its page ids (PB_NONE behind them). */
+PB_API uint32_t pb_pool_table(const pb_pool *pool, uint32_t seq, uint32_t *table, uint32_t width,
+                              uint32_t *length, uint32_t *needed);
+PB_API uint32_t pb_pool_free_pages(const pb_pool *pool);
+
 #ifdef __cplusplus
 }
 #endif

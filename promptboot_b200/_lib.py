@@ -66,7 +66,29 @@ class PbModelError(ctypes.Structure):
                 self.available, self.detail]
 
 
+class PbRows(ctypes.Structure):
+    """pb_rows: rows of heads on the device, strides in elements."""
+    _fields_ = [("data", P), ("row_stride", u64), ("head_stride", u64)]
+
+
+class PbCache(ctypes.Structure):
+    """pb_cache: a paged key/value cache on the device."""
+    _fields_ = [("k", P), ("v", P), ("layer_stride", u64), ("type", u32), ("layers", u32),
+                ("pages", u32), ("page_size", u32), ("kv_heads", u32), ("head_dim", u32)]
+
+
+class PbRotaryConfig(ctypes.Structure):
+    """pb_rotary_config."""
+    _fields_ = [("head_dim", u32), ("rotary_dim", u32), ("layout", u32), ("scaling", u32),
+                ("theta", ctypes.c_double), ("factor", ctypes.c_double),
+                ("original", ctypes.c_double), ("low", ctypes.c_double), ("high", ctypes.c_double),
+                ("magnitude", ctypes.c_double)]
+
+
 E = ctypes.POINTER(PbError)
+R = ctypes.POINTER(PbRows)
+C = ctypes.POINTER(PbCache)
+U = ctypes.POINTER(u32)
 S = ctypes.POINTER(PbStep)
 
 SIGNATURES = {
@@ -116,6 +138,27 @@ SIGNATURES = {
     "pb_attention_device": (u32, [P, P, u32, u32, P, u32, u32, P, P, P]),
     "pb_rope_table": (u32, [P]),
     "pb_expf_device": (u32, [P, u64, P, P]),
+    "pb_rotary_create": (u32, [ctypes.POINTER(PbRotaryConfig), ctypes.POINTER(P)]),
+    "pb_rotary_destroy": (None, [P]),
+    "pb_rotary_device": (u32, [P, u32, u32, P, u32, R, R, u32, R, R, P]),
+    "pb_rotary_cache_device": (u32, [P, u32, P, u32, R, R, R, R, C, u32, P, P]),
+    "pb_prompt_attention_device": (u32, [u32, u32, u32, u32, u32, u32, u32, R, R, R, R, P, P,
+                                         ctypes.c_float, P]),
+    "pb_tree_attention_workspace": (u64, [u32, u32, u32, u32, u32, u32]),
+    "pb_tree_attention_device": (u32, [C, u32, u32, u32, u32, R, R, P, u32, P, P, P,
+                                       ctypes.c_float, P, u64, P]),
+    "pb_cache_copy_pages_device": (u32, [C, u32, P, P]),
+    "pb_cache_keep_device": (u32, [C, u32, P, u32, P, P, P, u32, P]),
+    "pb_pool_create": (u32, [u32, u32, u32, ctypes.POINTER(P)]),
+    "pb_pool_destroy": (None, [P]),
+    "pb_pool_open": (u32, [P, U]),
+    "pb_pool_fork": (u32, [P, u32, U]),
+    "pb_pool_extend": (u32, [P, u32, u32, U, U]),
+    "pb_pool_truncate": (u32, [P, u32, u32]),
+    "pb_pool_free": (u32, [P, u32]),
+    "pb_pool_compact": (u32, [P, U, u32, U, U, U]),
+    "pb_pool_table": (u32, [P, u32, U, u32, U, U]),
+    "pb_pool_free_pages": (u32, [P]),
 }
 
 _LIB = None

@@ -1,0 +1,327 @@
+// Paged serving attention on the CUDA cores, with every product and sum in
+// binary32.
+//
+// One pass over the keys per row with a running maximum m and sum l (Milakov and
+// Gimelshein's online softmax): for a tile of scores x (in powers of two),
+//   m' = max(m, max x),  o <- o 2^(m - m') + sum 2^(x - m') v,  l alike,
+// and out = o / l.
+#include "pb_attention_paged.cuh"
+#include "pb_attention_launch.h"
+#include "pb_kernels.cuh"
+
+namespace pb {
+namespace paged {
+namespace {
+
+constexpr int kThreads = 128;
+constexpr int kLeast = 2;  // key tiles of a CTA's run at least
+
+// kRpt rows and kKpt keys per thread: 8 thread rows x 16 thread columns.
+template <int kDim, int kRpt>
+struct Simt {
+  static constexpr int kRows = 8 * kRpt;
+  static constexpr int kKeys = kDim == 64 ? 64 : 32;
+  static constexpr int kKpt = kKeys / 16;
+  static constexpr int kPad = kDim + 4;   // row pitch: 16-byte reads of 8 rows hit all banks once
+  static constexpr int kPadP = kKeys + 4;
+  static constexpr int kWords = kRows * kPad + 2 * kKeys * kPad + kRows * kPadP;
+  static size_t bytes(uint32_t seqs) { return (size_t)(kWords + seqs) * 4; }
+};
+
+// kN elements of a row as binary32 at `dst`, from 16 bytes at `src` (zeros: NULL).
+template <class T>
+__device__ __forceinline__ void fill(float* dst, const T* src) {
+  float x[Elements<T>::n] = {};
+  if (src) Elements<T>::load(*reinterpret_cast<const uint4*>(src), x);
+#pragma unroll
+  for (int i = 0; i < Elements<T>::n; i += 4)
+    *reinterpret_cast<float4*>(dst + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+}
+
+template <class T, int kDim, int kRpt, bool kTree>
+__global__ void __launch_bounds__(kThreads) attention_simt_kernel(const __grid_constant__ AttnArgs a) {
+  using C = Simt<kDim, kRpt>;
+  constexpr int kRows = C::kRows, kKeys = C::kKeys, kKpt = C::kKpt, kCols = kDim / 64;
+  extern __shared__ __align__(16) float smem[];
+  float* qs = smem;
+  float* ks = qs + kRows * C::kPad;
+  float* vs = ks + kKeys * C::kPad;
+  float* ps = vs + kKeys * C::kPad;
+  uint32_t* prefix = reinterpret_cast<uint32_t*>(ps + kRows * C::kPadP);
+  work_prefix<kTree, kRows, kKeys, kThreads>(a, prefix);
+  const uint32_t total = prefix[a.seqs - 1];
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+
+  uint32_t next, end;  // this CTA's items: one segment, or a run of key tiles
+  if (kTree) {
+    if (total == 0) return;
+    const Share<kLeast> share(total, gridDim.x);
+    if (blockIdx.x >= share.ctas) return;
+    next = share.start(blockIdx.x);
+    end = share.start(blockIdx.x + 1);
+  } else {
+    if (blockIdx.x >= total) return;
+    next = blockIdx.x;
+    end = next + 1;
+  }
+
+  while (next < end) {
+    Piece p;
+    uint32_t x = next;
+    p.seq = find_sequence(prefix, a.seqs, x);
+    const Sequence s = load_sequence<kTree>(a, p.seq);
+    const uint32_t rows = s.t * a.group, row_tiles = ceil_div(rows, kRows);
+    p.partial = -1;
+    if (kTree) {
+      const uint32_t tiles = max(1u, ceil_div(s.len, kKeys));
+      p.tile0 = x % tiles;
+      p.tile1 = min(tiles, p.tile0 + (end - next));
+      p.head = x / tiles / row_tiles;
+      p.row_tile = x / tiles % row_tiles;
+      if (p.tile0 > 0 || p.tile1 < tiles) p.partial = partial_of(blockIdx.x, p.tile0 == 0);
+      next += p.tile1 - p.tile0;
+    } else {
+      p.head = x % a.kv_heads;
+      p.row_tile = row_tiles - 1 - x / a.kv_heads;
+      const uint32_t last = min(rows, (p.row_tile + 1) * kRows) - 1;
+      p.tile0 = 0;
+      p.tile1 = ceil_div(row_view<false>(a, s, last / a.group).all, kKeys);
+      ++next;
+    }
+
+    __syncthreads();  // the piece before is done with shared memory
+    constexpr int kWord = Elements<T>::n, kWords = kDim / kWord;
+    for (int i = threadIdx.x; i < kRows * kWords; i += kThreads) {
+      const int r = i / kWords, c = i % kWords * kWord;
+      const uint32_t row = p.row_tile * kRows + r;
+      const T* src = nullptr;
+      if (row < rows)
+        src = static_cast<const T*>(a.q.data) + (uint64_t)(s.q0 + row / a.group) * a.q.row_stride +
+              (uint64_t)(p.head * a.group + row % a.group) * a.q.head_stride + c;
+      fill(qs + r * C::kPad + c, src);
+    }
+    RowView view[kRpt];
+    uint32_t all_see = 0xffffffffu;  // keys that every row of this thread sees
+#pragma unroll
+    for (int i = 0; i < kRpt; ++i) {
+      const uint32_t row = p.row_tile * kRows + ty * kRpt + i;
+      view[i] = row < rows ? row_view<kTree>(a, s, row / a.group) : RowView{0xffffffffu, 0ull};
+      all_see = min(all_see, view[i].all);
+    }
+    float m[kRpt], l[kRpt];
+    float4 o[kRpt][kCols];
+#pragma unroll
+    for (int i = 0; i < kRpt; ++i) {
+      m[i] = -INFINITY;
+      l[i] = 0.f;
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) o[i][c] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+
+    for (uint32_t tile = p.tile0; tile < p.tile1; ++tile) {
+      const uint32_t key0 = tile * kKeys;
+      __syncthreads();
+      for (int i = threadIdx.x; i < kKeys * kWords; i += kThreads) {
+        const int j = i / kWords, c = i % kWords * kWord;
+        const uint32_t key = key0 + j;
+        const T *kw = nullptr, *vw = nullptr;
+        if (key < s.len) {
+          if (kTree) {
+            const uint32_t page = a.tables[(uint64_t)p.seq * a.table_width + key / a.cache.page_size];
+            if (page < a.cache.pages) {
+              const uint64_t at = (((uint64_t)page * a.cache.kv_heads + p.head) * a.cache.page_size +
+                                   key % a.cache.page_size) * kDim + c;
+              kw = reinterpret_cast<const T*>(a.cache.k) + at;
+              vw = reinterpret_cast<const T*>(a.cache.v) + at;
+            }
+          } else {
+            const uint64_t row = s.kv0 + key;
+            kw = static_cast<const T*>(a.k.data) + row * a.k.row_stride + p.head * a.k.head_stride + c;
+            vw = static_cast<const T*>(a.v.data) + row * a.v.row_stride + p.head * a.v.head_stride + c;
+          }
+        }
+        fill(ks + j * C::kPad + c, kw);
+        fill(vs + j * C::kPad + c, vw);
+      }
+      __syncthreads();
+
+      float sc[kRpt][kKpt];  // key tx + 16 j
+#pragma unroll
+      for (int i = 0; i < kRpt; ++i)
+#pragma unroll
+        for (int j = 0; j < kKpt; ++j) sc[i][j] = 0.f;
+#pragma unroll 4
+      for (int c = 0; c < kDim; c += 4) {
+        float4 kf[kKpt];
+#pragma unroll
+        for (int j = 0; j < kKpt; ++j)
+          kf[j] = *reinterpret_cast<const float4*>(ks + (tx + 16 * j) * C::kPad + c);
+#pragma unroll
+        for (int i = 0; i < kRpt; ++i) {
+          const float4 qf = *reinterpret_cast<const float4*>(qs + (ty * kRpt + i) * C::kPad + c);
+#pragma unroll
+          for (int j = 0; j < kKpt; ++j) {
+            sc[i][j] = __fmaf_rn(qf.x, kf[j].x, sc[i][j]);
+            sc[i][j] = __fmaf_rn(qf.y, kf[j].y, sc[i][j]);
+            sc[i][j] = __fmaf_rn(qf.z, kf[j].z, sc[i][j]);
+            sc[i][j] = __fmaf_rn(qf.w, kf[j].w, sc[i][j]);
+          }
+        }
+      }
+      // A key that a row does not see gets the weight -0, which the sums below tell
+      // from the weight +0 of a score far below the maximum: its value is left out
+      // whatever it holds.
+      const bool masked = key0 + kKeys > all_see;
+#pragma unroll
+      for (int i = 0; i < kRpt; ++i) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < kKpt; ++j) {
+          const bool seen = !masked || view[i].sees(key0 + tx + 16 * j);
+          sc[i][j] = seen ? __fmul_rn(sc[i][j], a.scale_log2) : -INFINITY;
+          top = fmaxf(top, sc[i][j]);
+        }
+#pragma unroll
+        for (int d = 8; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        const float to = fmaxf(m[i], top);
+        const float base = to == -INFINITY ? 0.f : to;
+        const float keep = exp2f(m[i] - base);  // 0 from -inf
+        m[i] = to;
+        l[i] = __fmul_rn(l[i], keep);
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) {
+          o[i][c].x = __fmul_rn(o[i][c].x, keep); o[i][c].y = __fmul_rn(o[i][c].y, keep);
+          o[i][c].z = __fmul_rn(o[i][c].z, keep); o[i][c].w = __fmul_rn(o[i][c].w, keep);
+        }
+#pragma unroll
+        for (int j = 0; j < kKpt; ++j) {
+          const bool seen = !masked || view[i].sees(key0 + tx + 16 * j);
+          const float w = seen ? exp2f(__fsub_rn(sc[i][j], base)) : -0.f;
+          l[i] += seen ? w : 0.f;
+          ps[(ty * kRpt + i) * C::kPadP + tx + 16 * j] = w;
+        }
+      }
+      __syncwarp();  // a row's weights come from lanes of this warp alone
+      auto add_values = [&](auto checked) {
+#pragma unroll 2
+        for (int j = 0; j < kKeys; j += 4) {
+          float4 vf[4][kCols];
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int c = 0; c < kCols; ++c)
+              vf[u][c] = *reinterpret_cast<const float4*>(vs + (j + u) * C::kPad + c * 64 + tx * 4);
+#pragma unroll
+          for (int i = 0; i < kRpt; ++i) {
+            const float4 w4 = *reinterpret_cast<const float4*>(ps + (ty * kRpt + i) * C::kPadP + j);
+            const float w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              if (decltype(checked)::value && __float_as_uint(w[u]) == 0x80000000u) continue;
+#pragma unroll
+              for (int c = 0; c < kCols; ++c) {
+                o[i][c].x = __fmaf_rn(w[u], vf[u][c].x, o[i][c].x);
+                o[i][c].y = __fmaf_rn(w[u], vf[u][c].y, o[i][c].y);
+                o[i][c].z = __fmaf_rn(w[u], vf[u][c].z, o[i][c].z);
+                o[i][c].w = __fmaf_rn(w[u], vf[u][c].w, o[i][c].w);
+              }
+            }
+          }
+        }
+      };
+      if (masked) add_values(std::true_type{});
+      else add_values(std::false_type{});
+    }
+
+#pragma unroll
+    for (int i = 0; i < kRpt; ++i) {
+#pragma unroll
+      for (int d = 8; d; d >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], d);
+      const uint32_t r = ty * kRpt + i, row = p.row_tile * kRows + r;
+      if (row >= rows) continue;
+      if (p.partial >= 0) {
+        float* rec = a.partial + (size_t)p.partial * partial_words<kRows, kDim>();
+#pragma unroll
+        for (int c = 0; c < kCols; ++c)
+          *reinterpret_cast<float4*>(rec + r * kDim + c * 64 + tx * 4) = o[i][c];
+        if (tx == 0) {
+          rec[kRows * kDim + r] = m[i];
+          rec[kRows * kDim + kRows + r] = l[i];
+        }
+      } else {
+        const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
+        T* out = static_cast<T*>(a.out.data) + (uint64_t)(s.q0 + row / a.group) * a.out.row_stride +
+                 (uint64_t)(p.head * a.group + row % a.group) * a.out.head_stride;
+#pragma unroll
+        for (int c = 0; c < kCols; ++c)
+          store4(out + c * 64 + tx * 4,
+                 make_float4(o[i][c].x * inv, o[i][c].y * inv, o[i][c].z * inv, o[i][c].w * inv));
+      }
+    }
+  }
+}
+
+template <class T, int kDim, int kRpt, bool kTree>
+uint32_t launch(const AttnArgs& a, uint32_t grid, cudaStream_t s) {
+  using C = Simt<kDim, kRpt>;
+  auto kernel = attention_simt_kernel<T, kDim, kRpt, kTree>;
+  static std::atomic<uint64_t> configured{0};
+  if (attribute_needed(configured)) {
+    PB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 (int)C::bytes(PB_MAX_SEQS)));
+    attribute_done(configured);
+  }
+  kernel<<<grid, kThreads, C::bytes(a.seqs), s>>>(a);
+  PB_CUDA(cudaGetLastError());
+  if (kTree) {
+    const dim3 join(std::min<uint32_t>(grid, 1024), C::kRows >= 32 ? 4 : 1);
+    combine_kernel<T, kDim, C::kRows, C::kKeys, kLeast><<<join, 256, a.seqs * 4, s>>>(a, grid);
+    PB_CUDA(cudaGetLastError());
+  }
+  return PB_OK;
+}
+
+constexpr int kFewRpt = 2, kManyRpt = 8;  // 16 or 64 rows of a tile
+
+}  // namespace
+
+template <class T>
+static uint32_t prompt(const AttnArgs& a, uint32_t head_dim, cudaStream_t s) {
+  const uint32_t rows = a.q_rows * a.group;
+  const uint32_t grid = (rows / (8 * kManyRpt) + a.seqs) * a.kv_heads;
+  return head_dim == 64 ? launch<T, 64, kManyRpt, false>(a, grid, s)
+                        : launch<T, 128, kManyRpt, false>(a, grid, s);
+}
+
+uint32_t simt_prompt(const AttnArgs& a, uint32_t type, uint32_t head_dim, cudaStream_t s) {
+  if (type == PB_TYPE_F32) return prompt<float>(a, head_dim, s);
+  if (type == PB_TYPE_F16) return prompt<__half>(a, head_dim, s);
+  return prompt<__nv_bfloat16>(a, head_dim, s);
+}
+
+// Row tiles of 16 where a sequence has no more rows than that on average.
+static bool few(uint32_t rows, uint32_t seqs) { return rows <= 16 * seqs; }
+
+uint64_t simt_tree_words(uint32_t head_dim, uint32_t rows, uint32_t seqs) {
+  const uint32_t tile = few(rows, seqs) ? 8 * kFewRpt : 8 * kManyRpt;
+  return (uint64_t)tree_ctas(4) * 2 * tile * (head_dim + 2);
+}
+
+template <class T>
+static uint32_t tree(const AttnArgs& a, uint32_t head_dim, cudaStream_t s) {
+  const uint32_t grid = tree_ctas(4);
+  if (few(a.q_rows * a.group, a.seqs))
+    return head_dim == 64 ? launch<T, 64, kFewRpt, true>(a, grid, s)
+                          : launch<T, 128, kFewRpt, true>(a, grid, s);
+  return head_dim == 64 ? launch<T, 64, kManyRpt, true>(a, grid, s)
+                        : launch<T, 128, kManyRpt, true>(a, grid, s);
+}
+
+uint32_t simt_tree(const AttnArgs& a, uint32_t type, uint32_t head_dim, cudaStream_t s) {
+  if (type == PB_TYPE_F32) return tree<float>(a, head_dim, s);
+  if (type == PB_TYPE_F16) return tree<__half>(a, head_dim, s);
+  return tree<__nv_bfloat16>(a, head_dim, s);
+}
+
+}  // namespace paged
+}  // namespace pb

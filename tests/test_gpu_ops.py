@@ -1,0 +1,714 @@
+"""The paged serving operators (promptboot_b200.ops) on the GPU against their
+definitions in binary64.
+
+Tolerances are bounds, not fits.  A result rounded to its type is off by half a
+step, eps / 2 of its value (and half the smallest subnormal); what comes before it
+is bounded per element:
+ * rotary: the angle in turns is rounded to binary32 after its whole part is taken
+   off (2^-25 of half a turn), sincospi is within 2 ulp, and the two products, the
+   sum and the magnitude round once each: at most 7e-7 m (|a| + |b|) in all;
+ * attention: a score of d products summed in binary32 is off by 2 d 2^-24 of the
+   sum of their magnitudes (twice, for sums that truncate), which scales its weight
+   by as much times the scale; weights round to the type of v where products run on
+   the tensor cores (eps / 2), the exponential adds 2^-21, and n sums add n 2^-23.
+   All of these are relative to weights, so the result is off by at most their sum
+   (twice the score's part: it enters the sum of weights too) times the weighted
+   mean of |v|.
+"""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+from promptboot_b200 import ops  # noqa: E402
+
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+NAN = float("nan")
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def normal(g, *shape, dtype=torch.float32, scale=1.0):
+    return (torch.randn(*shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+def i32(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def starts(counts):
+    return i32(np.concatenate([[0], np.cumsum(counts)]).tolist())
+
+
+def half_step(dtype, y):
+    """Half a step of the type at y, in binary64."""
+    info = torch.finfo(dtype)
+    return y.abs() * (info.eps / 2) + info.smallest_normal * info.eps / 2
+
+
+def assert_within(got, want, bound):
+    assert got.shape == want.shape
+    off = (got.double() - want).abs()
+    bad = ~(off <= bound)
+    assert not bad.any(), (int(bad.sum()), off[bad].max().item(), (off / bound)[bad].max().item(),
+                           bad.nonzero()[:3].tolist())
+
+
+# ------------------------------------------------------------------------ rotary
+
+def frequencies(rd, theta, scaling, factor, original, low, high):
+    f = theta ** (-2.0 * np.arange(rd // 2) / rd)
+    if scaling == "linear":
+        return f / factor
+    if scaling == "bands":
+        keep = np.clip((original * f / (2 * math.pi) - low) / (high - low), 0, 1)
+        return f / factor * (1 - keep) + f * keep
+    if scaling == "yarn":
+        def place(turns):
+            return rd * math.log(original / (2 * math.pi * turns)) / (2 * math.log(theta))
+        i0, i1 = max(math.floor(place(high)), 0), min(math.ceil(place(low)), rd - 1)
+        i1 = i1 if i1 > i0 else i0 + 0.001
+        keep = 1 - np.clip((np.arange(rd // 2) - i0) / (i1 - i0), 0, 1)
+        return f / factor * (1 - keep) + f * keep
+    return f
+
+
+def turned(x, positions, f, interleaved, magnitude):
+    """(turned rows, |a| + |b| of each element's pair) in binary64."""
+    x = x.double()
+    rd = 2 * len(f)
+    angle = positions.double()[:, None] * torch.tensor(f, device="cuda")
+    c, s = angle.cos()[:, None] * magnitude, angle.sin()[:, None] * magnitude
+    y, size = x.clone(), torch.zeros_like(x)
+    a_at = slice(0, rd, 2) if interleaved else slice(0, rd // 2)
+    b_at = slice(1, rd, 2) if interleaved else slice(rd // 2, rd)
+    a, b = x[..., a_at], x[..., b_at]
+    y[..., a_at], y[..., b_at] = a * c - b * s, b * c + a * s
+    size[..., a_at] = size[..., b_at] = a.abs() + b.abs()
+    return y, size
+
+
+ROTARY = [  # head_dim, rotary_dim, interleaved, scaling, theta, factor, original, low, high
+    (64, 64, False, "none", 1e6, 1.0, 0, 0, 0),
+    (64, 64, True, "linear", 1e4, 4.0, 0, 0, 0),
+    (128, 64, False, "bands", 5e5, 8.0, 8192, 0, 0),
+    (128, 32, True, "yarn", 1e6, 4.0, 32768, 0, 0),
+    (64, 64, False, "yarn", 1e4, 2.5, 2048, 0.5, 16.0),
+    (80, 16, True, "bands", 1e4, 2.0, 4096, 1.0, 2.0),
+    (256, 256, False, "none", 1e4, 1.0, 0, 0, 0),
+    (16, 16, True, "none", 1e4, 1.0, 0, 0, 0),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", ROTARY, ids=lambda s: f"{s[0]}-{s[1]}-{'adjacent' if s[2] else 'halves'}-{s[3]}")
+@pytest.mark.parametrize("rows,heads,kv_heads", [(1, 14, 2), (37, 3, 1), (2100, 5, 2)])
+def test_rotary_matches_the_definition(dtype, shape, rows, heads, kv_heads):
+    dim, rd, interleaved, scaling, theta, factor, original, low, high = shape
+    g = gen(rows + dim)
+    q, k = normal(g, rows, heads, dim, dtype=dtype, scale=3.0), normal(g, rows, kv_heads, dim, dtype=dtype)
+    positions = torch.randint(0, 1 << 20, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    positions[0] = 0
+    plan = ops.Rotary(dim, rd, theta, interleaved, scaling, factor, original, low, high)
+    f = frequencies(rd, theta, scaling, factor, original, low or 1.0, high or (32.0 if scaling == "yarn" else 4.0))
+    m = 0.1 * math.log(factor) + 1 if scaling == "yarn" else 1.0
+    q1, k1 = plan.apply(q, k, positions)
+    for got, x in ((q1, q), (k1, k)):
+        want, size = turned(x, positions, f, interleaved, m)
+        assert got.dtype == dtype
+        assert_within(got, want, half_step(dtype, want) + 7e-7 * m * size)
+        assert torch.equal(got[..., rd:], x[..., rd:])
+    # in place gives the same bits
+    plan.apply(q, k, positions, q_out=q, k_out=k)
+    assert torch.equal(q, q1) and torch.equal(k, k1)
+
+
+def test_rotary_far_positions_magnitude_and_rows_left_out():
+    """Positions up to 2^32 - 2 keep their angle; 0xffffffff leaves a row alone."""
+    g = gen(3)
+    q, k = normal(g, 6, 2, 64), normal(g, 6, 1, 64)
+    at = np.array([0, 1, 2**24 + 1, 2**31 + 5, 2**32 - 2, 2**32 - 1], dtype=np.uint32)
+    positions = torch.from_numpy(at.view(np.int32)).cuda()
+    plan = ops.Rotary(64, theta=1e4, magnitude=1.75)
+    q_out, k_out = torch.full_like(q, NAN), torch.full_like(k, NAN)
+    plan.apply(q, k, positions, q_out, k_out)
+    f = frequencies(64, 1e4, "none", 1, 0, 0, 0)
+    # an angle of 2^32 is off by 2^32 2^-53 of a turn before it is reduced: below 4e-6
+    for got, x in ((q_out, q), (k_out, k)):
+        want, size = turned(x, torch.from_numpy(at.astype(np.float64)).cuda(), f, False, 1.75)
+        assert_within(got[:5], want[:5], half_step(torch.float32, want[:5]) + (1.75 * 7e-7 + 8e-6) * size[:5])
+        assert got[5].isnan().all()
+
+
+def test_rotary_of_stacked_projection_views():
+    g = gen(4)
+    stacked = normal(g, 50, 14 + 2 + 2, 64, dtype=torch.bfloat16)
+    q, k = stacked[:, :14], stacked[:, 14:16]
+    positions = torch.arange(50, dtype=torch.int32, device="cuda")
+    plan = ops.Rotary(64)
+    want = plan.apply(q.contiguous(), k.contiguous(), positions)
+    v = stacked[:, 16:].clone()
+    plan.apply(q, k, positions, q_out=q, k_out=k)  # in place in the stack
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(stacked[:, 16:], v)
+    by_head = torch.empty(14, 50, 64, dtype=torch.bfloat16, device="cuda")
+    plan.apply(normal(gen(4), 50, 18, 64, dtype=torch.bfloat16)[:, :14], k, positions, q_out=by_head.transpose(0, 1))
+    assert torch.equal(by_head.transpose(0, 1), want[0])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("page,rows", [(16, 1), (64, 45), (256, 1200)])
+def test_rotary_to_cache(dtype, page, rows):
+    g = gen(rows)
+    pages, layers, dim, kv_heads = rows // page + 4, 3, 64, 2
+    q = normal(g, rows, 6, dim, dtype=dtype)
+    k, v = normal(g, rows, kv_heads, dim, dtype=dtype), normal(g, rows, kv_heads, dim, dtype=dtype)
+    cache = ops.PageCache(normal(g, layers, pages, kv_heads, page, dim, dtype=dtype),
+                          normal(g, layers, pages, kv_heads, page, dim, dtype=dtype))
+    positions = torch.randint(0, 40000, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    slots = torch.randperm(pages * page, generator=g, device="cuda", dtype=torch.int32)[:rows].contiguous()
+    if rows > 10:
+        slots[2], slots[3], slots[4] = -1, pages * page, 2**31 - 1  # none, just past the cache, far past it
+        positions[5] = -1
+    plan = ops.Rotary(dim)
+    want_q, want_k = plan.apply(q, k, positions)
+    want = [cache.k.clone(), cache.v.clone()]
+    for r, (s, p) in enumerate(zip(slots.tolist(), positions.tolist())):
+        if 0 <= s < pages * page and p >= 0:
+            want[0][1, s // page, :, s % page] = want_k[r]
+            want[1][1, s // page, :, s % page] = v[r]
+    q_out = torch.zeros_like(q)
+    plan.apply_to_cache(q, k, v, positions, cache, slots, layer=1, q_out=q_out)
+    there = positions >= 0
+    assert torch.equal(q_out[there], want_q[there]) and not q_out[~there].any()
+    assert torch.equal(cache.k, want[0]) and torch.equal(cache.v, want[1])
+
+
+# --------------------------------------------------------------------- attention
+
+def attend(q, k, v, seen, scale, dtype):
+    """(result, bound) of one head in binary64: q [t, d], k and v [n, d], seen [t, n].
+    Keys and values that a row does not see are taken out of its sums."""
+    q, k, v = q.double(), k.double(), v.double()
+    hidden = ~seen.any(0)
+    k, v = k.masked_fill(hidden[:, None], 0.0), v.masked_fill(hidden[:, None], 0.0)
+    d, n = q.shape[1], k.shape[0]
+    if n == 0:
+        return torch.zeros_like(q), torch.full_like(q, 1e-300)
+    s = (q @ k.t() * scale).masked_fill(~seen, -math.inf)
+    p = torch.softmax(s, -1).nan_to_num(0.0)
+    y, mean = p @ v, p @ v.abs()
+    size = (q.abs() @ k.abs().t() * scale).masked_fill(~seen, 0.0).amax(-1, keepdim=True)
+    weights = 0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
+    part = 2 * (2 * d * 2.0**-24 * size + 2.0**-21) + weights + n * 2.0**-23
+    return y, half_step(dtype, y) + part * mean
+
+
+def check_heads(got, q, keys, values, seen, scale, dtype):
+    """got, q [t, heads, d]; keys and values [n, kv_heads, d]."""
+    group = q.shape[1] // keys.shape[1]
+    for h in range(q.shape[1]):
+        y, bound = attend(q[:, h], keys[:, h // group], values[:, h // group], seen, scale, dtype)
+        assert_within(got[:, h], y, bound)
+
+
+def causal(t, n):
+    return torch.ones(t, n, dtype=torch.bool, device="cuda").tril(n - t)
+
+
+PROMPTS = [  # tokens and keys of each sequence
+    ([1], None), ([5, 0, 1, 130, 0], None), ([257], None), ([64, 128, 127, 129, 2], None),
+    ([3, 40, 200], [700, 41, 200]), ([20, 9, 5], [4, 0, 9]), ([1, 1, 1], [1, 129, 1000]), ([1500, 33], None),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 14, 2), (128, 4, 4), (64, 3, 1), (128, 16, 2)])
+@pytest.mark.parametrize("tokens,keys", PROMPTS, ids=[f"{a}-{b}" for a, b in PROMPTS])
+def test_prompt_attention_matches_the_definition(dtype, dim, heads, kv_heads, tokens, keys):
+    g = gen(sum(tokens) + dim)
+    extra = 3  # rows behind the last sequence
+    q = normal(g, sum(tokens) + extra, heads, dim, dtype=dtype, scale=2.0)
+    counts = keys or tokens
+    n = sum(counts) + (extra if keys is None else 0)
+    k, v = normal(g, n, kv_heads, dim, dtype=dtype), normal(g, n, kv_heads, dim, dtype=dtype)
+    out = torch.full_like(q, 7.0)
+    got = ops.prompt_attention(q, k, v, starts(tokens), None if keys is None else starts(keys), out=out)
+    assert got is out and (out[sum(tokens):] == 7.0).all()
+    at = kv_at = 0
+    for t, c in zip(tokens, counts):
+        check_heads(out[at:at + t], q[at:at + t], k[kv_at:kv_at + c], v[kv_at:kv_at + c], causal(t, c),
+                    dim ** -0.5, dtype)
+        at, kv_at = at + t, kv_at + c
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_prompt_attention_keeps_out_what_a_row_does_not_see(dtype, dim):
+    """A NaN or an infinity in a key or a value reaches the rows that see it and no
+    other: not earlier rows, not the next sequence, not rows past the keys."""
+    g = gen(8)
+    tokens = [70, 133, 20]
+    total = sum(tokens)
+    q, k, v = (normal(g, total + 5, h, dim, dtype=dtype) for h in (4, 2, 2))
+    want = ops.prompt_attention(q, k, v, starts(tokens))[:total].clone()
+    k[total:], v[total:] = NAN, math.inf
+    k[100, 0], v[100, 1, 3] = NAN, NAN   # sequence 1, token 30
+    v[150, 0, 5], v[150, 0, 6] = math.inf, -math.inf   # its token 80
+    v[69, 0], k[69, 1] = NAN, math.inf   # the last token of sequence 0
+    got = ops.prompt_attention(q, k, v, starts(tokens))[:total]
+    clean = torch.ones(total, dtype=torch.bool, device="cuda")
+    clean[69] = False
+    clean[100:203] = False
+    assert torch.equal(got[clean], want[clean])
+    assert got[100:203, :2].isnan().all()      # heads of key head 0 see a NaN score
+    assert got[100:203, 2:, 3].isnan().all()   # a NaN value stays in its component
+    assert torch.equal(got[100:203, 2:, 4], want[100:203, 2:, 4])
+    assert got[69, :2].isnan().all()
+
+
+def test_prompt_attention_infinite_value_reaches_its_component():
+    for dtype in TYPES:
+        g = gen(9)
+        q, k, v = (normal(g, 40, 1, 64, dtype=dtype) for _ in range(3))
+        want = ops.prompt_attention(q, k, v, starts([40])).clone()
+        v[25, 0, 5], v[25, 0, 6] = math.inf, -math.inf
+        got = ops.prompt_attention(q, k, v, starts([40]))
+        assert (got[25:, 0, 5] == math.inf).all() and (got[25:, 0, 6] == -math.inf).all()
+        got[25:, 0, 5:7] = want[25:, 0, 5:7]
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_prompt_attention_of_stacked_views_and_a_given_scale(dtype):
+    g = gen(10)
+    stacked = normal(g, 300, 18, 64, dtype=dtype)
+    q, k, v = stacked[:, :14], stacked[:, 14:16], stacked[:, 16:]
+    by_head = torch.zeros(14, 300, 64, dtype=dtype, device="cuda")
+    tokens = [170, 130]
+    ops.prompt_attention(q, k, v, starts(tokens), scale=0.3, out=by_head.transpose(0, 1))
+    for at, t in ((0, 170), (170, 130)):
+        rows = slice(at, at + t)
+        check_heads(by_head.transpose(0, 1)[rows], q[rows], k[rows], v[rows], causal(t, t), 0.3, dtype)
+
+
+def test_prompt_attention_cuts_offsets_at_the_rows():
+    g = gen(11)
+    q, k, v = (normal(g, 40, 2, 64) for _ in range(3))
+    want = ops.prompt_attention(q, k, v, i32([0, 25, 40]))
+    got = ops.prompt_attention(q, k, v, i32([0, 25, 1000]))
+    assert torch.equal(got, want)
+    out = torch.full_like(q, 5.0)
+    ops.prompt_attention(q, k, v, i32([30, 10, 10, 2**31 - 1]), out=out)  # the first descends: no rows
+    assert (out[:10] == 5.0).all() and not (out[10:] == 5.0).any()
+
+
+def test_prompt_attention_large_scores_and_growing_maxima():
+    """Scores of some hundreds, growing along the keys, so that the running maximum
+    moves at every tile; and a row of equal scores."""
+    for dtype in TYPES:
+        g = gen(12)
+        n, dim = 700, 64
+        q = torch.ones(n, 1, dim, device="cuda")
+        k = torch.linspace(-6, 6, n, device="cuda")[:, None, None].expand(n, 1, dim).contiguous()
+        k[::3] *= -1
+        q, k = q.to(dtype), k.to(dtype)
+        v = normal(g, n, 1, dim, dtype=dtype)
+        got = ops.prompt_attention(q, k, v, starts([n]), scale=0.7)
+        check_heads(got, q, k, v, causal(n, n), 0.7, dtype)
+        got = ops.prompt_attention(q, k * 0, v, starts([n]))
+        check_heads(got, q, k * 0, v, causal(n, n), 0.125, dtype)
+
+
+def masks(values):
+    return torch.from_numpy(np.array(values, dtype=np.uint64).view(np.int64)).cuda()
+
+
+def random_tree(rng, t):
+    bits = []
+    for i in range(t):
+        parent = int(rng.integers(-1, i)) if i else -1
+        bits.append((bits[parent] if 0 <= parent < 64 else 0) | (1 << i if i < 64 else 0))
+    return bits
+
+
+def paged(g, rng, lengths, page, kv_heads, dim, dtype, layers=2, junk=None):
+    """A cache whose sequences lie on scattered pages, with `junk` in every slot that
+    holds none of their positions; and the sequences' keys and values."""
+    need = [-(-n // page) for n in lengths]
+    pages = sum(need) + 3
+    ids = rng.permutation(pages)
+    cache = ops.PageCache.empty(layers, pages, kv_heads, page, dim, dtype)
+    cache.k.fill_(1.0 if junk is None else junk)
+    cache.v.fill_(1.0 if junk is None else junk)
+    width = max(need + [1]) + 1
+    table = np.full((len(lengths), width), -1, dtype=np.int32)
+    keys, values, at = [], [], 0
+    for s, n in enumerate(lengths):
+        mine = ids[at:at + need[s]]
+        at += need[s]
+        table[s, :need[s]] = mine
+        k, v = normal(g, n, kv_heads, dim, dtype=dtype), normal(g, n, kv_heads, dim, dtype=dtype)
+        p = np.arange(n)
+        where = torch.from_numpy(mine[p // page].astype(np.int64)).cuda(), slice(None), torch.from_numpy(p % page).cuda()
+        cache.k[1][where], cache.v[1][where] = k, v
+        keys.append(k)
+        values.append(v)
+    return cache, torch.from_numpy(table).cuda(), keys, values
+
+
+def check_tree(got, q, contexts, nodes, visible, keys, values, scale, dtype):
+    at = 0
+    for s, (c, t) in enumerate(zip(contexts, nodes)):
+        n = c + min(t, 64)
+        seen = torch.zeros(t, n, dtype=torch.bool, device="cuda")
+        seen[:, :c] = True
+        for i in range(t):
+            for j in range(n - c):
+                seen[i, c + j] = (visible[at + i] >> j) & 1
+        check_heads(got[at:at + t], q[at:at + t], keys[s][:n], values[s][:n], seen, scale, dtype)
+        at += t
+
+
+TREES = [  # contexts, nodes
+    ([0], [1]), ([1], [1]), ([300, 17, 0, 128], [1, 1, 1, 1]), ([127, 129, 64], [1, 2, 5]),
+    ([1000, 0, 5, 250], [17, 33, 0, 9]), ([90, 200], [64, 63]), ([40], [70]), ([4097, 3, 2000], [4, 4, 8]),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,heads,kv_heads,page", [(64, 14, 2, 16), (128, 4, 4, 64), (64, 8, 1, 256), (128, 16, 2, 32),
+                                                     (64, 4, 2, 128)])
+@pytest.mark.parametrize("contexts,nodes", TREES, ids=[f"{a}-{b}" for a, b in TREES])
+def test_tree_attention_matches_the_definition(dtype, dim, heads, kv_heads, page, contexts, nodes):
+    g, rng = gen(sum(contexts) + dim), np.random.default_rng(sum(contexts) + page)
+    # slots behind the last position hold NaN: they are seen by none
+    cache, tables, keys, values = paged(g, rng, [c + t for c, t in zip(contexts, nodes)], page, kv_heads, dim, dtype,
+                                        junk=NAN)
+    q = normal(g, sum(nodes) + 2, heads, dim, dtype=dtype, scale=2.0)
+    visible = [b for t in nodes for b in random_tree(rng, t)]
+    out = torch.full_like(q, 7.0)
+    got = ops.tree_attention(q, cache, tables, i32(contexts), starts(nodes), masks(visible + [0, 0]), layer=1, out=out)
+    assert got is out and (out[sum(nodes):] == 7.0).all()
+    check_tree(out, q, contexts, nodes, visible, keys, values, dim ** -0.5, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_tree_attention_rows_that_see_nothing_and_odd_masks(dtype):
+    """Masks that leave a row empty without a context, that skip the row's own node,
+    and whose bits past the last node mean nothing."""
+    g, rng = gen(20), np.random.default_rng(20)
+    contexts, nodes = [0, 30], [4, 4]
+    cache, tables, keys, values = paged(g, rng, [4, 34], 16, 2, 64, dtype)
+    q = normal(g, 8, 6, 64, dtype=dtype)
+    visible = [0, 1, 0b1110, 2**64 - 1, 0, 0b0100, 2**63 + 1, 2**64 - 16]
+    got = ops.tree_attention(q, cache, tables, i32(contexts), starts(nodes), masks(visible), layer=1)
+    assert not got[0].any()
+    check_tree(got, q, contexts, nodes, visible, keys, values, 0.125, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("nodes", [1, 12])
+def test_tree_attention_keeps_out_what_a_node_does_not_see(dtype, nodes):
+    """NaN keys and values of a node that others do not see stay with it."""
+    g, rng = gen(21), np.random.default_rng(21)
+    contexts = [200, 75]
+    cache, tables, keys, values = paged(g, rng, [c + nodes for c in contexts], 32, 2, 64, dtype)
+    q = normal(g, 2 * nodes, 8, 64, dtype=dtype)
+    visible = [1 << i for i in range(nodes)] * 2
+    args = (tables, i32(contexts), starts([nodes] * 2), masks(visible))
+    want = ops.tree_attention(q, cache, *args, layer=1).clone()
+    bad = 200 + nodes - 1
+    page, slot = int(tables[0, bad // 32]), bad % 32
+    cache.v[1, page, 0, slot] = math.inf
+    cache.v[1, page, 1, slot, 7] = NAN
+    got = ops.tree_attention(q, cache, *args, layer=1)
+    others = [r for r in range(2 * nodes) if r != nodes - 1]
+    assert torch.equal(got[others], want[others])
+    assert (got[nodes - 1, :4] == math.inf).all() and got[nodes - 1, 4:, 7].isnan().all()
+    cache.k[1, page, :, slot] = NAN
+    got = ops.tree_attention(q, cache, *args, layer=1)
+    assert torch.equal(got[others], want[others]) and got[nodes - 1].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_tree_attention_tables_that_end_and_pages_outside_the_cache(dtype):
+    """Positions past the table are not seen; a page id outside the cache is zeros."""
+    g, rng = gen(22), np.random.default_rng(22)
+    cache, tables, keys, values = paged(g, rng, [64], 16, 1, 64, dtype)
+    q = normal(g, 1, 2, 64, dtype=dtype)
+    short = tables[:, :2].contiguous()  # 32 positions
+    got = ops.tree_attention(q, cache, short, i32([60]), i32([0, 1]), masks([1]), layer=1)
+    seen = torch.ones(1, 32, dtype=torch.bool, device="cuda")
+    check_heads(got, q, keys[0][:32], values[0][:32], seen, 0.125, dtype)
+    lost = tables[:, :4].clone()
+    lost[0, 1], lost[0, 2] = -1, cache.pages
+    keys[0][16:48], values[0][16:48] = 0, 0
+    got = ops.tree_attention(q, cache, lost, i32([63]), i32([0, 1]), masks([1]), layer=1)
+    check_heads(got, q, keys[0], values[0], torch.ones(1, 64, dtype=torch.bool, device="cuda"), 0.125, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("seqs,nodes", [(1, 1), (2, 48), (300, 1), (40, 3)])
+def test_tree_attention_of_long_and_of_many_contexts(dtype, seqs, nodes):
+    """Contexts that are split over many CTAs, and more sequences than CTAs; the
+    second call on the same workspace gives the same bits."""
+    g, rng = gen(23), np.random.default_rng(seqs)
+    contexts = [30011, 12345][:seqs] if seqs < 3 else [int(c) for c in rng.integers(0, 900, seqs)]
+    cache, tables, keys, values = paged(g, rng, [c + nodes for c in contexts], 64, 2, 64, dtype)
+    q = normal(g, seqs * nodes, 14, 64, dtype=dtype, scale=2.0)
+    visible = [b for _ in range(seqs) for b in random_tree(rng, nodes)]
+    work = torch.full((ops.tree_workspace_bytes(cache, 14, seqs, seqs * nodes),), 255, dtype=torch.uint8, device="cuda")
+    args = (q, cache, tables, i32(contexts), starts([nodes] * seqs), masks(visible))
+    got = ops.tree_attention(*args, layer=1, workspace=work)
+    check_tree(got, q, contexts, [nodes] * seqs, visible, keys, values, 0.125, dtype)
+    assert torch.equal(got, ops.tree_attention(*args, layer=1, workspace=work))
+
+
+# ------------------------------------------------------------------------- pages
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layers,page,kv_heads,dim,n", [(1, 16, 1, 16, 1), (3, 32, 2, 64, 7), (2, 256, 1, 128, 40), (24, 16, 3, 48, 5)])
+def test_copy_pages(dtype, layers, page, kv_heads, dim, n):
+    g = gen(n)
+    pages = 2 * n + 3
+    big = normal(g, layers + 1, pages, kv_heads, page, dim, dtype=dtype)
+    other = normal(g, layers + 1, pages, kv_heads, page, dim, dtype=dtype)
+    cache = ops.PageCache(big[:layers], other[:layers])
+    ids = torch.randperm(pages, generator=g, device="cuda", dtype=torch.int32)
+    pairs = ids[:2 * n].reshape(-1, 2).contiguous()
+    lost = i32([[0, pages], [-1, 1], [pages, 2]])  # left out
+    want = [big.clone(), other.clone()]
+    for a, b in pairs.tolist():
+        for w in want:
+            w[:layers, b] = w[:layers, a]
+    cache.copy_pages(torch.cat([pairs, lost]))
+    assert torch.equal(big, want[0]) and torch.equal(other, want[1])
+    cache.copy_pages(pairs[:0])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("page,kv_heads,dim", [(16, 2, 64), (64, 1, 128), (32, 3, 16)])
+def test_keep_moves_the_accepted_path(dtype, page, kv_heads, dim):
+    g, rng = gen(page), np.random.default_rng(page)
+    contexts = [0, 13, 16, 100, 255]
+    paths = [[0, 1, 2], [2, 5, 9, 10, 11, 20, 21, 30, 33, 40], [], [63], [0, 2, 3]]
+    counts = [len(p) for p in paths]
+    counts[4] = 2  # the rest of the row is not kept
+    cache, tables, _, _ = paged(g, rng, [c + 64 for c in contexts], page, kv_heads, dim, dtype)
+    cache.k.copy_(normal(g, *cache.k.shape, dtype=dtype))
+    cache.v.copy_(normal(g, *cache.v.shape, dtype=dtype))
+    want, table = [cache.k.clone(), cache.v.clone()], tables.tolist()
+    for s, (c, path) in enumerate(zip(contexts, paths)):
+        for w, x in zip(want, (cache.k, cache.v)):
+            for i, n in enumerate(path[:counts[s]]):
+                a, b = c + n, c + i
+                w[:, table[s][b // page], :, b % page] = x[:, table[s][a // page], :, a % page]
+    nodes = i32([p + [0] * (10 - len(p)) for p in paths])
+    cache.keep(tables, i32(contexts), i32(counts), nodes)
+    assert torch.equal(cache.k, want[0]) and torch.equal(cache.v, want[1])
+
+
+def test_keep_leaves_out_entries_that_are_no_path():
+    """Below their own index, not ascending, past the table, on a page outside the
+    cache; a count past the row is cut."""
+    g, rng = gen(30), np.random.default_rng(30)
+    cache, tables, _, _ = paged(g, rng, [64], 16, 1, 64, torch.float32, layers=2)
+    cache.k.copy_(normal(g, *cache.k.shape))
+    cache.v.copy_(cache.k + 1)
+    tables = tables[:, :4].contiguous()
+    tables[0, 3] = -1
+    table = tables[0].tolist()
+    before = cache.k.clone()
+    # from position 10: 3 -> 0; 2 does not ascend; 5 -> 2; 5 again; 2^31 - 1 and 60 are past; 6 is below itself
+    cache.keep(tables, i32([10]), i32([99]), i32([[3, 2, 5, 5, 40, 2**31 - 1, 6]]))
+    want = before.clone()
+
+    def move(w, x, a, b):
+        w[:, table[b // 16], :, b % 16] = x[:, table[a // 16], :, a % 16]
+    move(want, before, 13, 10)
+    move(want, before, 15, 12)
+    assert torch.equal(cache.k, want)
+    assert torch.equal(cache.v, want + 1)
+
+
+# ------------------------------------------------------------- streams and graphs
+
+def test_operators_on_a_side_stream_and_in_graphs():
+    """Each operator captured into a graph and replayed on new inputs; two graphs of
+    tree attention with workspaces of their own; a side stream while the default
+    stream is busy."""
+    g, rng = gen(40), np.random.default_rng(40)
+    dtype = torch.bfloat16
+    contexts, nodes = [500, 60], [6, 3]
+    cache, tables, keys, values = paged(g, rng, [506, 63], 16, 2, 64, dtype)
+    q, k, v = (normal(g, 9, h, 64, dtype=dtype) for h in (14, 2, 2))
+    visible = [b for t in nodes for b in random_tree(rng, t)]
+    plan, positions = ops.Rotary(64), i32(list(range(9)))
+    slots = i32([-1] * 9)
+    cs, offs, vis = i32(contexts), starts(nodes), masks(visible)
+    pairs = i32([[0, 1]]) * 0 - 1
+
+    def chain():
+        turned_q = plan.apply_to_cache(q, k, v, positions, cache, slots, layer=1)
+        tree = ops.tree_attention(turned_q, cache, tables, cs, offs, vis, layer=1)
+        kept = ops.prompt_attention(tree, k, v, offs)
+        cache.copy_pages(pairs)
+        cache.keep(tables, cs, i32_zero, nodes_zero)
+        return tree, kept
+
+    i32_zero, nodes_zero = i32([0, 0]), i32([[0], [0]])
+    want = [x.clone() for x in chain()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = chain()
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(chain())
+        graphs.append(graph)
+    fresh = normal(g, 9, 14, 64, dtype=dtype)
+    q.copy_(fresh)
+    graphs[0].replay()
+    graphs[1].replay()
+    torch.cuda.synchronize()
+    want = chain()
+    for out in outs:
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+# ---------------------------------------------------------------- the run of them
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_drafting_step_of_forked_sequences(dtype):
+    """Prompt, fork, drafted trees, kept paths and one more token: what every layer
+    attends to is what plain attention over the same tokens in a row gives."""
+    g = gen(50)
+    heads, kv_heads, dim, page, layers = 14, 2, 64, 16, 2
+    pool = ops.PagePool(64, page, 8)
+    cache = ops.PageCache.empty(layers, 64, kv_heads, page, dim, dtype)
+    cache.k.fill_(NAN)
+    cache.v.fill_(NAN)
+    plan = ops.Rotary(dim, scaling="yarn", factor=4.0, original_context=32768)
+    length = 57
+
+    def rows(n):
+        return tuple(normal(g, n, h, dim, dtype=dtype) for h in (heads, kv_heads, kv_heads))
+
+    def position(first, n):
+        return torch.arange(first, first + n, dtype=torch.int32, device="cuda")
+
+    # the prompt: turned into the cache, and attended from the packed rows
+    parent = pool.open()
+    assert pool.extend(parent, length) is None
+    q, k, v = rows(length)
+    for layer in range(layers):
+        tq = plan.apply_to_cache(q, k, v, position(0, length), cache, pool.slots(parent, 0, length), layer=layer)
+    tk = plan.apply(q, k, position(0, length))[1]
+    got = ops.prompt_attention(tq, tk, v, starts([length]))
+    check_heads(got, tq, tk, v, causal(length, length), dim ** -0.5, dtype)
+    # two forks of it draft: the shared last page is copied before it is written
+    seqs, paths, nodes = [parent, pool.fork(parent)], [[0, 2, 5], [1, 3]], [7, 4]
+    trees = [[1, 3, 5, 9, 17, 0b100101, 0b1000000], [1, 2, 5, 0b1010]]
+    pairs = [pool.extend(s, t) for s, t in zip(seqs, nodes)]
+    assert [p is None for p in pairs] == [False, True]
+    cache.copy_pages(i32([list(pairs[0])]))
+    drafts = [rows(t) for t in nodes]
+    dq, dk, dv = (torch.cat([d[i] for d in drafts]) for i in range(3))
+    depth = torch.cat([i32([bin(b).count("1") - 1 for b in tree]) for tree in trees])
+    slots = torch.cat([pool.slots(s, length, t) for s, t in zip(seqs, nodes)])
+    tables, contexts = pool.tables(seqs), i32([length, length])
+    visible = masks([b for tree in trees for b in tree])
+    for layer in range(layers):
+        tq = plan.apply_to_cache(dq, dk, dv, length + depth, cache, slots, layer=layer)
+    got = ops.tree_attention(tq, cache, tables, contexts, starts(nodes), visible, layer=1)
+    at = 0
+    for s, t in enumerate(nodes):
+        for i in range(t):  # each node against its path laid out in a row
+            path = [j for j in range(t) if trees[s][i] >> j & 1]
+            row_k = torch.cat([k, drafts[s][1][path]])
+            tk = plan.apply(torch.cat([q, drafts[s][0][path]]), row_k, position(0, length + len(path)))[1]
+            row_v = torch.cat([v, drafts[s][2][path]])
+            seen = torch.ones(1, length + len(path), dtype=torch.bool, device="cuda")
+            check_heads(got[at + i:at + i + 1], tq[at + i:at + i + 1], tk, row_v, seen, dim ** -0.5, dtype)
+        at += t
+    # the accepted paths stay, the rest of the pages goes back
+    width = max(len(p) for p in paths)
+    cache.keep(tables, contexts, i32([len(p) for p in paths]), i32([p + [0] * (width - len(p)) for p in paths]))
+    for s, path in zip(seqs, paths):
+        pool.truncate(s, length + len(path))
+    # compaction moves pages under the sequences
+    extra = pool.open()
+    pool.extend(extra, 5 * page)
+    hold = pool.fork(extra)
+    pool.free(extra)
+    pool.free(hold)
+    moves, used = pool.compact()
+    assert used + pool.free_pages() == 64
+    if moves:
+        cache.copy_pages(i32([list(m) for m in moves]))
+    assert all(p < used for s in seqs for p in pool.pages_of(s))
+    # one more token each, by plain decode
+    for s in seqs:
+        pair = pool.extend(s, 1)
+        assert pair is None
+    nq, nk, nv = rows(2)
+    ends = [length + len(p) for p in paths]
+    slots = torch.cat([pool.slots(s, e, 1) for s, e in zip(seqs, ends)])
+    for layer in range(layers):
+        tq = plan.apply_to_cache(nq, nk, nv, i32(ends), cache, slots, layer=layer)
+    for layer in range(layers):
+        got = ops.tree_attention(tq, cache, pool.tables(seqs), i32(ends), i32([0, 1, 2]), masks([1, 1]), layer=layer)
+        for s, path in enumerate(paths):
+            row_k = torch.cat([k, drafts[s][1][path], nk[s:s + 1]])
+            row_v = torch.cat([v, drafts[s][2][path], nv[s:s + 1]])
+            tk = plan.apply(row_k, row_k, position(0, ends[s] + 1))[1]
+            seen = torch.ones(1, ends[s] + 1, dtype=torch.bool, device="cuda")
+            check_heads(got[s:s + 1], tq[s:s + 1], tk, row_v, seen, dim ** -0.5, dtype)
+
+
+# ---------------------------------------------------------------------- refusals
+
+def test_refusals_launch_nothing():
+    q = torch.zeros(4, 2, 64, device="cuda")
+    k = torch.zeros(4, 1, 64, device="cuda")
+    with pytest.raises(ops.OperatorError, match="another type"):
+        ops.prompt_attention(q, k.half(), k.half(), i32([0, 4]))
+    with pytest.raises(ops.OperatorError, match="offsets"):
+        ops.prompt_attention(q, k, k, torch.tensor([0, 4], device="cuda"))
+    with pytest.raises(ops.OperatorError, match="head_dim must be"):
+        ops.prompt_attention(q[..., :32], k[..., :32], k[..., :32], i32([0, 4]))
+    with pytest.raises(ops.OperatorError, match="aligned") as e:
+        wide = torch.zeros(4, 2, 66, device="cuda")
+        ops.prompt_attention(wide[..., 1:65], k, k, i32([0, 4]))
+    assert e.value.status == 5
+    with pytest.raises(ops.OperatorError, match="multiple of kv_heads"):
+        ops.prompt_attention(torch.zeros(4, 3, 64, device="cuda"), torch.zeros(4, 2, 64, device="cuda"),
+                             torch.zeros(4, 2, 64, device="cuda"), i32([0, 4]))
+    with pytest.raises(ops.OperatorError, match="scale"):
+        ops.prompt_attention(q, k, k, i32([0, 4]), scale=NAN)
+    with pytest.raises(ops.OperatorError, match="kv_offsets"):
+        ops.prompt_attention(q, k[:3], k[:3], i32([0, 4]))
+    cache = ops.PageCache.empty(1, 4, 1, 16, 64, torch.float32)
+    args = (i32([[0, 1]]), i32([9]), i32([0, 1]), masks([1]))
+    with pytest.raises(ops.OperatorError, match="workspace"):
+        ops.tree_attention(q[:1], cache, *args, workspace=torch.empty(16, dtype=torch.uint8, device="cuda"))
+    with pytest.raises(ops.OperatorError, match="layer"):
+        ops.tree_attention(q[:1], cache, *args, layer=1)
+    with pytest.raises(ops.OperatorError, match="cache's type"):
+        ops.tree_attention(q[:1].half(), cache, *args)
+    with pytest.raises(ops.OperatorError, match="contiguous"):
+        ops.PageCache(cache.k.transpose(2, 3), cache.v.transpose(2, 3))
+    with pytest.raises(ops.OperatorError, match="strides"):
+        stack = torch.zeros(4, 6, 64, device="cuda")
+        ops.Rotary(64).apply(stack[:, :2], stack[:, 2:3], i32([0, 1, 2, 3]), q_out=stack.view(-1)[:512].view(4, 2, 64))
+    assert ops.prompt_attention(q[:0], k[:0], k[:0], i32([0, 0])).shape == (0, 2, 64)

@@ -1,0 +1,276 @@
+"""Host side of the paged serving operators: the C ABI's refusals, which come before
+anything touches a device, and the book of a cache's pages."""
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import pytest
+
+from promptboot_b200 import _lib
+
+torch = pytest.importorskip("torch")
+from promptboot_b200 import ops  # noqa: E402
+
+CAPACITY, ALIGNMENT, STATE = 4, 5, 1
+FAKE = 1 << 20  # an address that is only looked at
+
+
+def ref(x):
+    return ctypes.byref(x)
+
+
+def rows(data=FAKE, row=128, head=64):
+    return _lib.PbRows(data, row, head)
+
+
+def cache(**changes):
+    c = _lib.PbCache(FAKE, 2 * FAKE, 1 << 20, 2, 2, 8, 16, 2, 64)
+    for name, value in changes.items():
+        setattr(c, name, value)
+    return c
+
+
+def refused(status, want, text):
+    assert status == want and text in _lib.last_error(), (status, _lib.last_error())
+
+
+@pytest.mark.parametrize("changes,text", [
+    (dict(head_dim=60), "multiples of 16"), (dict(rotary_dim=72), "multiples of 16"),
+    (dict(rotary_dim=80), "rotary_dim <= head_dim"), (dict(head_dim=272, rotary_dim=16), "256"),
+    (dict(layout=2), "unknown"), (dict(scaling=4), "unknown"), (dict(theta=1.0), "theta"),
+    (dict(theta=float("nan")), "theta"), (dict(magnitude=-1.0), "magnitude"),
+    (dict(scaling=1, factor=0.5), "factor"), (dict(scaling=1, factor=float("inf")), "factor"),
+    (dict(scaling=2, original=0.0), "original"), (dict(scaling=3, low=8.0, high=4.0), "low < high"),
+    (dict(scaling=3, original=float("nan")), "original"),
+])
+def test_rotary_configurations_refused(changes, text):
+    c = _lib.PbRotaryConfig(64, 64, 0, 0, 1e4, 2.0, 4096.0, 0.0, 0.0, 0.0)
+    for name, value in changes.items():
+        setattr(c, name, value)
+    h = ctypes.c_void_p(1)
+    refused(_lib.load().pb_rotary_create(ref(c), ref(h)), CAPACITY, text)
+    assert not h.value
+
+
+def test_rotary_refusals():
+    lib, plan = _lib.load(), ops.Rotary(64)
+    q, k = rows(), rows()
+
+    def turn(type_=0, n=4, positions=FAKE, q=q, q_out=q, k_heads=2, k=k, k_out=k):
+        return lib.pb_rotary_device(plan._h, type_, n, positions, 2, q and ref(q), q_out and ref(q_out), k_heads,
+                                    k and ref(k), k_out and ref(k_out), None)
+    refused(turn(type_=3), CAPACITY, "type")
+    refused(turn(n=0), CAPACITY, "rows")
+    refused(turn(positions=None), CAPACITY, "NULL")
+    refused(turn(q=None), CAPACITY, "q is NULL")
+    refused(turn(k_out=None), CAPACITY, "k_out is NULL")
+    refused(turn(q=rows(FAKE + 4)), ALIGNMENT, "16-byte")
+    refused(turn(k=rows(row=130)), ALIGNMENT, "16-byte")
+    refused(turn(q_out=rows(row=256)), CAPACITY, "strides")
+
+    def store(c, layer=0, slots=FAKE, v=rows()):
+        return lib.pb_rotary_cache_device(plan._h, 4, FAKE, 2, ref(q), ref(q), ref(k), v and ref(v), ref(c), layer,
+                                          slots, None)
+    refused(store(cache(), layer=2), CAPACITY, "layer")
+    refused(store(cache(), slots=None), CAPACITY, "NULL")
+    refused(store(cache(), v=None), CAPACITY, "v is NULL")
+    refused(store(cache(head_dim=128, layer_stride=1 << 21)), CAPACITY, "head_dim")
+
+
+@pytest.mark.parametrize("changes,status,text", [
+    (dict(k=None), CAPACITY, "NULL"), (dict(type=7), CAPACITY, "type"), (dict(page_size=24), CAPACITY, "page_size"),
+    (dict(page_size=8), CAPACITY, "page_size"), (dict(page_size=512), CAPACITY, "page_size"),
+    (dict(pages=0), CAPACITY, "pages"), (dict(layers=0), CAPACITY, "layers"), (dict(kv_heads=0), CAPACITY, "heads"),
+    (dict(pages=1 << 27), CAPACITY, "2^31"), (dict(head_dim=72), CAPACITY, "head_dim"),
+    (dict(v=FAKE + 8), ALIGNMENT, "16-byte"), (dict(layer_stride=(1 << 20) + 4), ALIGNMENT, "16-byte"),
+    (dict(layer_stride=128), CAPACITY, "smaller"),
+])
+def test_caches_refused_by_every_operator(changes, status, text):
+    lib, c = _lib.load(), cache(**changes)
+    refused(lib.pb_cache_copy_pages_device(ref(c), 1, FAKE, None), status, text)
+    refused(lib.pb_cache_keep_device(ref(c), 1, FAKE, 1, FAKE, FAKE, FAKE, 1, None), status, text)
+    refused(lib.pb_tree_attention_device(ref(c), 0, 2, 1, 1, ref(rows()), ref(rows()), FAKE, 1, FAKE, FAKE, FAKE, 1.0,
+                                         FAKE, 1 << 40, None), status, text)
+
+
+def test_page_operations_without_work_or_arguments():
+    lib, c = _lib.load(), cache()
+    assert lib.pb_cache_copy_pages_device(ref(c), 0, None, None) == 0
+    assert lib.pb_cache_keep_device(ref(c), 0, None, 0, None, None, None, 0, None) == 0
+    refused(lib.pb_cache_copy_pages_device(ref(c), 1, None, None), CAPACITY, "NULL")
+    refused(lib.pb_cache_keep_device(ref(c), 1, FAKE, 0, FAKE, FAKE, FAKE, 1, None), CAPACITY, "empty table")
+    refused(lib.pb_cache_keep_device(ref(c), 1, FAKE, 1, FAKE, None, FAKE, 1, None), CAPACITY, "NULL")
+
+
+def test_prompt_attention_refusals():
+    lib = _lib.load()
+
+    def prompt(type_=2, dim=64, heads=4, kv_heads=2, seqs=1, n=8, kv_n=8, q=rows(), k=rows(), out=rows(), offsets=FAKE,
+               kv_offsets=FAKE, scale=1.0):
+        return lib.pb_prompt_attention_device(type_, dim, heads, kv_heads, seqs, n, kv_n, q and ref(q), ref(k), ref(k),
+                                              ref(out), offsets, kv_offsets, scale, None)
+    refused(prompt(type_=9), CAPACITY, "type")
+    for dim in (0, 32, 96, 256):
+        refused(prompt(dim=dim), CAPACITY, "head_dim")
+    refused(prompt(heads=3), CAPACITY, "multiple of kv_heads")
+    refused(prompt(kv_heads=0), CAPACITY, "multiple of kv_heads")
+    refused(prompt(seqs=0), CAPACITY, "sequences")
+    refused(prompt(seqs=2049), CAPACITY, "sequences")
+    refused(prompt(n=1 << 29), CAPACITY, "2^30")
+    refused(prompt(kv_n=1 << 30), CAPACITY, "2^30")
+    for scale in (0.0, -1.0, float("inf"), float("nan")):
+        refused(prompt(scale=scale), CAPACITY, "scale")
+    refused(prompt(kv_offsets=None, kv_n=9), CAPACITY, "kv_offsets")
+    refused(prompt(offsets=None), CAPACITY, "q_offsets")
+    refused(prompt(q=None), CAPACITY, "q is NULL")
+    refused(prompt(out=rows(head=68)), ALIGNMENT, "out")
+    assert prompt(n=0) == 0
+
+
+def test_tree_attention_refusals():
+    lib = _lib.load()
+
+    def tree(c=cache(), layer=0, heads=4, seqs=1, n=8, q=rows(), tables=FAKE, width=4, visible=FAKE, work=FAKE,
+             size=1 << 40):
+        return lib.pb_tree_attention_device(ref(c), layer, heads, seqs, n, q and ref(q), ref(rows()), tables, width,
+                                            FAKE, FAKE, visible, 1.0, work, size, None)
+    refused(tree(layer=2), CAPACITY, "layer")
+    refused(tree(c=cache(head_dim=32)), CAPACITY, "head_dim must be 64 or 128")
+    refused(tree(heads=5), CAPACITY, "multiple of kv_heads")
+    refused(tree(q=None), CAPACITY, "q is NULL")
+    refused(tree(tables=None), CAPACITY, "NULL")
+    refused(tree(width=0), CAPACITY, "empty table")
+    refused(tree(visible=None), CAPACITY, "NULL")
+    refused(tree(width=1 << 28), CAPACITY, "reach too far")
+    refused(tree(width=1 << 25, seqs=2048), CAPACITY, "reach too far")
+    refused(tree(work=None), CAPACITY, "workspace")
+    refused(tree(size=64), CAPACITY, "workspace")
+    refused(tree(work=FAKE + 8), ALIGNMENT, "workspace")
+    assert tree(n=0) == 0
+    assert lib.pb_tree_attention_workspace(2, 96, 4, 2, 1, 8) == 0
+
+
+def test_wrappers_refuse_tensors_off_the_gpu():
+    x = torch.zeros(4, 2, 64)
+    with pytest.raises(ops.OperatorError, match="CUDA"):
+        ops.prompt_attention(x, x, x, torch.zeros(2, dtype=torch.int32))
+    with pytest.raises(ops.OperatorError, match="CUDA"):
+        ops.PageCache(torch.zeros(1, 2, 1, 16, 64), torch.zeros(1, 2, 1, 16, 64))
+    with pytest.raises(ops.OperatorError, match="scaling"):
+        ops.Rotary(64, scaling="ntk")
+
+
+# ---------------------------------------------------------------- the book of pages
+
+def test_pool_shares_pages_until_one_sequence_writes():
+    pool = ops.PagePool(8, 16, 3)
+    a = pool.open()
+    assert pool.extend(a, 20) is None and pool.pages_of(a) == [0, 1] and pool.length(a) == 20
+    b = pool.fork(a)
+    assert pool.pages_of(b) == [0, 1] and pool.free_pages() == 6
+    assert pool.extend(b, 0) is None and pool.pages_of(b) == [0, 1]  # nothing will be written
+    pair = pool.extend(b, 1)
+    assert pair == (1, 2) and pool.pages_of(b) == [0, 2] and pool.pages_of(a) == [0, 1]
+    assert pool.extend(a, 1) is None  # its last page is its own again
+    pool.truncate(b, 16)
+    assert pool.pages_of(b) == [0] and pool.free_pages() == 6
+    assert pool.extend(b, 1) is None  # a full shared page needs no copy
+    pool.free(a)
+    assert pool.free_pages() == 6 and pool.pages_of(b)[0] == 0
+    pool.free(b)
+    assert pool.free_pages() == 8
+
+
+def test_pool_refusals_change_nothing():
+    pool = ops.PagePool(4, 16, 2)
+    a = pool.open()
+    pool.extend(a, 40)
+    for _ in range(2):
+        with pytest.raises(ops.OperatorError, match="too few free pages"):
+            pool.extend(a, 25)
+        assert pool.pages_of(a) == [0, 1, 2] and pool.length(a) == 40 and pool.free_pages() == 1
+    b = pool.fork(a)
+    with pytest.raises(ops.OperatorError, match="too few free pages"):
+        pool.extend(b, 10)  # one new page and the copy of the shared last one
+    assert pool.pages_of(b) == [0, 1, 2] and pool.length(b) == 40
+    with pytest.raises(ops.OperatorError, match="every sequence is open"):
+        pool.fork(a)
+    with pytest.raises(ops.OperatorError, match="shorter"):
+        pool.truncate(a, 41)
+    with pytest.raises(ops.OperatorError, match="has 40 tokens"):
+        pool.slots(a, 30, 11, device="cpu")
+    with pytest.raises(ops.OperatorError) as e:
+        pool.free(7)
+    assert e.value.status == STATE
+    pool.free(b)
+    with pytest.raises(ops.OperatorError, match="not open"):
+        pool.free(b)
+    with pytest.raises(ops.OperatorError, match="too few"):
+        pool.extend(a, 2**32 - 1)
+    for bad in ((0, 16, 1), (4, 0, 1), (4, 16, 0), (1 << 27, 16, 1)):
+        with pytest.raises(ops.OperatorError):
+            ops.PagePool(*bad)
+
+
+def test_pool_short_arrays_are_refused_with_the_number_needed():
+    lib, pool = _lib.load(), ops.PagePool(8, 16, 2)
+    a, b = pool.open(), pool.open()
+    pool.extend(a, 40)
+    pool.extend(b, 40)
+    table, length, needed = (ctypes.c_uint32 * 4)(), ctypes.c_uint32(), ctypes.c_uint32()
+    refused(lib.pb_pool_table(pool._h, a, table, 2, ref(length), ref(needed)), CAPACITY, "too short")
+    assert needed.value == 3
+    assert lib.pb_pool_table(pool._h, a, table, 4, ref(length), ref(needed)) == 0
+    assert list(table) == [0, 1, 2, 0xFFFFFFFF] and length.value == 40
+    pool.free(a)
+    n, used = ctypes.c_uint32(), ctypes.c_uint32()
+    refused(lib.pb_pool_compact(pool._h, table, 2, ref(n), ref(used), ref(needed)), CAPACITY, "too short")
+    assert needed.value == 3 and pool.pages_of(b) == [3, 4, 5]
+
+
+def test_pool_against_a_plain_book():
+    """Random opens, forks, writes, cuts and compactions, with the tokens of every
+    sequence held in a plain list beside the pages."""
+    rng = np.random.default_rng(0)
+    page, pages = 4, 24
+    pool, memory, books, fresh = ops.PagePool(pages, page, 6), np.zeros((pages, page), int), {}, iter(range(1, 10**6))
+    for _ in range(4000):
+        what = rng.integers(0, 6)
+        seq = int(rng.choice(list(books))) if books else None
+        try:
+            if what == 0 or seq is None:
+                books[pool.open()] = []
+            elif what == 1:
+                child = pool.fork(seq)
+                books[child] = list(books[seq])
+            elif what == 2 and rng.random() < 0.5:
+                pool.free(seq)
+                del books[seq]
+            elif what == 3:
+                cut = int(rng.integers(0, len(books[seq]) + 1))
+                pool.truncate(seq, cut)
+                del books[seq][cut:]
+            elif what == 4 and rng.random() < 0.2:
+                moves, used = pool.compact()
+                assert len({t for _, t in moves} | {f for f, _ in moves}) == 2 * len(moves)
+                for a, b in moves:
+                    memory[b] = memory[a]
+                assert all(p < used for s in books for p in pool.pages_of(s)) and used == pages - pool.free_pages()
+            else:
+                tokens = [next(fresh) for _ in range(int(rng.integers(0, 11)))]
+                pair = pool.extend(seq, len(tokens))
+                if pair:
+                    memory[pair[1]] = memory[pair[0]]
+                start = len(books[seq])
+                books[seq] += tokens
+                for slot, token in zip(pool.slots(seq, start, len(tokens), device="cpu").tolist(), tokens):
+                    memory[slot // page, slot % page] = token
+        except ops.OperatorError as e:
+            assert e.status == CAPACITY
+        for s, tokens in books.items():
+            ids = pool.pages_of(s)
+            assert pool.length(s) == len(tokens) and len(ids) == -(-len(tokens) // page)
+            assert [memory[ids[i // page], i % page] for i in range(len(tokens))] == tokens
+    used = {p for s in books for p in pool.pages_of(s)}
+    assert pool.free_pages() == pages - len(used)
