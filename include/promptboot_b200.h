@@ -408,6 +408,10 @@ PB_API uint32_t pb_tree_attention_device(const pb_cache *cache, uint32_t layer, 
                                          const uint64_t *visible_device, float scale,
                                          void *workspace, uint64_t workspace_bytes, void *stream);
 
+/* Waits for `stream` and reports a prompt or tree attention whose kernel gave up
+ * waiting for a copy or a product (PB_DEVICE, once; its outputs are not complete). */
+PB_API uint32_t pb_attention_status(void *stream);
+
 /* Copies page pairs[2 i] to page pairs[2 i + 1] for i < n, keys and values of
  * every layer.  No page may be the target of two pairs or the target of one and
  * the source of another.  Pairs with a page outside the cache are left out. */

@@ -147,6 +147,7 @@ SIGNATURES = {
     "pb_tree_attention_workspace": (u64, [u32, u32, u32, u32, u32, u32]),
     "pb_tree_attention_device": (u32, [C, u32, u32, u32, u32, R, R, P, u32, P, P, P,
                                        ctypes.c_float, P, u64, P]),
+    "pb_attention_status": (u32, [P]),
     "pb_cache_copy_pages_device": (u32, [C, u32, P, P]),
     "pb_cache_keep_device": (u32, [C, u32, P, u32, P, P, P, u32, P]),
     "pb_pool_create": (u32, [u32, u32, u32, ctypes.POINTER(P)]),

@@ -64,6 +64,8 @@ uint32_t pb_prompt_attention_device(uint32_t type, uint32_t head_dim, uint32_t q
   if ((st = pb::paged::check_rows(k, bytes, who, "k"))) return st;
   if ((st = pb::paged::check_rows(v, bytes, who, "v"))) return st;
   if ((st = pb::paged::check_rows(out, bytes, who, "out"))) return st;
+  if (kv_rows > 1 && (!k->row_stride || !v->row_stride))
+    return refuse(PB_CAPACITY, who, "k and v need a row stride");
   pb::paged::AttnArgs a{};
   a.q = *q; a.k = *k; a.v = *v; a.out = *out;
   a.q_offsets = q_offsets;
@@ -71,13 +73,15 @@ uint32_t pb_prompt_attention_device(uint32_t type, uint32_t head_dim, uint32_t q
   a.seqs = seqs; a.q_rows = q_rows; a.kv_rows = kv_rows;
   a.kv_heads = kv_heads; a.group = q_heads / kv_heads;
   a.scale_log2 = scale * pb::paged::kLog2E;
-  return pb::paged::simt_prompt(a, type, head_dim, (cudaStream_t)stream);
+  if (bytes == 2) return pb::paged::tc_prompt(a, type, head_dim, (cudaStream_t)stream);
+  return pb::paged::simt_prompt(a, head_dim, (cudaStream_t)stream);
 }
 
 uint64_t pb_tree_attention_workspace(uint32_t type, uint32_t head_dim, uint32_t q_heads,
                                      uint32_t kv_heads, uint32_t seqs, uint32_t rows) {
   if (pb::paged::check_heads("pb_tree_attention_workspace", type, head_dim, q_heads, kv_heads, seqs, rows))
     return 0;
+  if (pb::paged::type_bytes(type) == 2) return pb::paged::tc_tree_words(head_dim) * 4;
   return pb::paged::simt_tree_words(head_dim, rows * (q_heads / kv_heads), seqs) * 4;
 }
 
@@ -119,7 +123,10 @@ uint32_t pb_tree_attention_device(const pb_cache* cache, uint32_t layer, uint32_
   a.kv_heads = cache->kv_heads; a.group = (uint32_t)group; a.table_width = table_width;
   a.scale_log2 = scale * pb::paged::kLog2E;
   a.partial = static_cast<float*>(workspace);
-  return pb::paged::simt_tree(a, cache->type, cache->head_dim, (cudaStream_t)stream);
+  if (bytes == 2) return pb::paged::tc_tree(a, cache->type, cache->head_dim, (cudaStream_t)stream);
+  return pb::paged::simt_tree(a, cache->head_dim, (cudaStream_t)stream);
 }
+
+uint32_t pb_attention_status(void* stream) { return pb::paged::tc_status((cudaStream_t)stream); }
 
 }  // extern "C"

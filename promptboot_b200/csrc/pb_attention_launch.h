@@ -10,10 +10,17 @@ namespace paged {
 uint32_t tree_ctas(uint32_t per_sm);
 
 // Prompt attention; tree attention and the words of its workspace, for rows =
-// q_rows * group.
-uint32_t simt_prompt(const AttnArgs& a, uint32_t type, uint32_t head_dim, cudaStream_t s);
-uint32_t simt_tree(const AttnArgs& a, uint32_t type, uint32_t head_dim, cudaStream_t s);
+// q_rows * group: binary32 elements on the CUDA cores.
+uint32_t simt_prompt(const AttnArgs& a, uint32_t head_dim, cudaStream_t s);
+uint32_t simt_tree(const AttnArgs& a, uint32_t head_dim, cudaStream_t s);
 uint64_t simt_tree_words(uint32_t head_dim, uint32_t rows, uint32_t seqs);
+
+// The same on the tensor cores, for 16-bit elements; whether a wait of theirs gave
+// up since the last look (waits for the stream).
+uint32_t tc_prompt(const AttnArgs& a, uint32_t type, uint32_t head_dim, cudaStream_t s);
+uint32_t tc_tree(const AttnArgs& a, uint32_t type, uint32_t head_dim, cudaStream_t s);
+uint64_t tc_tree_words(uint32_t head_dim);
+uint32_t tc_status(cudaStream_t s);
 
 }  // namespace paged
 }  // namespace pb

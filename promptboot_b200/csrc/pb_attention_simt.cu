@@ -1,5 +1,5 @@
-// Paged serving attention on the CUDA cores, with every product and sum in
-// binary32.
+// Paged serving attention of binary32 elements on the CUDA cores, with every product
+// and sum in binary32.
 //
 // One pass over the keys per row with a running maximum m and sum l (Milakov and
 // Gimelshein's online softmax): for a tile of scores x (in powers of two),
@@ -28,17 +28,13 @@ struct Simt {
   static size_t bytes(uint32_t seqs) { return (size_t)(kWords + seqs) * 4; }
 };
 
-// kN elements of a row as binary32 at `dst`, from 16 bytes at `src` (zeros: NULL).
-template <class T>
-__device__ __forceinline__ void fill(float* dst, const T* src) {
-  float x[Elements<T>::n] = {};
-  if (src) Elements<T>::load(*reinterpret_cast<const uint4*>(src), x);
-#pragma unroll
-  for (int i = 0; i < Elements<T>::n; i += 4)
-    *reinterpret_cast<float4*>(dst + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+// Four elements at `dst` from `src` (zeros: NULL).
+__device__ __forceinline__ void fill(float* dst, const float* src) {
+  *reinterpret_cast<float4*>(dst) =
+      src ? *reinterpret_cast<const float4*>(src) : make_float4(0.f, 0.f, 0.f, 0.f);
 }
 
-template <class T, int kDim, int kRpt, bool kTree>
+template <int kDim, int kRpt, bool kTree>
 __global__ void __launch_bounds__(kThreads) attention_simt_kernel(const __grid_constant__ AttnArgs a) {
   using C = Simt<kDim, kRpt>;
   constexpr int kRows = C::kRows, kKeys = C::kKeys, kKpt = C::kKpt, kCols = kDim / 64;
@@ -90,13 +86,13 @@ __global__ void __launch_bounds__(kThreads) attention_simt_kernel(const __grid_c
     }
 
     __syncthreads();  // the piece before is done with shared memory
-    constexpr int kWord = Elements<T>::n, kWords = kDim / kWord;
+    constexpr int kWords = kDim / 4;
     for (int i = threadIdx.x; i < kRows * kWords; i += kThreads) {
-      const int r = i / kWords, c = i % kWords * kWord;
+      const int r = i / kWords, c = i % kWords * 4;
       const uint32_t row = p.row_tile * kRows + r;
-      const T* src = nullptr;
+      const float* src = nullptr;
       if (row < rows)
-        src = static_cast<const T*>(a.q.data) + (uint64_t)(s.q0 + row / a.group) * a.q.row_stride +
+        src = static_cast<const float*>(a.q.data) + (uint64_t)(s.q0 + row / a.group) * a.q.row_stride +
               (uint64_t)(p.head * a.group + row % a.group) * a.q.head_stride + c;
       fill(qs + r * C::kPad + c, src);
     }
@@ -122,22 +118,22 @@ __global__ void __launch_bounds__(kThreads) attention_simt_kernel(const __grid_c
       const uint32_t key0 = tile * kKeys;
       __syncthreads();
       for (int i = threadIdx.x; i < kKeys * kWords; i += kThreads) {
-        const int j = i / kWords, c = i % kWords * kWord;
+        const int j = i / kWords, c = i % kWords * 4;
         const uint32_t key = key0 + j;
-        const T *kw = nullptr, *vw = nullptr;
+        const float *kw = nullptr, *vw = nullptr;
         if (key < s.len) {
           if (kTree) {
             const uint32_t page = a.tables[(uint64_t)p.seq * a.table_width + key / a.cache.page_size];
             if (page < a.cache.pages) {
               const uint64_t at = (((uint64_t)page * a.cache.kv_heads + p.head) * a.cache.page_size +
                                    key % a.cache.page_size) * kDim + c;
-              kw = reinterpret_cast<const T*>(a.cache.k) + at;
-              vw = reinterpret_cast<const T*>(a.cache.v) + at;
+              kw = reinterpret_cast<const float*>(a.cache.k) + at;
+              vw = reinterpret_cast<const float*>(a.cache.v) + at;
             }
           } else {
             const uint64_t row = s.kv0 + key;
-            kw = static_cast<const T*>(a.k.data) + row * a.k.row_stride + p.head * a.k.head_stride + c;
-            vw = static_cast<const T*>(a.v.data) + row * a.v.row_stride + p.head * a.v.head_stride + c;
+            kw = static_cast<const float*>(a.k.data) + row * a.k.row_stride + p.head * a.k.head_stride + c;
+            vw = static_cast<const float*>(a.v.data) + row * a.v.row_stride + p.head * a.v.head_stride + c;
           }
         }
         fill(ks + j * C::kPad + c, kw);
@@ -250,7 +246,7 @@ __global__ void __launch_bounds__(kThreads) attention_simt_kernel(const __grid_c
         }
       } else {
         const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
-        T* out = static_cast<T*>(a.out.data) + (uint64_t)(s.q0 + row / a.group) * a.out.row_stride +
+        float* out = static_cast<float*>(a.out.data) + (uint64_t)(s.q0 + row / a.group) * a.out.row_stride +
                  (uint64_t)(p.head * a.group + row % a.group) * a.out.head_stride;
 #pragma unroll
         for (int c = 0; c < kCols; ++c)
@@ -261,10 +257,10 @@ __global__ void __launch_bounds__(kThreads) attention_simt_kernel(const __grid_c
   }
 }
 
-template <class T, int kDim, int kRpt, bool kTree>
+template <int kDim, int kRpt, bool kTree>
 uint32_t launch(const AttnArgs& a, uint32_t grid, cudaStream_t s) {
   using C = Simt<kDim, kRpt>;
-  auto kernel = attention_simt_kernel<T, kDim, kRpt, kTree>;
+  auto kernel = attention_simt_kernel<kDim, kRpt, kTree>;
   static std::atomic<uint64_t> configured{0};
   if (attribute_needed(configured)) {
     PB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -275,7 +271,7 @@ uint32_t launch(const AttnArgs& a, uint32_t grid, cudaStream_t s) {
   PB_CUDA(cudaGetLastError());
   if (kTree) {
     const dim3 join(std::min<uint32_t>(grid, 1024), C::kRows >= 32 ? 4 : 1);
-    combine_kernel<T, kDim, C::kRows, C::kKeys, kLeast><<<join, 256, a.seqs * 4, s>>>(a, grid);
+    combine_kernel<float, kDim, C::kRows, C::kKeys, kLeast><<<join, 256, a.seqs * 4, s>>>(a, grid);
     PB_CUDA(cudaGetLastError());
   }
   return PB_OK;
@@ -285,18 +281,10 @@ constexpr int kFewRpt = 2, kManyRpt = 8;  // 16 or 64 rows of a tile
 
 }  // namespace
 
-template <class T>
-static uint32_t prompt(const AttnArgs& a, uint32_t head_dim, cudaStream_t s) {
+uint32_t simt_prompt(const AttnArgs& a, uint32_t head_dim, cudaStream_t s) {
   const uint32_t rows = a.q_rows * a.group;
   const uint32_t grid = (rows / (8 * kManyRpt) + a.seqs) * a.kv_heads;
-  return head_dim == 64 ? launch<T, 64, kManyRpt, false>(a, grid, s)
-                        : launch<T, 128, kManyRpt, false>(a, grid, s);
-}
-
-uint32_t simt_prompt(const AttnArgs& a, uint32_t type, uint32_t head_dim, cudaStream_t s) {
-  if (type == PB_TYPE_F32) return prompt<float>(a, head_dim, s);
-  if (type == PB_TYPE_F16) return prompt<__half>(a, head_dim, s);
-  return prompt<__nv_bfloat16>(a, head_dim, s);
+  return head_dim == 64 ? launch<64, kManyRpt, false>(a, grid, s) : launch<128, kManyRpt, false>(a, grid, s);
 }
 
 // Row tiles of 16 where a sequence has no more rows than that on average.
@@ -307,20 +295,11 @@ uint64_t simt_tree_words(uint32_t head_dim, uint32_t rows, uint32_t seqs) {
   return (uint64_t)tree_ctas(4) * 2 * tile * (head_dim + 2);
 }
 
-template <class T>
-static uint32_t tree(const AttnArgs& a, uint32_t head_dim, cudaStream_t s) {
+uint32_t simt_tree(const AttnArgs& a, uint32_t head_dim, cudaStream_t s) {
   const uint32_t grid = tree_ctas(4);
   if (few(a.q_rows * a.group, a.seqs))
-    return head_dim == 64 ? launch<T, 64, kFewRpt, true>(a, grid, s)
-                          : launch<T, 128, kFewRpt, true>(a, grid, s);
-  return head_dim == 64 ? launch<T, 64, kManyRpt, true>(a, grid, s)
-                        : launch<T, 128, kManyRpt, true>(a, grid, s);
-}
-
-uint32_t simt_tree(const AttnArgs& a, uint32_t type, uint32_t head_dim, cudaStream_t s) {
-  if (type == PB_TYPE_F32) return tree<float>(a, head_dim, s);
-  if (type == PB_TYPE_F16) return tree<__half>(a, head_dim, s);
-  return tree<__nv_bfloat16>(a, head_dim, s);
+    return head_dim == 64 ? launch<64, kFewRpt, true>(a, grid, s) : launch<128, kFewRpt, true>(a, grid, s);
+  return head_dim == 64 ? launch<64, kManyRpt, true>(a, grid, s) : launch<128, kManyRpt, true>(a, grid, s);
 }
 
 }  // namespace paged

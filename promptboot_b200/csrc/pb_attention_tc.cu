@@ -1,0 +1,675 @@
+// Paged serving attention on the 5th-generation tensor cores (tcgen05, kind::f16)
+// for binary16 and bfloat16: prompts, and trees with many rows per sequence.
+//
+// A CTA walks the keys of one row tile (128 rows) in tiles of kKeys, with the
+// online softmax of pb_attention_simt.cu in binary32:
+//   S = Q K^T (both from shared memory, S in TMEM),  P = 2^(S c - m) rounded to
+//   the type of V (into TMEM),  O += P V (P from TMEM, V from shared memory).
+// The weights' sum adds the unrounded weights, so P's rounding is one more half
+// step of the type per weight and averages out over the keys.
+//
+// Warps: 0..3 softmax, one row per thread (TMEM lane = row); 4 issues the MMAs;
+// 5 brings K and V tiles by TMA (128-byte swizzle) into rings of kStages.  S, P and
+// O have TMEM columns of their own, 256 in all, so two CTAs share an SM and one's
+// products run under the other's exponentials; and no MMA of a tile depends on the
+// order of two MMAs of different shapes.
+//
+// The running maximum is the one in use until a row's true maximum passes it by
+// 2^kSlack: O is rescaled (through registers) only then, seldom after the first
+// tiles.  Weights may then reach 2^kSlack; binary16 weights are also raised by
+// 2^kRaise, so that those far below the maximum keep their bits.
+//
+// Masked tiles (a key that some row of the tile does not see): scores are replaced
+// by -inf; value rows past the keys are zeroed in shared memory; values that are
+// not finite are taken out there, and added to the rows that see them at the end.
+#include "pb_attention_launch.h"
+#include "pb_kernels.cuh"
+#include "pb_tcgen05.cuh"
+
+#include <cuda.h>
+
+namespace pb {
+namespace paged {
+
+// Set where a bounded wait of this file's kernels gave up; read and cleared by
+// tc_status.
+static __device__ unsigned int g_tc_status;
+
+namespace {
+
+constexpr int kThreads = 192;
+constexpr int kRows = 128;
+constexpr int kLeast = 2;
+
+template <class T>
+struct Format;
+template <>
+struct Format<__half> {
+  static constexpr uint32_t kCode = 0;  // instruction descriptor
+  static constexpr CUtensorMapDataType kMap = CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  static constexpr float kSlack = 4.f, kRaise = 10.f;  // weights stay below 2^14 of 65504
+  static constexpr uint32_t kExponents = 0x7c007c00u;
+};
+template <>
+struct Format<__nv_bfloat16> {
+  static constexpr uint32_t kCode = 1;
+  static constexpr CUtensorMapDataType kMap = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  static constexpr float kSlack = 8.f, kRaise = 0.f;
+  static constexpr uint32_t kExponents = 0x7f807f80u;
+};
+
+template <int kDim>
+struct Tc {
+  static constexpr int kKeys = kDim == 64 ? 128 : 64;
+  static constexpr int kStages = 2;
+  static constexpr int kHalves = kDim / 64;           // 128-byte column blocks of a row
+  static constexpr int kQBlock = kRows * 128;
+  static constexpr int kBlock = kKeys * 128;          // one column block of a K or V tile
+  static constexpr int kTile = kHalves * kBlock;
+  static constexpr int kKOff = kHalves * kQBlock;
+  static constexpr int kVOff = kKOff + kStages * kTile;
+  static constexpr int kBarOff = kVOff + kStages * kTile;
+  static constexpr int kBars = 4 * kStages + 4;
+  static constexpr int kPrefixOff = kBarOff + kBars * 8 + 16;
+  static constexpr int kSCol = 0, kPCol = kKeys, kOCol = kKeys + kKeys / 2;
+  static constexpr int kCols = 256;
+  static_assert(kOCol + kDim <= kCols, "TMEM columns");
+  static size_t bytes(uint32_t seqs) { return 1024 + kPrefixOff + (size_t)seqs * 4; }
+};
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+        "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+        "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+      ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+        "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
+        "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
+        "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+      ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+        "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+// Waits for this thread's TMEM loads; the registers pass through, so that nothing
+// that uses them moves up.
+__device__ __forceinline__ void tmem_wait_ld32(uint32_t (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                 "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]),
+                 "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]),
+                 "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]),
+                 "+r"(v[30]), "+r"(v[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// TMA tile loads: the innermost coordinate is 0 or 64 elements (128 bytes).
+__device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tma_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+      ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// Shared-memory matrix descriptor, 128-byte swizzle (8 rows of 128 bytes repeat):
+// stride 1024 bytes between 8-row groups.  `lead`: bytes between 64-element column
+// blocks of an N-major operand (V); unused by K-major ones (Q, K).
+__device__ __forceinline__ uint64_t desc128(uint32_t addr, uint32_t lead) {
+  return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Which of the 32 keys from `key` on a row sees.
+__device__ __forceinline__ uint32_t seen32(const RowView& r, uint32_t key) {
+  const uint32_t below = r.all > key ? r.all - key : 0;
+  if (below >= 32) return 0xffffffffu;
+  uint32_t m = (1u << below) - 1u;
+  if (key >= r.all) {
+    const uint32_t at = key - r.all;
+    if (at < 64) m |= (uint32_t)(r.bits >> at);
+  } else {
+    m |= (uint32_t)(r.bits << below);
+  }
+  return m;
+}
+
+struct Maps {
+  CUtensorMap k, v;
+  uint32_t k_step, v_step;  // 0: one key head's rows serve all
+};
+
+template <class T, int kDim, bool kTree>
+__global__ void __launch_bounds__(kThreads, 2)
+attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Maps maps) {
+  using C = Tc<kDim>;
+  using F = Format<T>;
+  constexpr int kKeys = C::kKeys, kStages = C::kStages, kHalves = C::kHalves;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
+  uint64_t* k_empty = k_full + kStages;
+  uint64_t* v_full = k_empty + kStages;
+  uint64_t* v_empty = v_full + kStages;
+  uint64_t* q_full = v_empty + kStages;
+  uint64_t* s_full = q_full + 1;
+  uint64_t* p_full = s_full + 1;
+  uint64_t* o_full = p_full + 1;  // O holds the tile's products, P is free
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* dirty = abort_flag + 1;  // the last piece with a value that was taken out
+  uint32_t* prefix = reinterpret_cast<uint32_t*>(smem + C::kPrefixOff);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  work_prefix<kTree, kRows, kKeys, kThreads>(a, prefix);
+  const uint32_t total = prefix[a.seqs - 1];
+  uint32_t next, end;
+  if (kTree) {
+    if (total == 0) return;
+    const Share<kLeast> share(total, gridDim.x);
+    if (blockIdx.x >= share.ctas) return;
+    next = share.start(blockIdx.x);
+    end = share.start(blockIdx.x + 1);
+  } else {
+    if (blockIdx.x >= total) return;
+    next = blockIdx.x;
+    end = next + 1;
+  }
+
+  if (warp == 4) tmem_alloc(tmem_slot, C::kCols);
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
+    }
+    mbar_init(q_full, kRows);
+    mbar_init(s_full, 1);
+    mbar_init(p_full, kRows);
+    mbar_init(o_full, 1);
+    *abort_flag = 0;
+    *dirty = 0;
+    fence_barrier_init();
+  }
+  tc_before_sync();
+  __syncthreads();
+  tc_after_sync();
+  const uint32_t tmem = *tmem_slot;
+
+  // The CTA's pieces, decoded alike by every role.
+  Sequence s;
+  uint32_t rows, row_tiles;
+  auto take = [&](Piece& p) {
+    uint32_t x = next;
+    p.seq = find_sequence(prefix, a.seqs, x);
+    s = load_sequence<kTree>(a, p.seq);
+    rows = s.t * a.group;
+    row_tiles = ceil_div(rows, kRows);
+    p.partial = -1;
+    if (kTree) {
+      const uint32_t tiles = max(1u, ceil_div(s.len, kKeys));
+      p.tile0 = x % tiles;
+      p.tile1 = min(tiles, p.tile0 + (end - next));
+      p.head = x / tiles / row_tiles;
+      p.row_tile = x / tiles % row_tiles;
+      if (p.tile0 > 0 || p.tile1 < tiles) p.partial = partial_of(blockIdx.x, p.tile0 == 0);
+      next += p.tile1 - p.tile0;
+      if (s.len == 0) p.tile1 = p.tile0 = 0;  // nothing to see
+    } else {
+      p.head = x % a.kv_heads;
+      p.row_tile = row_tiles - 1 - x / a.kv_heads;
+      const uint32_t last = min(rows, (p.row_tile + 1) * kRows) - 1;
+      p.tile0 = 0;
+      p.tile1 = ceil_div(row_view<false>(a, s, last / a.group).all, kKeys);
+      ++next;
+    }
+  };
+
+  int k_issued = 0, v_issued = 0, o_commits = 0;  // for the way out
+
+  if (warp == 5) {
+    bool stop = false;
+    int q = 0;  // tiles so far
+    while (next < end && !stop) {
+      Piece p;
+      take(p);
+      const uint32_t size = kTree ? min(a.cache.page_size, (uint32_t)kKeys) : kKeys;  // rows of a box
+      for (uint32_t tile = p.tile0; tile < p.tile1 && !stop; ++tile, ++q) {
+        const int st = q % kStages;
+        const uint32_t key = tile * kKeys + lane * size;  // this lane's box
+        const uint32_t boxes = min((uint32_t)kKeys / size, ceil_div(s.len - tile * kKeys, size));
+        int page = 0;
+        if (kTree && (uint32_t)lane < boxes)
+          page = (int)a.tables[(uint64_t)p.seq * a.table_width + key / a.cache.page_size];
+        uint8_t* kt = smem + C::kKOff + st * C::kTile + lane * size * 128;
+        uint8_t* vt = smem + C::kVOff + st * C::kTile + lane * size * 128;
+        auto bring = [&](uint8_t* to, const CUtensorMap* map, uint32_t step, uint64_t* bar) {
+          if (lane == 0) mbar_expect_tx(bar, boxes * size * kHalves * 128);
+          __syncwarp();
+          if ((uint32_t)lane < boxes) {
+#pragma unroll
+            for (int c = 0; c < kHalves; ++c) {
+              if (kTree)
+                tma_4d(to + c * C::kBlock, map, c * 64, (int)(key % a.cache.page_size), (int)p.head, page, bar);
+              else
+                tma_3d(to + c * C::kBlock, map, c * 64, (int)(s.kv0 + key), (int)(p.head * step), bar);
+            }
+          }
+        };
+        if (!wait_warp(&k_empty[st], ((q / kStages) & 1) ^ 1, abort_flag)) { stop = true; break; }
+        bring(kt, &maps.k, maps.k_step, &k_full[st]);
+        k_issued = q + 1;
+        if (!wait_warp(&v_empty[st], ((q / kStages) & 1) ^ 1, abort_flag)) { stop = true; break; }
+        bring(vt, &maps.v, maps.v_step, &v_full[st]);
+        v_issued = q + 1;
+      }
+    }
+    // Every copy lands before the CTA may exit.
+    for (int i = max(0, k_issued - kStages); i < k_issued; ++i)
+      wait_drain(&k_full[i % kStages], (i / kStages) & 1, 50000000ull);
+    for (int i = max(0, v_issued - kStages); i < v_issued; ++i)
+      wait_drain(&v_full[i % kStages], (i / kStages) & 1, 50000000ull);
+    __syncwarp();
+  } else if (warp == 4) {
+    if (lane == 0) {
+      constexpr uint32_t kBase = (1u << 4) | (F::kCode << 7) | (F::kCode << 10) | ((uint32_t)(kRows >> 4) << 24);
+      constexpr uint32_t kQk = kBase | ((uint32_t)(kKeys >> 3) << 17);
+      constexpr uint32_t kPv = kBase | ((uint32_t)(kDim >> 3) << 17) | (1u << 16);  // V is N-major
+      const uint32_t qa = smem_u32(smem), ka = qa + C::kKOff, va = qa + C::kVOff;
+      int q = 0, pieces = 0;
+      bool stop = false;
+      auto scores = [&](int i) {  // S = Q K^T of tile i
+        const int st = i % kStages;
+        if (!wait_phase(&k_full[st], (i / kStages) & 1, abort_flag)) return false;
+        tc_after_sync();
+#pragma unroll
+        for (int j = 0; j < kDim / 16; ++j)
+          mma_ss(tmem + C::kSCol, desc128(qa + j / 4 * C::kQBlock + j % 4 * 32, 16),
+                 desc128(ka + st * C::kTile + j / 4 * C::kBlock + j % 4 * 32, 16), kQk, j > 0);
+        mma_commit(&k_empty[st]);
+        mma_commit(s_full);
+        return true;
+      };
+      while (next < end && !stop) {
+        Piece p;
+        take(p);
+        if (p.tile0 >= p.tile1) continue;
+        if (!wait_phase(q_full, pieces & 1, abort_flag) || !scores(q)) break;
+        ++pieces;
+        for (uint32_t tile = p.tile0; tile < p.tile1; ++tile, ++q) {
+          const int st = q % kStages;
+          // P is written and S has been read: the next scores go first, so that
+          // their softmax can start under this tile's products.
+          if (!wait_phase(p_full, q & 1, abort_flag) || (tile + 1 < p.tile1 && !scores(q + 1)) ||
+              !wait_phase(&v_full[st], (q / kStages) & 1, abort_flag)) {
+            stop = true;
+            break;
+          }
+          tc_after_sync();
+#pragma unroll
+          for (int j = 0; j < kKeys / 16; ++j)
+            mma_ts(tmem + C::kOCol, tmem + C::kPCol + j * 8, desc128(va + st * C::kTile + j * 2048, C::kBlock), kPv,
+                   tile > p.tile0 || j > 0);
+          mma_commit(&v_empty[st]);
+          mma_commit(o_full);
+          o_commits = q + 1;
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    const uint32_t tl = tmem + ((uint32_t)(warp * 32) << 16);  // this warp's lanes
+    int q = 0, pieces = 0;
+    bool stop = false;
+    while (next < end && !stop) {
+      Piece p;
+      take(p);
+      ++pieces;
+      const uint32_t row = p.row_tile * kRows + tid, token = row / a.group;
+      const uint32_t head = p.head * a.group + row % a.group;
+      const bool there = row < rows;
+      // Rows past the last see everything: zeros times finite or other keys, never stored.
+      const RowView view = there ? row_view<kTree>(a, s, token) : RowView{0xffffffffu, 0ull};
+      float m = -INFINITY, l = 0.f;  // the maximum in use, in powers of two; the sum of weights
+      // Tiles from here on hold a key that some row does not see.
+      const uint32_t mask0 = (kTree ? s.context : row_view<false>(a, s, p.row_tile * kRows / a.group).all) / kKeys;
+      if (p.tile0 < p.tile1) {
+        const T* src = static_cast<const T*>(a.q.data) + (uint64_t)(s.q0 + token) * a.q.row_stride +
+                       (uint64_t)head * a.q.head_stride;
+#pragma unroll
+        for (int c = 0; c < kDim / 8; ++c) {
+          const uint4 w = there ? reinterpret_cast<const uint4*>(src)[c] : make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(smem + c / 8 * C::kQBlock + tid * 128 + ((c % 8) ^ (tid & 7)) * 16) = w;
+        }
+        fence_async_smem();
+        tc_before_sync();  // the piece before has been read from TMEM
+        mbar_arrive(q_full);
+      }
+      for (uint32_t tile = p.tile0; tile < p.tile1; ++tile, ++q) {
+        const uint32_t key0 = tile * kKeys;
+        const bool masked = tile >= mask0;
+        if (!wait_warp(s_full, q & 1, abort_flag)) { stop = true; break; }
+        tc_after_sync();
+        uint32_t v[32];
+        float top = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < kKeys; c += 32) {
+          tmem_ld32(tl + C::kSCol + c, v);
+          tmem_wait_ld32(v);
+          if (masked) {
+            const uint32_t seen = seen32(view, key0 + c);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              top = fmaxf(top, (seen >> i) & 1 ? __uint_as_float(v[i]) : -INFINITY);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(v[i]));
+          }
+        }
+        top = __fmul_rn(top, a.scale_log2);
+        // P and O are free once the products before are done.
+        if (q > 0 && !wait_warp(o_full, (q - 1) & 1, abort_flag)) { stop = true; break; }
+        tc_after_sync();
+        float keep = 1.f;
+        if (m == -INFINITY) {
+          m = top;  // O holds zeros at most
+        } else if (top > m + F::kSlack) {
+          keep = exp2_fast(m - top);
+          m = top;
+        }
+        if (__any_sync(0xffffffffu, keep != 1.f) && tile > p.tile0) {
+#pragma unroll
+          for (int c = 0; c < kDim; c += 32) {
+            tmem_ld32(tl + C::kOCol + c, v);
+            tmem_wait_ld32(v);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__fmul_rn(__uint_as_float(v[i]), keep));
+            tmem_st32(tl + C::kOCol + c, v);
+          }
+          l = __fmul_rn(l, keep);
+        }
+        const float base = (m == -INFINITY ? 0.f : m) - F::kRaise;
+#pragma unroll
+        for (int c = 0; c < kKeys; c += 32) {
+          tmem_ld32(tl + C::kSCol + c, v);
+          tmem_wait_ld32(v);
+          const uint32_t seen = masked ? seen32(view, key0 + c) : 0xffffffffu;
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            float x = exp2_fast(__fmaf_rn(__uint_as_float(v[i]), a.scale_log2, -base));
+            float y = exp2_fast(__fmaf_rn(__uint_as_float(v[i + 1]), a.scale_log2, -base));
+            if (masked) {
+              x = (seen >> i) & 1 ? x : 0.f;
+              y = (seen >> (i + 1)) & 1 ? y : 0.f;
+            }
+            l += x;
+            l += y;
+            w[i / 2] = Elements<T>::pair(x, y);
+          }
+          tmem_st16(tl + C::kPCol + c / 2, w);
+        }
+        if (masked) {
+          // Value rows of this tile, one per thread: zero past the keys, and without
+          // what is not finite.
+          if (!wait_warp(&v_full[q % kStages], (q / kStages) & 1, abort_flag)) { stop = true; break; }
+          if (tid < kKeys) {
+            uint8_t* at = smem + C::kVOff + (q % kStages) * C::kTile + tid * 128;
+            const bool past = key0 + tid >= s.len;
+            bool found = false;
+#pragma unroll 4
+            for (int c = 0; c < kDim / 8; ++c) {
+              uint4* word = reinterpret_cast<uint4*>(at + c / 8 * C::kBlock + ((c % 8) ^ (tid & 7)) * 16);
+              uint4 x = past ? make_uint4(0, 0, 0, 0) : *word;
+              uint32_t* u = reinterpret_cast<uint32_t*>(&x);
+              bool write = past;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t e = u[i] & F::kExponents;
+                if ((e & 0xffffu) == (F::kExponents & 0xffffu)) { u[i] &= 0xffff0000u; found = write = true; }
+                if ((e >> 16) == (F::kExponents >> 16)) { u[i] &= 0xffffu; found = write = true; }
+              }
+              if (write) *word = x;
+            }
+            if (found) *dirty = pieces;
+          }
+          fence_async_smem();
+        }
+        tmem_wait_st();
+        tc_before_sync();
+        mbar_arrive(p_full);
+      }
+      if (stop) break;
+
+      // The piece is done: O / l, or O with its maximum and sum.
+      if (p.tile0 < p.tile1) {
+        if (!wait_warp(o_full, (q - 1) & 1, abort_flag)) break;
+        tc_after_sync();
+      }
+      const float inv = l == 0.f ? 0.f : __frcp_rn(l);
+      T* out = static_cast<T*>(a.out.data) + (uint64_t)(s.q0 + token) * a.out.row_stride +
+               (uint64_t)head * a.out.head_stride;
+      float* rec = kTree && p.partial >= 0 ? a.partial + (size_t)p.partial * partial_words<kRows, kDim>() : nullptr;
+      const bool mend = *dirty == pieces;
+#pragma unroll
+      for (int c = 0; c < kDim; c += 32) {
+        uint32_t v[32];
+        if (p.tile0 < p.tile1) {
+          tmem_ld32(tl + C::kOCol + c, v);
+          tmem_wait_ld32(v);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = 0;
+        }
+        if (!there) continue;
+        if (mend) {
+          // A weight is positive: what is not finite passes through the sum as it is.
+          for (uint32_t key = max(p.tile0, mask0) * kKeys; key < min(p.tile1 * kKeys, s.len); ++key) {
+            if (!view.sees(key)) continue;
+            const T* from;
+            if (kTree) {
+              const uint32_t page = a.tables[(uint64_t)p.seq * a.table_width + key / a.cache.page_size];
+              if (page >= a.cache.pages) continue;
+              from = reinterpret_cast<const T*>(a.cache.v) +
+                     (((uint64_t)page * a.cache.kv_heads + p.head) * a.cache.page_size + key % a.cache.page_size) * kDim;
+            } else {
+              from = static_cast<const T*>(a.v.data) + (uint64_t)(s.kv0 + key) * a.v.row_stride +
+                     (uint64_t)p.head * a.v.head_stride;
+            }
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float x = (float)from[c + i];
+              if (!(fabsf(x) < INFINITY)) v[i] = __float_as_uint(__uint_as_float(v[i]) + x);
+            }
+          }
+        }
+        if (rec) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<uint4*>(rec + tid * kDim + c + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            float y[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) y[u] = __fmul_rn(__uint_as_float(v[i + u]), inv);
+            *reinterpret_cast<uint4*>(out + c + i) = Elements<T>::store(y);
+          }
+        }
+      }
+      if (there && rec) {
+        rec[kRows * kDim + tid] = m == -INFINITY ? m : m - F::kRaise;
+        rec[kRows * kDim + kRows + tid] = l;
+      }
+    }
+  }
+
+  tc_before_sync();
+  __syncthreads();
+  tc_after_sync();
+  if (*abort_flag) {
+    if (warp == 4 && lane == 0 && o_commits)  // issued MMAs finish
+      wait_drain(o_full, (o_commits - 1) & 1, 50000000ull);
+    if (tid == 0) atomicOr(&g_tc_status, 1u);
+  }
+  tc_before_sync();
+  __syncthreads();
+  tc_after_sync();
+  if (warp == 4) tmem_dealloc(tmem, C::kCols);
+}
+
+using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                            const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                            CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+uint32_t encoder(Encode* out) {
+  static Encode found = nullptr;
+  if (!found) {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult how;
+    PB_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &how));
+    if (how != cudaDriverEntryPointSuccess || !f) {
+      set_last_error("the driver has no cuTensorMapEncodeTiled");
+      return PB_DEVICE;
+    }
+    found = reinterpret_cast<Encode>(f);
+  }
+  *out = found;
+  return PB_OK;
+}
+
+template <class T, int kDim, bool kTree>
+uint32_t make_map(const AttnArgs& a, const pb_rows& r, const void* cache, CUtensorMap* map) {
+  using C = Tc<kDim>;
+  Encode encode = nullptr;
+  uint32_t st = encoder(&encode);
+  if (st) return st;
+  CUresult e;
+  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  if (kTree) {
+    const cuuint64_t size = a.cache.page_size;
+    const cuuint64_t dims[4] = {(cuuint64_t)kDim, size, a.cache.kv_heads, a.cache.pages};
+    const cuuint64_t strides[3] = {kDim * 2, size * kDim * 2, a.cache.kv_heads * size * kDim * 2};
+    const cuuint32_t box[4] = {64, (cuuint32_t)std::min<cuuint64_t>(size, C::kKeys), 1, 1};
+    e = encode(map, Format<T>::kMap, 4, const_cast<void*>(cache), dims, strides, box, ones,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  } else {
+    const bool one = a.kv_heads == 1 || r.head_stride == 0;
+    const cuuint64_t dims[3] = {(cuuint64_t)kDim, std::max(1u, a.kv_rows), one ? 1 : a.kv_heads};
+    const cuuint64_t strides[2] = {std::max<cuuint64_t>(16, r.row_stride * 2), one ? 16 : r.head_stride * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)C::kKeys, 1};
+    e = encode(map, Format<T>::kMap, 3, r.data, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  }
+  if (e != CUDA_SUCCESS) {
+    char text[96];
+    std::snprintf(text, sizeof text, "cuTensorMapEncodeTiled refused the keys or values (error %d)", (int)e);
+    set_last_error(text);
+    return PB_DEVICE;
+  }
+  return PB_OK;
+}
+
+template <class T, int kDim, bool kTree>
+uint32_t launch(const AttnArgs& a, uint32_t grid, cudaStream_t s) {
+  using C = Tc<kDim>;
+  auto kernel = attention_tc_kernel<T, kDim, kTree>;
+  static std::atomic<uint64_t> configured{0};
+  if (attribute_needed(configured)) {
+    PB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::bytes(PB_MAX_SEQS)));
+    attribute_done(configured);
+  }
+  Maps maps;
+  uint32_t st = make_map<T, kDim, kTree>(a, a.k, a.cache.k, &maps.k);
+  if (!st) st = make_map<T, kDim, kTree>(a, a.v, a.cache.v, &maps.v);
+  if (st) return st;
+  maps.k_step = a.k.head_stride != 0;
+  maps.v_step = a.v.head_stride != 0;
+  kernel<<<grid, kThreads, C::bytes(a.seqs), s>>>(a, maps);
+  PB_CUDA(cudaGetLastError());
+  if (kTree) {
+    const dim3 join(std::min<uint32_t>(grid, 1024), 4);
+    combine_kernel<T, kDim, kRows, C::kKeys, kLeast><<<join, 256, a.seqs * 4, s>>>(a, grid);
+    PB_CUDA(cudaGetLastError());
+  }
+  return PB_OK;
+}
+
+}  // namespace
+
+uint32_t tc_prompt(const AttnArgs& a, uint32_t type, uint32_t head_dim, cudaStream_t s) {
+  const uint32_t grid = (a.q_rows * a.group / kRows + a.seqs) * a.kv_heads;
+  if (type == PB_TYPE_F16)
+    return head_dim == 64 ? launch<__half, 64, false>(a, grid, s) : launch<__half, 128, false>(a, grid, s);
+  return head_dim == 64 ? launch<__nv_bfloat16, 64, false>(a, grid, s)
+                        : launch<__nv_bfloat16, 128, false>(a, grid, s);
+}
+
+uint64_t tc_tree_words(uint32_t head_dim) { return (uint64_t)tree_ctas(2) * 2 * kRows * (head_dim + 2); }
+
+uint32_t tc_tree(const AttnArgs& a, uint32_t type, uint32_t head_dim, cudaStream_t s) {
+  const uint32_t grid = tree_ctas(2);
+  if (type == PB_TYPE_F16)
+    return head_dim == 64 ? launch<__half, 64, true>(a, grid, s) : launch<__half, 128, true>(a, grid, s);
+  return head_dim == 64 ? launch<__nv_bfloat16, 64, true>(a, grid, s) : launch<__nv_bfloat16, 128, true>(a, grid, s);
+}
+
+uint32_t tc_status(cudaStream_t s) {
+  unsigned int st = 0;
+  PB_CUDA(cudaStreamSynchronize(s));
+  PB_CUDA(cudaMemcpyFromSymbol(&st, g_tc_status, 4));
+  if (!st) return PB_OK;
+  const unsigned int zero = 0;
+  PB_CUDA(cudaMemcpyToSymbol(g_tc_status, &zero, 4));
+  set_last_error("an attention pipeline timed out waiting for a copy or an MMA");
+  return PB_DEVICE;
+}
+
+}  // namespace paged
+}  // namespace pb
