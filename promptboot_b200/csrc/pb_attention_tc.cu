@@ -9,10 +9,11 @@
 // step of the type per weight and averages out over the keys.
 //
 // Warps: 0..3 softmax, one row per thread (TMEM lane = row); 4 issues the MMAs;
-// 5 brings K and V tiles by TMA (128-byte swizzle) into rings of kStages.  S, P and
-// O have TMEM columns of their own, 256 in all, so two CTAs share an SM and one's
-// products run under the other's exponentials; and no MMA of a tile depends on the
-// order of two MMAs of different shapes.
+// 5 brings K and V tiles by TMA (128-byte swizzle) into rings of kStages.  S has two
+// buffers in TMEM, P takes the place of the scores it comes from: the scores of tile
+// j + 2 go out when the products of tile j are done, a tile ahead of their softmax,
+// which therefore seldom waits.  256 TMEM columns, so two CTAs share an SM and one's
+// products run under the other's exponentials.
 //
 // The running maximum is the one in use until a row's true maximum passes it by
 // 2^kSlack: O is rescaled (through registers) only then, seldom after the first
@@ -60,8 +61,8 @@ struct Format<__nv_bfloat16> {
 
 template <int kDim>
 struct Tc {
-  static constexpr int kKeys = kDim == 64 ? 128 : 64;
-  static constexpr int kStages = 2;
+  static constexpr int kKeys = 64;
+  static constexpr int kStages = kDim == 64 ? 4 : 2;
   static constexpr int kHalves = kDim / 64;           // 128-byte column blocks of a row
   static constexpr int kQBlock = kRows * 128;
   static constexpr int kBlock = kKeys * 128;          // one column block of a K or V tile
@@ -69,9 +70,9 @@ struct Tc {
   static constexpr int kKOff = kHalves * kQBlock;
   static constexpr int kVOff = kKOff + kStages * kTile;
   static constexpr int kBarOff = kVOff + kStages * kTile;
-  static constexpr int kBars = 4 * kStages + 4;
+  static constexpr int kBars = 4 * kStages + 5;
   static constexpr int kPrefixOff = kBarOff + kBars * 8 + 16;
-  static constexpr int kSCol = 0, kPCol = kKeys, kOCol = kKeys + kKeys / 2;
+  static constexpr int kOCol = 2 * kKeys;             // S and P: [0, 64) and [64, 128)
   static constexpr int kCols = 256;
   static_assert(kOCol + kDim <= kCols, "TMEM columns");
   static size_t bytes(uint32_t seqs) { return 1024 + kPrefixOff + (size_t)seqs * 4; }
@@ -197,8 +198,8 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   uint64_t* v_empty = v_full + kStages;
   uint64_t* q_full = v_empty + kStages;
   uint64_t* s_full = q_full + 1;
-  uint64_t* p_full = s_full + 1;
-  uint64_t* o_full = p_full + 1;  // O holds the tile's products, P is free
+  uint64_t* p_full = s_full + 2;
+  uint64_t* o_full = p_full + 1;  // O holds the tile's products, its P is free
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* dirty = abort_flag + 1;  // the last piece with a value that was taken out
@@ -229,7 +230,8 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       mbar_init(&v_empty[i], 1);
     }
     mbar_init(q_full, kRows);
-    mbar_init(s_full, 1);
+    mbar_init(&s_full[0], 1);
+    mbar_init(&s_full[1], 1);
     mbar_init(p_full, kRows);
     mbar_init(o_full, 1);
     *abort_flag = 0;
@@ -329,35 +331,38 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         tc_after_sync();
 #pragma unroll
         for (int j = 0; j < kDim / 16; ++j)
-          mma_ss(tmem + C::kSCol, desc128(qa + j / 4 * C::kQBlock + j % 4 * 32, 16),
+          mma_ss(tmem + (i & 1) * kKeys, desc128(qa + j / 4 * C::kQBlock + j % 4 * 32, 16),
                  desc128(ka + st * C::kTile + j / 4 * C::kBlock + j % 4 * 32, 16), kQk, j > 0);
         mma_commit(&k_empty[st]);
-        mma_commit(s_full);
+        mma_commit(&s_full[i & 1]);
         return true;
       };
       while (next < end && !stop) {
         Piece p;
         take(p);
         if (p.tile0 >= p.tile1) continue;
-        if (!wait_phase(q_full, pieces & 1, abort_flag) || !scores(q)) break;
+        if (!wait_phase(q_full, pieces & 1, abort_flag) || !scores(q) || (p.tile0 + 1 < p.tile1 && !scores(q + 1)))
+          break;
         ++pieces;
         for (uint32_t tile = p.tile0; tile < p.tile1; ++tile, ++q) {
           const int st = q % kStages;
-          // P is written and S has been read: the next scores go first, so that
-          // their softmax can start under this tile's products.
-          if (!wait_phase(p_full, q & 1, abort_flag) || (tile + 1 < p.tile1 && !scores(q + 1)) ||
-              !wait_phase(&v_full[st], (q / kStages) & 1, abort_flag)) {
+          if (!wait_phase(p_full, q & 1, abort_flag) || !wait_phase(&v_full[st], (q / kStages) & 1, abort_flag)) {
             stop = true;
             break;
           }
           tc_after_sync();
 #pragma unroll
           for (int j = 0; j < kKeys / 16; ++j)
-            mma_ts(tmem + C::kOCol, tmem + C::kPCol + j * 8, desc128(va + st * C::kTile + j * 2048, C::kBlock), kPv,
-                   tile > p.tile0 || j > 0);
+            mma_ts(tmem + C::kOCol, tmem + (q & 1) * kKeys + j * 8, desc128(va + st * C::kTile + j * 2048, C::kBlock),
+                   kPv, tile > p.tile0 || j > 0);
           mma_commit(&v_empty[st]);
           mma_commit(o_full);
           o_commits = q + 1;
+          // The scores after the next take the place of this P, once it has been read.
+          if (tile + 2 < p.tile1 && (!wait_phase(o_full, q & 1, abort_flag) || !scores(q + 2))) {
+            stop = true;
+            break;
+          }
         }
       }
     }
@@ -375,7 +380,8 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       const bool there = row < rows;
       // Rows past the last see everything: zeros times finite or other keys, never stored.
       const RowView view = there ? row_view<kTree>(a, s, token) : RowView{0xffffffffu, 0ull};
-      float m = -INFINITY, l = 0.f;  // the maximum in use, in powers of two; the sum of weights
+      float m = -INFINITY;          // the maximum in use, in powers of two
+      uint64_t l2[2] = {0, 0};      // the sum of weights, in four parts
       // Tiles from here on hold a key that some row does not see.
       const uint32_t mask0 = (kTree ? s.context : row_view<false>(a, s, p.row_tile * kRows / a.group).all) / kKeys;
       if (p.tile0 < p.tile1) {
@@ -393,28 +399,30 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       for (uint32_t tile = p.tile0; tile < p.tile1; ++tile, ++q) {
         const uint32_t key0 = tile * kKeys;
         const bool masked = tile >= mask0;
-        if (!wait_warp(s_full, q & 1, abort_flag)) { stop = true; break; }
+        const uint32_t sc = tl + (q & 1) * kKeys;
+        if (!wait_warp(&s_full[q & 1], (q >> 1) & 1, abort_flag)) { stop = true; break; }
         tc_after_sync();
-        uint32_t v[32];
-        float top = -INFINITY;
+        uint32_t v[2][32];
+        tmem_ld32(sc, v[0]);
+        tmem_ld32(sc + 32, v[1]);
+        tmem_wait_ld32(v[0]);
+        tmem_wait_ld32(v[1]);
+        if (masked) {
 #pragma unroll
-        for (int c = 0; c < kKeys; c += 32) {
-          tmem_ld32(tl + C::kSCol + c, v);
-          tmem_wait_ld32(v);
-          if (masked) {
-            const uint32_t seen = seen32(view, key0 + c);
+          for (int c = 0; c < 2; ++c) {
+            const uint32_t seen = seen32(view, key0 + 32 * c);
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              top = fmaxf(top, (seen >> i) & 1 ? __uint_as_float(v[i]) : -INFINITY);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(v[i]));
+            for (int i = 0; i < 32; ++i) v[c][i] = (seen >> i) & 1 ? v[c][i] : 0xff800000u;  // -inf
           }
         }
-        top = __fmul_rn(top, a.scale_log2);
-        // P and O are free once the products before are done.
-        if (q > 0 && !wait_warp(o_full, (q - 1) & 1, abort_flag)) { stop = true; break; }
-        tc_after_sync();
+        float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 64; i += 8)
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            t[u] = fmaxf(t[u], fmaxf(__uint_as_float(v[i / 32][i % 32 + 2 * u]),
+                                     __uint_as_float(v[i / 32][i % 32 + 2 * u + 1])));
+        const float top = __fmul_rn(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), a.scale_log2);
         float keep = 1.f;
         if (m == -INFINITY) {
           m = top;  // O holds zeros at most
@@ -422,37 +430,36 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
           keep = exp2_fast(m - top);
           m = top;
         }
-        if (__any_sync(0xffffffffu, keep != 1.f) && tile > p.tile0) {
+        if (__any_sync(0xffffffffu, keep != 1.f)) {  // never in a piece's first tile
+          if (!wait_warp(o_full, (q - 1) & 1, abort_flag)) { stop = true; break; }
+          tc_after_sync();
+          uint32_t o[32];
 #pragma unroll
           for (int c = 0; c < kDim; c += 32) {
-            tmem_ld32(tl + C::kOCol + c, v);
-            tmem_wait_ld32(v);
+            tmem_ld32(tl + C::kOCol + c, o);
+            tmem_wait_ld32(o);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__fmul_rn(__uint_as_float(v[i]), keep));
-            tmem_st32(tl + C::kOCol + c, v);
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__fmul_rn(__uint_as_float(o[i]), keep));
+            tmem_st32(tl + C::kOCol + c, o);
           }
-          l = __fmul_rn(l, keep);
+          l2[0] = mul2(l2[0], pk(keep, keep));
+          l2[1] = mul2(l2[1], pk(keep, keep));
         }
-        const float base = (m == -INFINITY ? 0.f : m) - F::kRaise;
+        const float base = F::kRaise - (m == -INFINITY ? 0.f : m);
+        const uint64_t scale2 = pk(a.scale_log2, a.scale_log2), base2 = pk(base, base);
 #pragma unroll
-        for (int c = 0; c < kKeys; c += 32) {
-          tmem_ld32(tl + C::kSCol + c, v);
-          tmem_wait_ld32(v);
-          const uint32_t seen = masked ? seen32(view, key0 + c) : 0xffffffffu;
+        for (int c = 0; c < 2; ++c) {
           uint32_t w[16];
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
-            float x = exp2_fast(__fmaf_rn(__uint_as_float(v[i]), a.scale_log2, -base));
-            float y = exp2_fast(__fmaf_rn(__uint_as_float(v[i + 1]), a.scale_log2, -base));
-            if (masked) {
-              x = (seen >> i) & 1 ? x : 0.f;
-              y = (seen >> (i + 1)) & 1 ? y : 0.f;
-            }
-            l += x;
-            l += y;
-            w[i / 2] = Elements<T>::pair(x, y);
+            float y0, y1;
+            unpk(fma2(pk_u(v[c][i], v[c][i + 1]), scale2, base2), y0, y1);
+            y0 = exp2_fast(y0);
+            y1 = exp2_fast(y1);
+            l2[i / 2 & 1] = add2(l2[i / 2 & 1], pk(y0, y1));
+            w[i / 2] = Elements<T>::pair(y0, y1);
           }
-          tmem_st16(tl + C::kPCol + c / 2, w);
+          tmem_st16(sc + 16 * c, w);
         }
         if (masked) {
           // Value rows of this tile, one per thread: zero past the keys, and without
@@ -480,6 +487,9 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
           }
           fence_async_smem();
         }
+        // By now the products before are done; their phase is waited for at every tile,
+        // so that a wait for the next cannot take it for an older one.
+        if (q > 0 && !wait_warp(o_full, (q - 1) & 1, abort_flag)) { stop = true; break; }
         tmem_wait_st();
         tc_before_sync();
         mbar_arrive(p_full);
@@ -491,6 +501,10 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         if (!wait_warp(o_full, (q - 1) & 1, abort_flag)) break;
         tc_after_sync();
       }
+      float part[4];
+      unpk(l2[0], part[0], part[1]);
+      unpk(l2[1], part[2], part[3]);
+      const float l = (part[0] + part[1]) + (part[2] + part[3]);
       const float inv = l == 0.f ? 0.f : __frcp_rn(l);
       T* out = static_cast<T*>(a.out.data) + (uint64_t)(s.q0 + token) * a.out.row_stride +
                (uint64_t)head * a.out.head_stride;
