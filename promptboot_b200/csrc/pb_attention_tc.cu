@@ -10,10 +10,12 @@
 //
 // Warps: 0..3 softmax, one row per thread (TMEM lane = row); 4 issues the MMAs;
 // 5 brings K and V tiles by TMA (128-byte swizzle) into rings of kStages.  S has two
-// buffers in TMEM, P takes the place of the scores it comes from: the scores of tile
-// j + 2 go out when the products of tile j are done, a tile ahead of their softmax,
-// which therefore seldom waits.  256 TMEM columns, so two CTAs share an SM and one's
-// products run under the other's exponentials.
+// buffers in TMEM, P takes the place of the upper half of the scores it comes from: the
+// scores of tile j + 2 go out when the products of tile j are done, a tile ahead of
+// their softmax, which therefore seldom waits.  256 TMEM columns, so two CTAs share an
+// SM and one's products run under the other's exponentials.  (Four CTAs of one score
+// buffer each measured the same at heads of 64: the SM's 16 exponentials a cycle bind
+// both.)
 //
 // The running maximum is the one in use until a row's true maximum passes it by
 // 2^kSlack: O is rescaled (through registers) only then, seldom after the first
@@ -50,6 +52,7 @@ struct Format<__half> {
   static constexpr CUtensorMapDataType kMap = CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   static constexpr float kSlack = 4.f, kRaise = 10.f;  // weights stay below 2^14 of 65504
   static constexpr uint32_t kExponents = 0x7c007c00u;
+  static constexpr int kDegree = 4;
 };
 template <>
 struct Format<__nv_bfloat16> {
@@ -57,6 +60,7 @@ struct Format<__nv_bfloat16> {
   static constexpr CUtensorMapDataType kMap = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   static constexpr float kSlack = 8.f, kRaise = 0.f;
   static constexpr uint32_t kExponents = 0x7f807f80u;
+  static constexpr int kDegree = 3;
 };
 
 template <int kDim>
@@ -70,7 +74,7 @@ struct Tc {
   static constexpr int kKOff = kHalves * kQBlock;
   static constexpr int kVOff = kKOff + kStages * kTile;
   static constexpr int kBarOff = kVOff + kStages * kTile;
-  static constexpr int kBars = 4 * kStages + 5;
+  static constexpr int kBars = 4 * kStages + 6;
   static constexpr int kPrefixOff = kBarOff + kBars * 8 + 16;
   static constexpr int kOCol = 2 * kKeys;             // S and P: [0, 64) and [64, 128)
   static constexpr int kCols = 256;
@@ -78,20 +82,54 @@ struct Tc {
   static size_t bytes(uint32_t seqs) { return 1024 + kPrefixOff + (size_t)seqs * 4; }
 };
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+// One lane of the warp, for the instructions below: the whole warp runs them, with
+// that lane's predicate, so that their operands stay in uniform registers (issued from
+// a branch of one lane, four MMAs and their commit took 450 cycles).
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t is;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(is)
+      :
+      : "memory");
+  return is;
+}
+__device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                       uint32_t add) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add)
+      "setp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add), "r"(leader)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+__device__ __forceinline__ void mma_ts(uint32_t leader, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                       uint32_t add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, e;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add)
+      "setp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void commit_to(uint32_t leader, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "setp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+      ::"r"(smem_u32(bar)), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void expect_tx(uint32_t leader, uint64_t* bar, uint32_t bytes) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "setp.ne.b32 e, %2, 0;\n\t"
+      "@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}"
+      ::"r"(smem_u32(bar)), "r"(bytes), "r"(leader)
       : "memory");
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
@@ -105,16 +143,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
-      ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
-        "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
-        "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
-        "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-      : "memory");
-}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
@@ -124,30 +152,32 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
 }
 // Waits for this thread's TMEM loads; the registers pass through, so that nothing
 // that uses them moves up.
-__device__ __forceinline__ void tmem_wait_ld32(uint32_t (&v)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
-                 "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]),
-                 "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]),
-                 "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]),
-                 "+r"(v[30]), "+r"(v[31])
-               :
-               : "memory");
+template <int N>
+__device__ __forceinline__ void tmem_wait(uint32_t (&v)[N]) {
+  tmem_wait_ld();
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(v[i]));
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // TMA tile loads: the innermost coordinate is 0 or 64 elements (128 bytes).
-__device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+__device__ __forceinline__ void tma_3d(uint32_t leader, uint32_t dst, const CUtensorMap* map, int x, int y, int z,
+                                       uint64_t* bar) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-      ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      "{\n\t.reg .pred e;\n\t"
+      "setp.ne.b32 e, %6, 0;\n\t"
+      "@e cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n\t}"
+      ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar)), "r"(leader)
       : "memory");
 }
-__device__ __forceinline__ void tma_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+__device__ __forceinline__ void tma_4d(uint32_t leader, uint32_t dst, const CUtensorMap* map, int x, int y, int z,
+                                       int w, uint64_t* bar) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-      ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      "{\n\t.reg .pred e;\n\t"
+      "setp.ne.b32 e, %7, 0;\n\t"
+      "@e cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n\t}"
+      ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar)), "r"(leader)
       : "memory");
 }
 
@@ -162,6 +192,47 @@ __device__ __forceinline__ uint64_t desc128(uint32_t addr, uint32_t lead) {
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
+  float x0, x1;
+  unpk(x, x0, x1);
+  return pk(exp2_fast(x0), exp2_fast(x1));
+}
+// The same without the exponential unit: x less its nearest whole number n (Cody and
+// Waite's reduction; n comes out of the low bits of x + 1.5 * 2^23) through a
+// polynomial of least relative error on [-1/2, 1/2], 7.5e-5 of degree 3 and 2.6e-6
+// of degree 4, times 2^n by an addition to the exponent.  x from -126 (below: 2^-126
+// at most) to 127.
+template <int kDegree>
+__device__ __forceinline__ uint64_t exp2_poly(uint64_t x) {
+  float x0, x1;
+  unpk(x, x0, x1);
+  x = pk(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
+  const uint64_t t = add2(x, pk(12582912.f, 12582912.f));
+  const uint64_t f = fma2(add2(t, pk(-12582912.f, -12582912.f)), pk(-1.f, -1.f), x);
+  auto both = [](float c) { return pk(c, c); };
+  uint64_t y;
+  if (kDegree == 3) {
+    y = fma2(both(0.055171669f), f, both(0.242611125f));
+    y = fma2(y, f, both(0.693260968f));
+    y = fma2(y, f, both(0.999928057f));
+  } else {
+    y = fma2(both(0.0095701022f), f, both(0.0559178628f));
+    y = fma2(y, f, both(0.240247443f));
+    y = fma2(y, f, both(0.693121791f));
+    y = fma2(y, f, both(0.999999285f));
+  }
+  float y0, y1, t0, t1;
+  unpk(y, y0, y1);
+  unpk(t, t0, t1);
+  return pk_u(__float_as_uint(y0) + (__float_as_uint(t0) << 23), __float_as_uint(y1) + (__float_as_uint(t1) << 23));
+}
+// The largest; not a number where one is not.
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
 
@@ -197,15 +268,16 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   uint64_t* v_full = k_empty + kStages;
   uint64_t* v_empty = v_full + kStages;
   uint64_t* q_full = v_empty + kStages;
-  uint64_t* s_full = q_full + 1;
-  uint64_t* p_full = s_full + 2;
+  uint64_t* p_full = q_full + 1;
   uint64_t* o_full = p_full + 1;  // O holds the tile's products, its P is free
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 1);
+  uint64_t* done = o_full + 1;    // O holds the piece's
+  uint64_t* s_full = done + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* dirty = abort_flag + 1;  // the last piece with a value that was taken out
   uint32_t* prefix = reinterpret_cast<uint32_t*>(smem + C::kPrefixOff);
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   work_prefix<kTree, kRows, kKeys, kThreads>(a, prefix);
   const uint32_t total = prefix[a.seqs - 1];
   uint32_t next, end;
@@ -234,6 +306,7 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     mbar_init(&s_full[1], 1);
     mbar_init(p_full, kRows);
     mbar_init(o_full, 1);
+    mbar_init(done, 1);
     *abort_flag = 0;
     *dirty = 0;
     fence_barrier_init();
@@ -272,104 +345,112 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     }
   };
 
-  int k_issued = 0, v_issued = 0, o_commits = 0;  // for the way out
+  int k_brought = 0, v_brought = 0, o_commits = 0;  // tiles, for the way out
 
   if (warp == 5) {
-    bool stop = false;
+    const uint32_t leader = elect_one();
+    const uint32_t size = kTree ? min(a.cache.page_size, (uint32_t)kKeys) : kKeys;  // keys of a box
+    const uint32_t ka = smem_u32(smem) + C::kKOff, va = smem_u32(smem) + C::kVOff;
     int q = 0;  // tiles so far
+    bool stop = false;
     while (next < end && !stop) {
       Piece p;
       take(p);
-      const uint32_t size = kTree ? min(a.cache.page_size, (uint32_t)kKeys) : kKeys;  // rows of a box
-      for (uint32_t tile = p.tile0; tile < p.tile1 && !stop; ++tile, ++q) {
-        const int st = q % kStages;
-        const uint32_t key = tile * kKeys + lane * size;  // this lane's box
-        const uint32_t boxes = min((uint32_t)kKeys / size, ceil_div(s.len - tile * kKeys, size));
-        int page = 0;
-        if (kTree && (uint32_t)lane < boxes)
-          page = (int)a.tables[(uint64_t)p.seq * a.table_width + key / a.cache.page_size];
-        uint8_t* kt = smem + C::kKOff + st * C::kTile + lane * size * 128;
-        uint8_t* vt = smem + C::kVOff + st * C::kTile + lane * size * 128;
-        auto bring = [&](uint8_t* to, const CUtensorMap* map, uint32_t step, uint64_t* bar) {
-          if (lane == 0) mbar_expect_tx(bar, boxes * size * kHalves * 128);
-          __syncwarp();
-          if ((uint32_t)lane < boxes) {
+      auto boxes = [&](uint32_t tile) { return min((uint32_t)kKeys / size, ceil_div(s.len - tile * kKeys, size)); };
+      auto page_of = [&](uint32_t tile) {  // of box `lane` of a tile
+        const uint32_t key = tile * kKeys + lane * size;
+        return kTree && tile < p.tile1 && (uint32_t)lane < boxes(tile)
+                   ? (int)a.tables[(uint64_t)p.seq * a.table_width + key / a.cache.page_size] : 0;
+      };
+      int page = page_of(p.tile0);
+      for (uint32_t tile = p.tile0; tile < p.tile1; ++tile, ++q) {
+        const int st = q % kStages, ahead = page_of(tile + 1);
+        const uint32_t key = tile * kKeys, count = boxes(tile);
+        auto bring = [&](uint32_t to, const CUtensorMap* map, uint32_t step, uint64_t* full) {
+          expect_tx(leader, full, count * size * kHalves * 128);
+          for (uint32_t b = 0; b < count; ++b) {
+            const int at = kTree ? __shfl_sync(0xffffffffu, page, b) : 0;
 #pragma unroll
             for (int c = 0; c < kHalves; ++c) {
               if (kTree)
-                tma_4d(to + c * C::kBlock, map, c * 64, (int)(key % a.cache.page_size), (int)p.head, page, bar);
+                tma_4d(leader, to + c * C::kBlock + b * size * 128, map, c * 64, (int)(key % a.cache.page_size),
+                       (int)p.head, at, full);
               else
-                tma_3d(to + c * C::kBlock, map, c * 64, (int)(s.kv0 + key), (int)(p.head * step), bar);
+                tma_3d(leader, to + c * C::kBlock, map, c * 64, (int)(s.kv0 + key), (int)(p.head * step), full);
             }
           }
         };
-        if (!wait_warp(&k_empty[st], ((q / kStages) & 1) ^ 1, abort_flag)) { stop = true; break; }
-        bring(kt, &maps.k, maps.k_step, &k_full[st]);
-        k_issued = q + 1;
-        if (!wait_warp(&v_empty[st], ((q / kStages) & 1) ^ 1, abort_flag)) { stop = true; break; }
-        bring(vt, &maps.v, maps.v_step, &v_full[st]);
-        v_issued = q + 1;
+        if (!wait_soon(&k_empty[st], ((q / kStages) & 1) ^ 1, abort_flag)) { stop = true; break; }
+        bring(ka + st * C::kTile, &maps.k, maps.k_step, &k_full[st]);
+        k_brought = q + 1;
+        if (!wait_soon(&v_empty[st], ((q / kStages) & 1) ^ 1, abort_flag)) { stop = true; break; }
+        bring(va + st * C::kTile, &maps.v, maps.v_step, &v_full[st]);
+        v_brought = q + 1;
+        page = ahead;
       }
     }
-    // Every copy lands before the CTA may exit.
-    for (int i = max(0, k_issued - kStages); i < k_issued; ++i)
-      wait_drain(&k_full[i % kStages], (i / kStages) & 1, 50000000ull);
-    for (int i = max(0, v_issued - kStages); i < v_issued; ++i)
-      wait_drain(&v_full[i % kStages], (i / kStages) & 1, 50000000ull);
+    if (*abort_flag) {  // every copy lands before the CTA may exit
+      for (int i = max(0, k_brought - kStages); i < k_brought; ++i)
+        wait_drain(&k_full[i % kStages], (i / kStages) & 1, 50000000ull);
+      for (int i = max(0, v_brought - kStages); i < v_brought; ++i)
+        wait_drain(&v_full[i % kStages], (i / kStages) & 1, 50000000ull);
+    }
     __syncwarp();
   } else if (warp == 4) {
-    if (lane == 0) {
-      constexpr uint32_t kBase = (1u << 4) | (F::kCode << 7) | (F::kCode << 10) | ((uint32_t)(kRows >> 4) << 24);
-      constexpr uint32_t kQk = kBase | ((uint32_t)(kKeys >> 3) << 17);
-      constexpr uint32_t kPv = kBase | ((uint32_t)(kDim >> 3) << 17) | (1u << 16);  // V is N-major
-      const uint32_t qa = smem_u32(smem), ka = qa + C::kKOff, va = qa + C::kVOff;
-      int q = 0, pieces = 0;
-      bool stop = false;
-      auto scores = [&](int i) {  // S = Q K^T of tile i
-        const int st = i % kStages;
-        if (!wait_phase(&k_full[st], (i / kStages) & 1, abort_flag)) return false;
+    const uint32_t leader = elect_one();
+    constexpr uint32_t kBase = (1u << 4) | (F::kCode << 7) | (F::kCode << 10) | ((uint32_t)(kRows >> 4) << 24);
+    constexpr uint32_t kQk = kBase | ((uint32_t)(kKeys >> 3) << 17);
+    constexpr uint32_t kPv = kBase | ((uint32_t)(kDim >> 3) << 17) | (1u << 16);  // V is N-major
+    const uint32_t qa = smem_u32(smem), ka = qa + C::kKOff, va = qa + C::kVOff;
+    int q = 0, pieces = 0;  // tiles and pieces so far
+    bool stop = false;
+    while (next < end && !stop) {
+      Piece p;
+      take(p);
+      const int n = (int)(p.tile1 - p.tile0);
+      if (n <= 0) continue;
+      auto scores = [&](int t) {  // S = Q K^T
+        const int st = t % kStages;
+        if (!wait_soon(&k_full[st], (t / kStages) & 1, abort_flag)) return false;
         tc_after_sync();
 #pragma unroll
         for (int j = 0; j < kDim / 16; ++j)
-          mma_ss(tmem + (i & 1) * kKeys, desc128(qa + j / 4 * C::kQBlock + j % 4 * 32, 16),
+          mma_ss(leader, tmem + (t & 1) * kKeys, desc128(qa + j / 4 * C::kQBlock + j % 4 * 32, 16),
                  desc128(ka + st * C::kTile + j / 4 * C::kBlock + j % 4 * 32, 16), kQk, j > 0);
-        mma_commit(&k_empty[st]);
-        mma_commit(&s_full[i & 1]);
+        commit_to(leader, &s_full[t & 1]);
+        commit_to(leader, &k_empty[st]);
         return true;
       };
-      while (next < end && !stop) {
-        Piece p;
-        take(p);
-        if (p.tile0 >= p.tile1) continue;
-        if (!wait_phase(q_full, pieces & 1, abort_flag) || !scores(q) || (p.tile0 + 1 < p.tile1 && !scores(q + 1)))
+      if (!wait_soon(q_full, pieces & 1, abort_flag) || !scores(q) || (n > 1 && !scores(q + 1))) break;
+      ++pieces;
+      for (int i = 0; i < n; ++i, ++q) {
+        const int st = q % kStages;
+        if (!wait_soon(p_full, q & 1, abort_flag) || !wait_soon(&v_full[st], (q / kStages) & 1, abort_flag)) {
+          stop = true;
           break;
-        ++pieces;
-        for (uint32_t tile = p.tile0; tile < p.tile1; ++tile, ++q) {
-          const int st = q % kStages;
-          if (!wait_phase(p_full, q & 1, abort_flag) || !wait_phase(&v_full[st], (q / kStages) & 1, abort_flag)) {
-            stop = true;
-            break;
-          }
-          tc_after_sync();
+        }
+        tc_after_sync();
 #pragma unroll
-          for (int j = 0; j < kKeys / 16; ++j)
-            mma_ts(tmem + C::kOCol, tmem + (q & 1) * kKeys + j * 8, desc128(va + st * C::kTile + j * 2048, C::kBlock),
-                   kPv, tile > p.tile0 || j > 0);
-          mma_commit(&v_empty[st]);
-          mma_commit(o_full);
-          o_commits = q + 1;
-          // The scores after the next take the place of this P, once it has been read.
-          if (tile + 2 < p.tile1 && (!wait_phase(o_full, q & 1, abort_flag) || !scores(q + 2))) {
-            stop = true;
-            break;
-          }
+        for (int j = 0; j < kKeys / 16; ++j)
+          mma_ts(leader, tmem + C::kOCol, tmem + (q & 1) * kKeys + kKeys / 2 + j * 8,
+                 desc128(va + st * C::kTile + j * 2048, C::kBlock), kPv, i > 0 || j > 0);
+        commit_to(leader, o_full);
+        commit_to(leader, &v_empty[st]);
+        if (i + 1 == n) commit_to(leader, done);
+        o_commits = q + 1;
+        // The scores of the tile after the next take the place of this P, once it has
+        // been read.
+        if (!wait_soon(o_full, q & 1, abort_flag) || (i + 2 < n && !scores(q + 2))) {
+          stop = true;
+          break;
         }
       }
     }
+    if (*abort_flag && o_commits) wait_drain(o_full, (o_commits - 1) & 1, 50000000ull);  // issued MMAs end
     __syncwarp();
   } else {
     const uint32_t tl = tmem + ((uint32_t)(warp * 32) << 16);  // this warp's lanes
-    int q = 0, pieces = 0;
+    int q = 0, pieces = 0, walked = 0;  // tiles; pieces, and those with tiles
     bool stop = false;
     while (next < end && !stop) {
       Piece p;
@@ -400,13 +481,13 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         const uint32_t key0 = tile * kKeys;
         const bool masked = tile >= mask0;
         const uint32_t sc = tl + (q & 1) * kKeys;
-        if (!wait_warp(&s_full[q & 1], (q >> 1) & 1, abort_flag)) { stop = true; break; }
+        if (!wait_soon(&s_full[q & 1], (q >> 1) & 1, abort_flag)) { stop = true; break; }
         tc_after_sync();
         uint32_t v[2][32];
         tmem_ld32(sc, v[0]);
         tmem_ld32(sc + 32, v[1]);
-        tmem_wait_ld32(v[0]);
-        tmem_wait_ld32(v[1]);
+        tmem_wait(v[0]);
+        tmem_wait(v[1]);
         if (masked) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
@@ -420,51 +501,57 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         for (int i = 0; i < 64; i += 8)
 #pragma unroll
           for (int u = 0; u < 4; ++u)
-            t[u] = fmaxf(t[u], fmaxf(__uint_as_float(v[i / 32][i % 32 + 2 * u]),
-                                     __uint_as_float(v[i / 32][i % 32 + 2 * u + 1])));
-        const float top = __fmul_rn(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), a.scale_log2);
+            t[u] = max_nan(t[u], __uint_as_float(v[i / 32][i % 32 + 2 * u]),
+                           __uint_as_float(v[i / 32][i % 32 + 2 * u + 1]));
+        const float top = __fmul_rn(max_nan(max_nan(t[0], t[1], t[2]), t[3], t[3]), a.scale_log2);
         float keep = 1.f;
-        if (m == -INFINITY) {
+        if (!(top < INFINITY)) {
+          m = NAN;  // a score that is not a number or +inf: so is the row
+        } else if (m == -INFINITY) {
           m = top;  // O holds zeros at most
         } else if (top > m + F::kSlack) {
           keep = exp2_fast(m - top);
           m = top;
         }
         if (__any_sync(0xffffffffu, keep != 1.f)) {  // never in a piece's first tile
-          if (!wait_warp(o_full, (q - 1) & 1, abort_flag)) { stop = true; break; }
+          if (!wait_soon(o_full, (q - 1) & 1, abort_flag)) { stop = true; break; }
           tc_after_sync();
-          uint32_t o[32];
+          uint32_t o[16];
 #pragma unroll
-          for (int c = 0; c < kDim; c += 32) {
-            tmem_ld32(tl + C::kOCol + c, o);
-            tmem_wait_ld32(o);
+          for (int c = 0; c < kDim; c += 16) {
+            tmem_ld16(tl + C::kOCol + c, o);
+            tmem_wait(o);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__fmul_rn(__uint_as_float(o[i]), keep));
-            tmem_st32(tl + C::kOCol + c, o);
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__fmul_rn(__uint_as_float(o[i]), keep));
+            tmem_st16(tl + C::kOCol + c, o);
           }
           l2[0] = mul2(l2[0], pk(keep, keep));
           l2[1] = mul2(l2[1], pk(keep, keep));
         }
         const float base = F::kRaise - (m == -INFINITY ? 0.f : m);
         const uint64_t scale2 = pk(a.scale_log2, a.scale_log2), base2 = pk(base, base);
+        auto weigh = [&](auto mixed) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t w[16];
+          for (int c = 0; c < 2; ++c) {
+            uint32_t w[16];
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            float y0, y1;
-            unpk(fma2(pk_u(v[c][i], v[c][i + 1]), scale2, base2), y0, y1);
-            y0 = exp2_fast(y0);
-            y1 = exp2_fast(y1);
-            l2[i / 2 & 1] = add2(l2[i / 2 & 1], pk(y0, y1));
-            w[i / 2] = Elements<T>::pair(y0, y1);
+            for (int i = 0; i < 32; i += 2) {
+              uint64_t y = fma2(pk_u(v[c][i], v[c][i + 1]), scale2, base2);
+              y = decltype(mixed)::value && i % 8 == 6 ? exp2_poly<F::kDegree>(y) : exp2_pair(y);
+              l2[i / 2 & 1] = add2(l2[i / 2 & 1], y);
+              float y0, y1;
+              unpk(y, y0, y1);
+              w[i / 2] = Elements<T>::pair(y0, y1);
+            }
+            tmem_st16(sc + kKeys / 2 + 16 * c, w);  // over scores that have been read
           }
-          tmem_st16(sc + 16 * c, w);
-        }
+        };
+        if (masked) weigh(std::false_type{});
+        else weigh(std::true_type{});
         if (masked) {
           // Value rows of this tile, one per thread: zero past the keys, and without
           // what is not finite.
-          if (!wait_warp(&v_full[q % kStages], (q / kStages) & 1, abort_flag)) { stop = true; break; }
+          if (!wait_soon(&v_full[q % kStages], (q / kStages) & 1, abort_flag)) { stop = true; break; }
           if (tid < kKeys) {
             uint8_t* at = smem + C::kVOff + (q % kStages) * C::kTile + tid * 128;
             const bool past = key0 + tid >= s.len;
@@ -487,9 +574,6 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
           }
           fence_async_smem();
         }
-        // By now the products before are done; their phase is waited for at every tile,
-        // so that a wait for the next cannot take it for an older one.
-        if (q > 0 && !wait_warp(o_full, (q - 1) & 1, abort_flag)) { stop = true; break; }
         tmem_wait_st();
         tc_before_sync();
         mbar_arrive(p_full);
@@ -498,7 +582,8 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
 
       // The piece is done: O / l, or O with its maximum and sum.
       if (p.tile0 < p.tile1) {
-        if (!wait_warp(o_full, (q - 1) & 1, abort_flag)) break;
+        if (!wait_soon(done, walked & 1, abort_flag)) break;
+        ++walked;
         tc_after_sync();
       }
       float part[4];
@@ -515,7 +600,7 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         uint32_t v[32];
         if (p.tile0 < p.tile1) {
           tmem_ld32(tl + C::kOCol + c, v);
-          tmem_wait_ld32(v);
+          tmem_wait(v);
         } else {
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = 0;
@@ -566,11 +651,7 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   tc_before_sync();
   __syncthreads();
   tc_after_sync();
-  if (*abort_flag) {
-    if (warp == 4 && lane == 0 && o_commits)  // issued MMAs finish
-      wait_drain(o_full, (o_commits - 1) & 1, 50000000ull);
-    if (tid == 0) atomicOr(&g_tc_status, 1u);
-  }
+  if (*abort_flag && tid == 0) atomicOr(&g_tc_status, 1u);
   tc_before_sync();
   __syncthreads();
   tc_after_sync();
@@ -637,6 +718,7 @@ uint32_t launch(const AttnArgs& a, uint32_t grid, cudaStream_t s) {
   static std::atomic<uint64_t> configured{0};
   if (attribute_needed(configured)) {
     PB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::bytes(PB_MAX_SEQS)));
+    PB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
     attribute_done(configured);
   }
   Maps maps;
@@ -665,7 +747,9 @@ uint32_t tc_prompt(const AttnArgs& a, uint32_t type, uint32_t head_dim, cudaStre
                         : launch<__nv_bfloat16, 128, false>(a, grid, s);
 }
 
-uint64_t tc_tree_words(uint32_t head_dim) { return (uint64_t)tree_ctas(2) * 2 * kRows * (head_dim + 2); }
+uint64_t tc_tree_words(uint32_t head_dim) {
+  return (uint64_t)tree_ctas(2) * 2 * kRows * (head_dim + 2);
+}
 
 uint32_t tc_tree(const AttnArgs& a, uint32_t type, uint32_t head_dim, cudaStream_t s) {
   const uint32_t grid = tree_ctas(2);

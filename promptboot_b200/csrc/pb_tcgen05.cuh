@@ -115,6 +115,14 @@ __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, volat
 __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   return __all_sync(0xffffffffu, wait_phase(bar, parity, abort_flag));
 }
+// wait_warp for waits that are short and many: it polls before it looks at the timer,
+// whose reading takes longer than such a wait.
+__device__ __forceinline__ bool wait_soon(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  bool done = mbar_try_wait(bar, parity);
+  for (int i = 0; i < 64 && !done; ++i) done = mbar_try_wait(bar, parity);
+  if (!done) done = wait_phase_slow(bar, parity, abort_flag);
+  return __all_sync(0xffffffffu, done);
+}
 // Drain wait used on the way out: bounded by `ns`, ignores the abort flag.
 static __device__ __noinline__ void wait_drain(uint64_t* bar, uint32_t parity, uint64_t ns) {
   const uint64_t deadline = global_ns() + ns;
