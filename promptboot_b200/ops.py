@@ -21,10 +21,12 @@ from . import _lib
 from .api import DeviceError
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-_INDEX = (torch.int32, torch.uint32)
+_I32, _U32, _I64, _U64 = torch.int32, torch.uint32, torch.int64, torch.uint64
 _LAYOUTS = {False: 0, True: 1}
 _SCALINGS = {"none": 0, "linear": 1, "bands": 2, "yarn": 3}
 _ref = ctypes.byref
+_Rows = _lib.PbRows
+_empty_like = torch.empty_like
 
 
 class OperatorError(ValueError):
@@ -44,43 +46,51 @@ def _check(status: int):
     raise OperatorError(text, status)
 
 
-def _heads(t, like, name):
-    """[rows, heads, head_dim] of like's type and device, as the C ABI takes it."""
-    if t.dim() != 3 or t.stride(2) != 1:
+# A decode step makes these calls once per layer, so what they do per tensor is kept
+# to a handful of attribute reads: a device is compared by its number, a stream is
+# taken as its handle.
+if hasattr(torch._C, "_cuda_getCurrentRawStream"):
+    def _stream(device: int) -> int:
+        return torch._C._cuda_getCurrentRawStream(device)
+else:
+    def _stream(device: int) -> int:
+        return torch.cuda.current_stream(device).cuda_stream
+
+
+def _call(device: int, fn, *args):
+    """fn(*args, the device's current stream) with the device current."""
+    if device == torch.cuda.current_device():
+        status = fn(*args, _stream(device))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, _stream(device))
+    if status:
+        _check(status)
+
+
+def _heads(t, dtype, device, name):
+    """[rows, heads, head_dim] of a type and device, as the C ABI takes it."""
+    s = t.stride()
+    if len(s) != 3 or s[2] != 1:
         raise OperatorError(f"{name} must be [rows, heads, head_dim] with a contiguous last dimension")
-    if t.dtype != like.dtype or t.device != like.device:
+    if t.dtype is not dtype or t.get_device() != device:
         raise OperatorError(f"{name} has another type or device")
-    return _lib.PbRows(t.data_ptr(), t.stride(0), t.stride(1))
+    return _Rows(t.data_ptr(), s[0], s[1])
 
 
 def _first(t, name):
-    """_heads of the tensor that sets type and device."""
-    if t.dtype not in _TYPES or not t.is_cuda:
+    """(type, device) of the tensor that sets them for the others."""
+    dtype, device = t.dtype, t.get_device()
+    if dtype not in _TYPES or device < 0:
         raise OperatorError(f"{name} must be a float32, float16 or bfloat16 CUDA tensor")
-    return _heads(t, t, name)
+    return dtype, device
 
 
-def _index(t, shape, device, name, types=_INDEX):
-    if t.dtype not in types or t.device != device or not t.is_contiguous() or t.shape != shape:
-        raise OperatorError(f"{name} must be a contiguous {types[0]} tensor {list(shape)} on {device}")
+def _index(t, shape, device, name, signed=_I32, unsigned=_U32):
+    if (t.dtype is not signed and t.dtype is not unsigned) or t.get_device() != device or t.shape != shape \
+            or not t.is_contiguous():
+        raise OperatorError(f"{name} must be a contiguous {signed} tensor {list(shape)} on cuda:{device}")
     return t.data_ptr()
-
-
-class _on:
-    """The device of a call, made current where it is not, and its current stream."""
-
-    def __init__(self, device):
-        self._guard = torch.cuda.device(device) if device.index != torch.cuda.current_device() else None
-        self.stream = torch.cuda.current_stream(device).cuda_stream
-
-    def __enter__(self):
-        if self._guard is not None:
-            self._guard.__enter__()
-        return self.stream
-
-    def __exit__(self, *what):
-        if self._guard is not None:
-            self._guard.__exit__(*what)
 
 
 class PageCache:
@@ -88,16 +98,17 @@ class PageCache:
     whose layers are contiguous; it holds the tensors, not a copy."""
 
     def __init__(self, k, v):
-        if k.dim() != 5 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.device != v.device:
+        shape, strides = k.shape, k.stride()
+        if len(shape) != 5 or v.shape != shape or v.stride() != strides or v.dtype is not k.dtype \
+                or v.get_device() != k.get_device():
             raise OperatorError("k and v must be alike: [layers, pages, kv_heads, page_size, head_dim]")
-        if k.dtype not in _TYPES or not k.is_cuda:
-            raise OperatorError("a cache holds float32, float16 or bfloat16 CUDA tensors")
-        layers, pages, heads, size, dim = k.shape
-        if k.stride()[1:] != (heads * size * dim, size * dim, dim, 1):
+        self.dtype, self.device = _first(k, "a cache")
+        layers, pages, heads, size, dim = shape
+        if strides[4] != 1 or strides[3] != dim or strides[2] != size * dim or strides[1] != heads * size * dim:
             raise OperatorError("each layer of a cache must be contiguous")
         self.k, self.v = k, v
         self.pages, self.kv_heads, self.page_size, self.head_dim = pages, heads, size, dim
-        self._c = _lib.PbCache(k.data_ptr(), v.data_ptr(), k.stride(0), _TYPES[k.dtype], layers,
+        self._c = _lib.PbCache(k.data_ptr(), v.data_ptr(), strides[0], _TYPES[self.dtype], layers,
                                pages, size, heads, dim)
 
     @classmethod
@@ -109,22 +120,21 @@ class PageCache:
 
     def copy_pages(self, pairs):
         """Copies page pairs[i, 0] to page pairs[i, 1] in every layer."""
-        at = _index(pairs, (pairs.shape[0], 2), self.k.device, "pairs")
-        with _on(self.k.device) as stream:
-            _check(_lib.load().pb_cache_copy_pages_device(_ref(self._c), pairs.shape[0], at, stream))
+        n = pairs.shape[0]
+        at = _index(pairs, (n, 2), self.device, "pairs")
+        _call(self.device, _lib.load().pb_cache_copy_pages_device, _ref(self._c), n, at)
 
     def keep(self, tables, contexts, counts, nodes):
         """Moves the accepted nodes of each sequence's draft tree behind its
         context, in every layer: position contexts[s] + nodes[s, i] to contexts[s]
         + i for i < counts[s].  tables [seqs, width] as in tree_attention."""
-        device, seqs = self.k.device, contexts.shape[0]
-        a = _index(tables, (seqs, tables.shape[-1]), device, "tables")
+        device, seqs = self.device, contexts.shape[0]
+        width, most = tables.shape[-1], nodes.shape[-1]
+        a = _index(tables, (seqs, width), device, "tables")
         b = _index(contexts, (seqs,), device, "contexts")
         c = _index(counts, (seqs,), device, "counts")
-        d = _index(nodes, (seqs, nodes.shape[-1]), device, "nodes")
-        with _on(device) as stream:
-            _check(_lib.load().pb_cache_keep_device(_ref(self._c), seqs, a, tables.shape[1], b, c, d,
-                                                    nodes.shape[1], stream))
+        d = _index(nodes, (seqs, most), device, "nodes")
+        _call(device, _lib.load().pb_cache_keep_device, _ref(self._c), seqs, a, width, b, c, d, most)
 
 
 class Rotary:
@@ -152,45 +162,43 @@ class Rotary:
 
     def apply(self, q, k, positions, q_out=None, k_out=None):
         """(q, k) turned, in new tensors or in q_out and k_out, which may be q and k."""
-        q_in = _first(q, "q")
-        k_in = _heads(k, q, "k")
-        rows = q.shape[0]
-        if q.shape[2] != self.head_dim or k.shape[2] != self.head_dim or k.shape[0] != rows:
+        dtype, device = _first(q, "q")
+        q_in, k_in = _heads(q, dtype, device, "q"), _heads(k, dtype, device, "k")
+        rows, heads, dim = q.shape
+        k_rows, k_heads, k_dim = k.shape
+        if dim != self.head_dim or k_dim != dim or k_rows != rows:
             raise OperatorError("q and k must have the same rows and the plan's head_dim")
-        at = _index(positions, (rows,), q.device, "positions")
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
-        k_out = torch.empty(k.shape, dtype=q.dtype, device=q.device) if k_out is None else k_out
-        q_to, k_to = _heads(q_out, q, "q_out"), _heads(k_out, q, "k_out")
+        at = _index(positions, (rows,), device, "positions")
+        q_out = _empty_like(q) if q_out is None else q_out
+        k_out = _empty_like(k) if k_out is None else k_out
+        q_to, k_to = _heads(q_out, dtype, device, "q_out"), _heads(k_out, dtype, device, "k_out")
         if q_out.shape != q.shape or k_out.shape != k.shape:
             raise OperatorError("q_out and k_out must have the shapes of q and k")
         if rows:
-            with _on(q.device) as stream:
-                _check(_lib.load().pb_rotary_device(
-                    self._h, _TYPES[q.dtype], rows, at, q.shape[1], _ref(q_in), _ref(q_to), k.shape[1],
-                    _ref(k_in), _ref(k_to), stream))
+            _call(device, _lib.load().pb_rotary_device, self._h, _TYPES[dtype], rows, at, heads, _ref(q_in), _ref(q_to),
+                  k_heads, _ref(k_in), _ref(k_to))
         return q_out, k_out
 
     def apply_to_cache(self, q, k, v, positions, cache, slots, layer=0, q_out=None):
         """q turned, as apply; k turned and v go to `layer` of the cache at
         slots[row] = page * page_size + slot in the page (-1: nowhere)."""
-        q_in = _first(q, "q")
-        k_in, v_in = _heads(k, cache.k, "k"), _heads(v, cache.k, "v")
-        rows = q.shape[0]
-        if q.dtype != cache.k.dtype or q.device != cache.k.device or q.shape[2] != self.head_dim:
-            raise OperatorError("q must have the cache's type and device and the plan's head_dim")
-        if k.shape != (rows, cache.kv_heads, self.head_dim) or v.shape != k.shape:
+        dtype, device = cache.dtype, cache.device
+        q_in, k_in, v_in = (_heads(q, dtype, device, "q"), _heads(k, dtype, device, "k"),
+                            _heads(v, dtype, device, "v"))
+        rows, heads, dim = q.shape
+        if dim != self.head_dim:
+            raise OperatorError("q must have the plan's head_dim")
+        if k.shape != (rows, cache.kv_heads, dim) or v.shape != k.shape:
             raise OperatorError("k and v must be [rows, the cache's heads, head_dim]")
-        a = _index(positions, (rows,), q.device, "positions")
-        b = _index(slots, (rows,), q.device, "slots")
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
-        q_to = _heads(q_out, q, "q_out")
+        a = _index(positions, (rows,), device, "positions")
+        b = _index(slots, (rows,), device, "slots")
+        q_out = _empty_like(q) if q_out is None else q_out
+        q_to = _heads(q_out, dtype, device, "q_out")
         if q_out.shape != q.shape:
             raise OperatorError("q_out must have the shape of q")
         if rows:
-            with _on(q.device) as stream:
-                _check(_lib.load().pb_rotary_cache_device(
-                    self._h, rows, a, q.shape[1], _ref(q_in), _ref(q_to), _ref(k_in), _ref(v_in),
-                    _ref(cache._c), layer, b, stream))
+            _call(device, _lib.load().pb_rotary_cache_device, self._h, rows, a, heads, _ref(q_in), _ref(q_to),
+                  _ref(k_in), _ref(v_in), _ref(cache._c), layer, b)
         return q_out
 
 
@@ -199,34 +207,33 @@ def prompt_attention(q, k, v, offsets, kv_offsets=None, scale=None, out=None):
     offsets[s + 1] of q and kv_offsets[s] to kv_offsets[s + 1] (default: the same)
     of k and v, aligned at their ends.  scale defaults to head_dim ** -0.5.  Rows
     behind offsets[-1] are left as they were (unset in a new tensor)."""
-    q_in = _first(q, "q")
-    k_in, v_in = _heads(k, q, "k"), _heads(v, q, "v")
+    dtype, device = _first(q, "q")
+    q_in, k_in, v_in = _heads(q, dtype, device, "q"), _heads(k, dtype, device, "k"), _heads(v, dtype, device, "v")
     rows, heads, dim = q.shape
-    if k.shape != v.shape or k.shape[2] != dim:
+    k_rows, k_heads, k_dim = k.shape
+    if k_dim != dim or v.shape != k.shape:
         raise OperatorError("k and v must have one shape and q's head_dim")
-    seqs = offsets.shape[0] - 1
-    a = _index(offsets, (seqs + 1,), q.device, "offsets")
-    b = None if kv_offsets is None else _index(kv_offsets, (seqs + 1,), q.device, "kv_offsets")
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
-    to = _heads(out, q, "out")
+    n = offsets.shape[0]
+    a = _index(offsets, (n,), device, "offsets")
+    b = None if kv_offsets is None else _index(kv_offsets, (n,), device, "kv_offsets")
+    out = _empty_like(q) if out is None else out
+    to = _heads(out, dtype, device, "out")
     if out.shape != q.shape:
         raise OperatorError("out must have the shape of q")
-    with _on(q.device) as stream:
-        _check(_lib.load().pb_prompt_attention_device(
-            _TYPES[q.dtype], dim, heads, k.shape[1], seqs, rows, k.shape[0], _ref(q_in), _ref(k_in),
-            _ref(v_in), _ref(to), a, b, dim ** -0.5 if scale is None else scale, stream))
+    _call(device, _lib.load().pb_prompt_attention_device, _TYPES[dtype], dim, heads, k_heads, n - 1, rows, k_rows,
+          _ref(q_in), _ref(k_in), _ref(v_in), _ref(to), a, b, dim ** -0.5 if scale is None else scale)
     return out
 
 
 @functools.lru_cache(maxsize=256)
 def _workspace_bytes(device, type_, dim, heads, kv_heads, seqs, rows):
-    return int(_lib.load().pb_tree_attention_workspace(type_, dim, heads, kv_heads, seqs, rows))
+    with torch.cuda.device(device):
+        return int(_lib.load().pb_tree_attention_workspace(type_, dim, heads, kv_heads, seqs, rows))
 
 
 def tree_workspace_bytes(cache, heads, seqs, rows):
     """Bytes of workspace that tree_attention needs for these sizes."""
-    with _on(cache.k.device):
-        got = _workspace_bytes(cache.k.device.index, cache._c.type, cache.head_dim, heads, cache.kv_heads, seqs, rows)
+    got = _workspace_bytes(cache.device, _TYPES[cache.dtype], cache.head_dim, heads, cache.kv_heads, seqs, rows)
     if not got:
         raise OperatorError(_lib.last_error())
     return got
@@ -240,30 +247,29 @@ def tree_attention(q, cache, tables, contexts, offsets, visible, layer=0, scale=
     tables[s, p // page_size].  One node with visible 1 is plain decode.
     `workspace`: a uint8 tensor of tree_workspace_bytes, for calls that never
     overlap; by default one from torch's allocator."""
-    q_in = _first(q, "q")
+    dtype, device = cache.dtype, cache.device
+    q_in = _heads(q, dtype, device, "q")
     rows, heads, dim = q.shape
-    seqs = contexts.shape[0]
-    if q.dtype != cache.k.dtype or q.device != cache.k.device or dim != cache.head_dim:
-        raise OperatorError("q must have the cache's type, device and head_dim")
-    a = _index(tables, (seqs, tables.shape[-1]), q.device, "tables")
-    b = _index(contexts, (seqs,), q.device, "contexts")
-    c = _index(offsets, (seqs + 1,), q.device, "offsets")
-    d = _index(visible, (rows,), q.device, "visible", (torch.int64, torch.uint64))
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
-    to = _heads(out, q, "out")
+    if dim != cache.head_dim:
+        raise OperatorError("q must have the cache's head_dim")
+    seqs, width = contexts.shape[0], tables.shape[-1]
+    a = _index(tables, (seqs, width), device, "tables")
+    b = _index(contexts, (seqs,), device, "contexts")
+    c = _index(offsets, (seqs + 1,), device, "offsets")
+    d = _index(visible, (rows,), device, "visible", _I64, _U64)
+    out = _empty_like(q) if out is None else out
+    to = _heads(out, dtype, device, "out")
     if out.shape != q.shape:
         raise OperatorError("out must have the shape of q")
     if not rows:
         return out
-    with _on(q.device) as stream:
-        if workspace is None:
-            need = _workspace_bytes(q.device.index, cache._c.type, dim, heads, cache.kv_heads, seqs, rows)
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-        elif workspace.dtype != torch.uint8 or workspace.device != q.device or not workspace.is_contiguous():
-            raise OperatorError("workspace must be a contiguous uint8 tensor on q's device")
-        _check(_lib.load().pb_tree_attention_device(
-            _ref(cache._c), layer, heads, seqs, rows, _ref(q_in), _ref(to), a, tables.shape[1], b, c, d,
-            dim ** -0.5 if scale is None else scale, workspace.data_ptr(), workspace.numel(), stream))
+    if workspace is None:
+        need = _workspace_bytes(device, _TYPES[dtype], dim, heads, cache.kv_heads, seqs, rows)
+        workspace = torch.empty(need, dtype=torch.uint8, device=cache.k.device)
+    elif workspace.dtype is not torch.uint8 or workspace.get_device() != device or not workspace.is_contiguous():
+        raise OperatorError("workspace must be a contiguous uint8 tensor on q's device")
+    _call(device, _lib.load().pb_tree_attention_device, _ref(cache._c), layer, heads, seqs, rows, _ref(q_in),
+          _ref(to), a, width, b, c, d, dim ** -0.5 if scale is None else scale, workspace.data_ptr(), workspace.numel())
     return out
 
 
