@@ -35,6 +35,14 @@ uint32_t check_scale(const char* who, float scale) {
   return PB_OK;
 }
 
+// Row groups of 16 that hold a sequence's rows of one key head on average (1, 2 or 4),
+// 0 where they are more than 64.
+uint32_t few_tiles(uint64_t rows, uint32_t seqs) {
+  if (rows <= 16ull * seqs) return 1;
+  if (rows <= 32ull * seqs) return 2;
+  return rows <= 64ull * seqs ? 4 : 0;
+}
+
 constexpr float kLog2E = 1.4426950408889634f;
 
 }  // namespace
@@ -81,7 +89,10 @@ uint64_t pb_tree_attention_workspace(uint32_t type, uint32_t head_dim, uint32_t 
                                      uint32_t kv_heads, uint32_t seqs, uint32_t rows) {
   if (pb::paged::check_heads("pb_tree_attention_workspace", type, head_dim, q_heads, kv_heads, seqs, rows))
     return 0;
-  if (pb::paged::type_bytes(type) == 2) return pb::paged::tc_tree_words(head_dim) * 4;
+  if (pb::paged::type_bytes(type) == 2) {
+    const uint32_t tiles = pb::paged::few_tiles(rows * (q_heads / kv_heads), seqs);
+    return (tiles ? pb::paged::few_tree_words(head_dim, tiles) : pb::paged::tc_tree_words(head_dim)) * 4;
+  }
   return pb::paged::simt_tree_words(head_dim, rows * (q_heads / kv_heads), seqs) * 4;
 }
 
@@ -123,10 +134,18 @@ uint32_t pb_tree_attention_device(const pb_cache* cache, uint32_t layer, uint32_
   a.kv_heads = cache->kv_heads; a.group = (uint32_t)group; a.table_width = table_width;
   a.scale_log2 = scale * pb::paged::kLog2E;
   a.partial = static_cast<float*>(workspace);
-  if (bytes == 2) return pb::paged::tc_tree(a, cache->type, cache->head_dim, (cudaStream_t)stream);
+  if (bytes == 2) {
+    const uint32_t tiles = pb::paged::few_tiles(rows * (uint32_t)group, seqs);
+    return tiles ? pb::paged::few_tree(a, cache->type, cache->head_dim, tiles, (cudaStream_t)stream)
+                 : pb::paged::tc_tree(a, cache->type, cache->head_dim, (cudaStream_t)stream);
+  }
   return pb::paged::simt_tree(a, cache->head_dim, (cudaStream_t)stream);
 }
 
-uint32_t pb_attention_status(void* stream) { return pb::paged::tc_status((cudaStream_t)stream); }
+uint32_t pb_attention_status(void* stream) {
+  PB_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
+  const uint32_t a = pb::paged::tc_status(), b = pb::paged::few_status();
+  return a ? a : b;
+}
 
 }  // extern "C"

@@ -16,11 +16,17 @@ uint32_t simt_tree(const AttnArgs& a, uint32_t head_dim, cudaStream_t s);
 uint64_t simt_tree_words(uint32_t head_dim, uint32_t rows, uint32_t seqs);
 
 // The same on the tensor cores, for 16-bit elements; whether a wait of theirs gave
-// up since the last look (waits for the stream).
+// up since the last look.
 uint32_t tc_prompt(const AttnArgs& a, uint32_t type, uint32_t head_dim, cudaStream_t s);
 uint32_t tc_tree(const AttnArgs& a, uint32_t type, uint32_t head_dim, cudaStream_t s);
 uint64_t tc_tree_words(uint32_t head_dim);
-uint32_t tc_status(cudaStream_t s);
+uint32_t tc_status();
+
+// Tree attention of 16-bit elements with 16 * tiles rows at most on average per
+// sequence and key head (tiles 1, 2 or 4).
+uint32_t few_tree(const AttnArgs& a, uint32_t type, uint32_t head_dim, uint32_t tiles, cudaStream_t s);
+uint64_t few_tree_words(uint32_t head_dim, uint32_t tiles);
+uint32_t few_status();
 
 }  // namespace paged
 }  // namespace pb

@@ -12,6 +12,8 @@
 // maximum, sum) per run in the workspace and combine_kernel joins them.
 #pragma once
 
+#include "pb_common.cuh"
+#include "pb_kernels.cuh"
 #include "pb_paged.cuh"
 
 #include <algorithm>
@@ -146,6 +148,35 @@ struct Piece {
   int partial;  // workspace record, -1: the whole segment, straight to out
 };
 
+// Takes the next piece of a CTA's items [next, end).
+template <bool kTree, int kRows, int kKeys>
+__device__ __forceinline__ void take_piece(const AttnArgs& a, const uint32_t* prefix, uint32_t& next, uint32_t end,
+                                           Piece& p, Sequence& s, uint32_t& rows) {
+  uint32_t x = next;
+  p.seq = find_sequence(prefix, a.seqs, x);
+  s = load_sequence<kTree>(a, p.seq);
+  rows = s.t * a.group;
+  const uint32_t row_tiles = ceil_div(rows, kRows);
+  p.partial = -1;
+  if (kTree) {
+    const uint32_t tiles = max(1u, ceil_div(s.len, kKeys));
+    p.tile0 = x % tiles;
+    p.tile1 = min(tiles, p.tile0 + (end - next));
+    p.head = x / tiles / row_tiles;
+    p.row_tile = x / tiles % row_tiles;
+    if (p.tile0 > 0 || p.tile1 < tiles) p.partial = (int)(2 * blockIdx.x + (p.tile0 == 0));
+    next += p.tile1 - p.tile0;
+    if (s.len == 0) p.tile1 = p.tile0 = 0;  // nothing to see
+  } else {
+    p.head = x % a.kv_heads;
+    p.row_tile = row_tiles - 1 - x / a.kv_heads;
+    const uint32_t last = min(rows, (p.row_tile + 1) * kRows) - 1;
+    p.tile0 = 0;
+    p.tile1 = ceil_div(row_view<false>(a, s, last / a.group).all, kKeys);
+    ++next;
+  }
+}
+
 // The partial of CTA c for a segment that began before it, or that begins in it.
 __device__ __forceinline__ int partial_of(uint32_t cta, bool begins) { return (int)(2 * cta + begins); }
 
@@ -169,6 +200,7 @@ template <class T, int kDim, int kRows, int kKeys, int kLeast>
 __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ AttnArgs a, uint32_t grid) {
   extern __shared__ uint32_t prefix[];
   work_prefix<true, kRows, kKeys, 256>(a, prefix);
+  pdl_wait();  // the partials
   const uint32_t total = prefix[a.seqs - 1];
   if (total == 0) return;
   const Share<kLeast> share(total, grid);
@@ -201,7 +233,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ At
         const float mp = rec[kRows * kDim + r];
         const float w = mp == -INFINITY ? 0.f : exp2f(mp - m);
         const float4 v = *reinterpret_cast<const float4*>(rec + r * kDim + chunk);
-        if (w != 0.f) {
+        if (mp != -INFINITY) {  // a run that a row saw nothing of
           o.x = __fmaf_rn(w, v.x, o.x); o.y = __fmaf_rn(w, v.y, o.y);
           o.z = __fmaf_rn(w, v.z, o.z); o.w = __fmaf_rn(w, v.w, o.w);
           l = __fmaf_rn(w, rec[kRows * kDim + kRows + r], l);
@@ -214,6 +246,15 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ At
       store4(out, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
     }
   }
+}
+
+// The trees' second launch, which may begin while the first ends.
+template <class T, int kDim, int kRows, int kKeys, int kLeast>
+uint32_t launch_combine(const AttnArgs& a, uint32_t grid, cudaStream_t s) {
+  constexpr int kStep = 256 / (kDim / 4);
+  const dim3 join(std::min<uint32_t>(grid, 1024), kRows > kStep ? std::min(4, kRows / kStep) : 1);
+  PB_CUDA(launch_pdl(combine_kernel<T, kDim, kRows, kKeys, kLeast>, join, 256, a.seqs * 4, s, a, grid));
+  return PB_OK;
 }
 
 }  // namespace paged

@@ -5,9 +5,7 @@
 // Gimelshein's online softmax): for a tile of scores x (in powers of two),
 //   m' = max(m, max x),  o <- o 2^(m - m') + sum 2^(x - m') v,  l alike,
 // and out = o / l.
-#include "pb_attention_paged.cuh"
 #include "pb_attention_launch.h"
-#include "pb_kernels.cuh"
 
 namespace pb {
 namespace paged {
@@ -43,6 +41,7 @@ __global__ void __launch_bounds__(kThreads) attention_simt_kernel(const __grid_c
   float* ks = qs + kRows * C::kPad;
   float* vs = ks + kKeys * C::kPad;
   float* ps = vs + kKeys * C::kPad;
+  if (kTree) pdl_trigger();
   uint32_t* prefix = reinterpret_cast<uint32_t*>(ps + kRows * C::kPadP);
   work_prefix<kTree, kRows, kKeys, kThreads>(a, prefix);
   const uint32_t total = prefix[a.seqs - 1];
@@ -63,28 +62,9 @@ __global__ void __launch_bounds__(kThreads) attention_simt_kernel(const __grid_c
 
   while (next < end) {
     Piece p;
-    uint32_t x = next;
-    p.seq = find_sequence(prefix, a.seqs, x);
-    const Sequence s = load_sequence<kTree>(a, p.seq);
-    const uint32_t rows = s.t * a.group, row_tiles = ceil_div(rows, kRows);
-    p.partial = -1;
-    if (kTree) {
-      const uint32_t tiles = max(1u, ceil_div(s.len, kKeys));
-      p.tile0 = x % tiles;
-      p.tile1 = min(tiles, p.tile0 + (end - next));
-      p.head = x / tiles / row_tiles;
-      p.row_tile = x / tiles % row_tiles;
-      if (p.tile0 > 0 || p.tile1 < tiles) p.partial = partial_of(blockIdx.x, p.tile0 == 0);
-      next += p.tile1 - p.tile0;
-    } else {
-      p.head = x % a.kv_heads;
-      p.row_tile = row_tiles - 1 - x / a.kv_heads;
-      const uint32_t last = min(rows, (p.row_tile + 1) * kRows) - 1;
-      p.tile0 = 0;
-      p.tile1 = ceil_div(row_view<false>(a, s, last / a.group).all, kKeys);
-      ++next;
-    }
-
+    Sequence s;
+    uint32_t rows;
+    take_piece<kTree, kRows, kKeys>(a, prefix, next, end, p, s, rows);
     __syncthreads();  // the piece before is done with shared memory
     constexpr int kWords = kDim / 4;
     for (int i = threadIdx.x; i < kRows * kWords; i += kThreads) {
@@ -269,12 +249,7 @@ uint32_t launch(const AttnArgs& a, uint32_t grid, cudaStream_t s) {
   }
   kernel<<<grid, kThreads, C::bytes(a.seqs), s>>>(a);
   PB_CUDA(cudaGetLastError());
-  if (kTree) {
-    const dim3 join(std::min<uint32_t>(grid, 1024), C::kRows >= 32 ? 4 : 1);
-    combine_kernel<float, kDim, C::kRows, C::kKeys, kLeast><<<join, 256, a.seqs * 4, s>>>(a, grid);
-    PB_CUDA(cudaGetLastError());
-  }
-  return PB_OK;
+  return kTree ? launch_combine<float, kDim, C::kRows, C::kKeys, kLeast>(a, grid, s) : PB_OK;
 }
 
 constexpr int kFewRpt = 2, kManyRpt = 8;  // 16 or 64 rows of a tile

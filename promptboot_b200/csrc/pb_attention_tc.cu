@@ -26,42 +26,16 @@
 // by -inf; value rows past the keys are zeroed in shared memory; values that are
 // not finite are taken out there, and added to the rows that see them at the end.
 #include "pb_attention_launch.h"
-#include "pb_kernels.cuh"
-#include "pb_tcgen05.cuh"
-
-#include <cuda.h>
+#include "pb_attention_tma.cuh"
 
 namespace pb {
 namespace paged {
-
-// Set where a bounded wait of this file's kernels gave up; read and cleared by
-// tc_status.
-static __device__ unsigned int g_tc_status;
 
 namespace {
 
 constexpr int kThreads = 192;
 constexpr int kRows = 128;
 constexpr int kLeast = 2;
-
-template <class T>
-struct Format;
-template <>
-struct Format<__half> {
-  static constexpr uint32_t kCode = 0;  // instruction descriptor
-  static constexpr CUtensorMapDataType kMap = CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  static constexpr float kSlack = 4.f, kRaise = 10.f;  // weights stay below 2^14 of 65504
-  static constexpr uint32_t kExponents = 0x7c007c00u;
-  static constexpr int kDegree = 4;
-};
-template <>
-struct Format<__nv_bfloat16> {
-  static constexpr uint32_t kCode = 1;
-  static constexpr CUtensorMapDataType kMap = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  static constexpr float kSlack = 8.f, kRaise = 0.f;
-  static constexpr uint32_t kExponents = 0x7f807f80u;
-  static constexpr int kDegree = 3;
-};
 
 template <int kDim>
 struct Tc {
@@ -82,20 +56,6 @@ struct Tc {
   static size_t bytes(uint32_t seqs) { return 1024 + kPrefixOff + (size_t)seqs * 4; }
 };
 
-// One lane of the warp, for the instructions below: the whole warp runs them, with
-// that lane's predicate, so that their operands stay in uniform registers (issued from
-// a branch of one lane, four MMAs and their commit took 450 cycles).
-__device__ __forceinline__ uint32_t elect_one() {
-  uint32_t is;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "elect.sync _|p, 0xffffffff;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(is)
-      :
-      : "memory");
-  return is;
-}
 __device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
                                        uint32_t add) {
   asm volatile(
@@ -122,14 +82,6 @@ __device__ __forceinline__ void commit_to(uint32_t leader, uint64_t* bar) {
       "setp.ne.b32 e, %1, 0;\n\t"
       "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
       ::"r"(smem_u32(bar)), "r"(leader)
-      : "memory");
-}
-__device__ __forceinline__ void expect_tx(uint32_t leader, uint64_t* bar, uint32_t bytes) {
-  asm volatile(
-      "{\n\t.reg .pred e;\n\t"
-      "setp.ne.b32 e, %2, 0;\n\t"
-      "@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}"
-      ::"r"(smem_u32(bar)), "r"(bytes), "r"(leader)
       : "memory");
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
@@ -159,40 +111,12 @@ __device__ __forceinline__ void tmem_wait(uint32_t (&v)[N]) {
   for (int i = 0; i < N; ++i) asm volatile("" : "+r"(v[i]));
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-
-// TMA tile loads: the innermost coordinate is 0 or 64 elements (128 bytes).
-__device__ __forceinline__ void tma_3d(uint32_t leader, uint32_t dst, const CUtensorMap* map, int x, int y, int z,
-                                       uint64_t* bar) {
-  asm volatile(
-      "{\n\t.reg .pred e;\n\t"
-      "setp.ne.b32 e, %6, 0;\n\t"
-      "@e cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n\t}"
-      ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar)), "r"(leader)
-      : "memory");
-}
-__device__ __forceinline__ void tma_4d(uint32_t leader, uint32_t dst, const CUtensorMap* map, int x, int y, int z,
-                                       int w, uint64_t* bar) {
-  asm volatile(
-      "{\n\t.reg .pred e;\n\t"
-      "setp.ne.b32 e, %7, 0;\n\t"
-      "@e cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n\t}"
-      ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar)), "r"(leader)
-      : "memory");
-}
-
 // Shared-memory matrix descriptor, 128-byte swizzle (8 rows of 128 bytes repeat):
 // stride 1024 bytes between 8-row groups.  `lead`: bytes between 64-element column
 // blocks of an N-major operand (V); unused by K-major ones (Q, K).
 __device__ __forceinline__ uint64_t desc128(uint32_t addr, uint32_t lead) {
   return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
          (1ull << 46) | (2ull << 61);
-}
-
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 __device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
@@ -229,13 +153,6 @@ __device__ __forceinline__ uint64_t exp2_poly(uint64_t x) {
   unpk(t, t0, t1);
   return pk_u(__float_as_uint(y0) + (__float_as_uint(t0) << 23), __float_as_uint(y1) + (__float_as_uint(t1) << 23));
 }
-// The largest; not a number where one is not.
-__device__ __forceinline__ float max_nan(float a, float b, float c) {
-  float y;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-  return y;
-}
-
 // Which of the 32 keys from `key` on a row sees.
 __device__ __forceinline__ uint32_t seen32(const RowView& r, uint32_t key) {
   const uint32_t below = r.all > key ? r.all - key : 0;
@@ -249,11 +166,6 @@ __device__ __forceinline__ uint32_t seen32(const RowView& r, uint32_t key) {
   }
   return m;
 }
-
-struct Maps {
-  CUtensorMap k, v;
-  uint32_t k_step, v_step;  // 0: one key head's rows serve all
-};
 
 template <class T, int kDim, bool kTree>
 __global__ void __launch_bounds__(kThreads, 2)
@@ -277,6 +189,7 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   volatile int* dirty = abort_flag + 1;  // the last piece with a value that was taken out
   uint32_t* prefix = reinterpret_cast<uint32_t*>(smem + C::kPrefixOff);
 
+  if (kTree) pdl_trigger();
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   work_prefix<kTree, kRows, kKeys, kThreads>(a, prefix);
   const uint32_t total = prefix[a.seqs - 1];
@@ -318,32 +231,8 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
 
   // The CTA's pieces, decoded alike by every role.
   Sequence s;
-  uint32_t rows, row_tiles;
-  auto take = [&](Piece& p) {
-    uint32_t x = next;
-    p.seq = find_sequence(prefix, a.seqs, x);
-    s = load_sequence<kTree>(a, p.seq);
-    rows = s.t * a.group;
-    row_tiles = ceil_div(rows, kRows);
-    p.partial = -1;
-    if (kTree) {
-      const uint32_t tiles = max(1u, ceil_div(s.len, kKeys));
-      p.tile0 = x % tiles;
-      p.tile1 = min(tiles, p.tile0 + (end - next));
-      p.head = x / tiles / row_tiles;
-      p.row_tile = x / tiles % row_tiles;
-      if (p.tile0 > 0 || p.tile1 < tiles) p.partial = partial_of(blockIdx.x, p.tile0 == 0);
-      next += p.tile1 - p.tile0;
-      if (s.len == 0) p.tile1 = p.tile0 = 0;  // nothing to see
-    } else {
-      p.head = x % a.kv_heads;
-      p.row_tile = row_tiles - 1 - x / a.kv_heads;
-      const uint32_t last = min(rows, (p.row_tile + 1) * kRows) - 1;
-      p.tile0 = 0;
-      p.tile1 = ceil_div(row_view<false>(a, s, last / a.group).all, kKeys);
-      ++next;
-    }
-  };
+  uint32_t rows;
+  auto take = [&](Piece& p) { take_piece<kTree, kRows, kKeys>(a, prefix, next, end, p, s, rows); };
 
   int k_brought = 0, v_brought = 0, o_commits = 0;  // tiles, for the way out
 
@@ -552,26 +441,9 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
           // Value rows of this tile, one per thread: zero past the keys, and without
           // what is not finite.
           if (!wait_soon(&v_full[q % kStages], (q / kStages) & 1, abort_flag)) { stop = true; break; }
-          if (tid < kKeys) {
-            uint8_t* at = smem + C::kVOff + (q % kStages) * C::kTile + tid * 128;
-            const bool past = key0 + tid >= s.len;
-            bool found = false;
-#pragma unroll 4
-            for (int c = 0; c < kDim / 8; ++c) {
-              uint4* word = reinterpret_cast<uint4*>(at + c / 8 * C::kBlock + ((c % 8) ^ (tid & 7)) * 16);
-              uint4 x = past ? make_uint4(0, 0, 0, 0) : *word;
-              uint32_t* u = reinterpret_cast<uint32_t*>(&x);
-              bool write = past;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const uint32_t e = u[i] & F::kExponents;
-                if ((e & 0xffffu) == (F::kExponents & 0xffffu)) { u[i] &= 0xffff0000u; found = write = true; }
-                if ((e >> 16) == (F::kExponents >> 16)) { u[i] &= 0xffffu; found = write = true; }
-              }
-              if (write) *word = x;
-            }
-            if (found) *dirty = pieces;
-          }
+          if (tid < kKeys &&
+              clean_value_row<F, kDim, C::kBlock>(smem + C::kVOff + (q % kStages) * C::kTile, tid, key0 + tid >= s.len))
+            *dirty = pieces;
           fence_async_smem();
         }
         tmem_wait_st();
@@ -651,64 +523,11 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   tc_before_sync();
   __syncthreads();
   tc_after_sync();
-  if (*abort_flag && tid == 0) atomicOr(&g_tc_status, 1u);
+  if (*abort_flag && tid == 0) mark_timeout();
   tc_before_sync();
   __syncthreads();
   tc_after_sync();
   if (warp == 4) tmem_dealloc(tmem, C::kCols);
-}
-
-using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                            const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                            CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-uint32_t encoder(Encode* out) {
-  static Encode found = nullptr;
-  if (!found) {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult how;
-    PB_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &how));
-    if (how != cudaDriverEntryPointSuccess || !f) {
-      set_last_error("the driver has no cuTensorMapEncodeTiled");
-      return PB_DEVICE;
-    }
-    found = reinterpret_cast<Encode>(f);
-  }
-  *out = found;
-  return PB_OK;
-}
-
-template <class T, int kDim, bool kTree>
-uint32_t make_map(const AttnArgs& a, const pb_rows& r, const void* cache, CUtensorMap* map) {
-  using C = Tc<kDim>;
-  Encode encode = nullptr;
-  uint32_t st = encoder(&encode);
-  if (st) return st;
-  CUresult e;
-  const cuuint32_t ones[4] = {1, 1, 1, 1};
-  if (kTree) {
-    const cuuint64_t size = a.cache.page_size;
-    const cuuint64_t dims[4] = {(cuuint64_t)kDim, size, a.cache.kv_heads, a.cache.pages};
-    const cuuint64_t strides[3] = {kDim * 2, size * kDim * 2, a.cache.kv_heads * size * kDim * 2};
-    const cuuint32_t box[4] = {64, (cuuint32_t)std::min<cuuint64_t>(size, C::kKeys), 1, 1};
-    e = encode(map, Format<T>::kMap, 4, const_cast<void*>(cache), dims, strides, box, ones,
-               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  } else {
-    const bool one = a.kv_heads == 1 || r.head_stride == 0;
-    const cuuint64_t dims[3] = {(cuuint64_t)kDim, std::max(1u, a.kv_rows), one ? 1 : a.kv_heads};
-    const cuuint64_t strides[2] = {std::max<cuuint64_t>(16, r.row_stride * 2), one ? 16 : r.head_stride * 2};
-    const cuuint32_t box[3] = {64, (cuuint32_t)C::kKeys, 1};
-    e = encode(map, Format<T>::kMap, 3, r.data, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  }
-  if (e != CUDA_SUCCESS) {
-    char text[96];
-    std::snprintf(text, sizeof text, "cuTensorMapEncodeTiled refused the keys or values (error %d)", (int)e);
-    set_last_error(text);
-    return PB_DEVICE;
-  }
-  return PB_OK;
 }
 
 template <class T, int kDim, bool kTree>
@@ -721,20 +540,12 @@ uint32_t launch(const AttnArgs& a, uint32_t grid, cudaStream_t s) {
     PB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
     attribute_done(configured);
   }
-  Maps maps;
-  uint32_t st = make_map<T, kDim, kTree>(a, a.k, a.cache.k, &maps.k);
-  if (!st) st = make_map<T, kDim, kTree>(a, a.v, a.cache.v, &maps.v);
+  Maps maps{};
+  uint32_t st = kTree ? cache_maps<T>(a, kDim, C::kKeys, &maps) : rows_maps<T>(a, kDim, C::kKeys, &maps);
   if (st) return st;
-  maps.k_step = a.k.head_stride != 0;
-  maps.v_step = a.v.head_stride != 0;
   kernel<<<grid, kThreads, C::bytes(a.seqs), s>>>(a, maps);
   PB_CUDA(cudaGetLastError());
-  if (kTree) {
-    const dim3 join(std::min<uint32_t>(grid, 1024), 4);
-    combine_kernel<T, kDim, kRows, C::kKeys, kLeast><<<join, 256, a.seqs * 4, s>>>(a, grid);
-    PB_CUDA(cudaGetLastError());
-  }
-  return PB_OK;
+  return kTree ? launch_combine<T, kDim, kRows, C::kKeys, kLeast>(a, grid, s) : PB_OK;
 }
 
 }  // namespace
@@ -758,16 +569,7 @@ uint32_t tc_tree(const AttnArgs& a, uint32_t type, uint32_t head_dim, cudaStream
   return head_dim == 64 ? launch<__nv_bfloat16, 64, true>(a, grid, s) : launch<__nv_bfloat16, 128, true>(a, grid, s);
 }
 
-uint32_t tc_status(cudaStream_t s) {
-  unsigned int st = 0;
-  PB_CUDA(cudaStreamSynchronize(s));
-  PB_CUDA(cudaMemcpyFromSymbol(&st, g_tc_status, 4));
-  if (!st) return PB_OK;
-  const unsigned int zero = 0;
-  PB_CUDA(cudaMemcpyToSymbol(g_tc_status, &zero, 4));
-  set_last_error("an attention pipeline timed out waiting for a copy or an MMA");
-  return PB_DEVICE;
-}
+uint32_t tc_status() { return take_status(); }
 
 }  // namespace paged
 }  // namespace pb

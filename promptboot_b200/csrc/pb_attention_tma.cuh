@@ -1,0 +1,203 @@
+// Shared by the paged serving attention kernels that take tiles by TMA: element
+// formats, tensor maps of packed rows and of the paged cache, and small device parts.
+#pragma once
+
+#include "pb_attention_paged.cuh"
+#include "pb_tcgen05.cuh"
+
+#include <cuda.h>
+
+namespace pb {
+namespace paged {
+
+template <class T>
+struct Format;
+template <>
+struct Format<__half> {
+  static constexpr uint32_t kCode = 0;  // instruction descriptor
+  static constexpr CUtensorMapDataType kMap = CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  static constexpr float kSlack = 4.f, kRaise = 10.f;  // weights stay below 2^14 of 65504
+  static constexpr uint32_t kExponents = 0x7c007c00u;
+  static constexpr int kDegree = 4;
+};
+template <>
+struct Format<__nv_bfloat16> {
+  static constexpr uint32_t kCode = 1;
+  static constexpr CUtensorMapDataType kMap = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  static constexpr float kSlack = 8.f, kRaise = 0.f;
+  static constexpr uint32_t kExponents = 0x7f807f80u;
+  static constexpr int kDegree = 3;
+};
+
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+
+// One lane of the warp, for the instructions below: the whole warp runs them, with
+// that lane's predicate, so that their operands stay in uniform registers (issued from
+// a branch of one lane, four MMAs and their commit took 450 cycles).
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t is;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(is)
+      :
+      : "memory");
+  return is;
+}
+__device__ __forceinline__ void expect_tx(uint32_t leader, uint64_t* bar, uint32_t bytes) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "setp.ne.b32 e, %2, 0;\n\t"
+      "@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}"
+      ::"r"(smem_u32(bar)), "r"(bytes), "r"(leader)
+      : "memory");
+}
+// TMA tile loads: the innermost coordinate is 0 or 64 elements (128 bytes).
+__device__ __forceinline__ void tma_3d(uint32_t leader, uint32_t dst, const CUtensorMap* map, int x, int y, int z,
+                                       uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "setp.ne.b32 e, %6, 0;\n\t"
+      "@e cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n\t}"
+      ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar)), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void tma_4d(uint32_t leader, uint32_t dst, const CUtensorMap* map, int x, int y, int z,
+                                       int w, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "setp.ne.b32 e, %7, 0;\n\t"
+      "@e cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n\t}"
+      ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar)), "r"(leader)
+      : "memory");
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The largest; not a number where one is not.
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
+// Value row `key` of a tile in shared memory (column blocks of 128 bytes, kBlock
+// apart, 128-byte swizzle): zeroed where it is past the keys; else what is not finite
+// is zeroed.  Whether there was any.
+template <class F, int kDim, int kBlock>
+__device__ __forceinline__ bool clean_value_row(uint8_t* tile, int key, bool past) {
+  bool found = false;
+#pragma unroll 4
+  for (int c = 0; c < kDim / 8; ++c) {
+    uint4* word = reinterpret_cast<uint4*>(tile + c / 8 * kBlock + key * 128 + ((c % 8) ^ (key & 7)) * 16);
+    uint4 x = past ? make_uint4(0, 0, 0, 0) : *word;
+    uint32_t* u = reinterpret_cast<uint32_t*>(&x);
+    bool write = past;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t e = u[i] & F::kExponents;
+      if ((e & 0xffffu) == (F::kExponents & 0xffffu)) { u[i] &= 0xffff0000u; found = write = true; }
+      if ((e >> 16) == (F::kExponents >> 16)) { u[i] &= 0xffffu; found = write = true; }
+    }
+    if (write) *word = x;
+  }
+  return found;
+}
+
+// Set where a bounded wait of a kernel gave up (one word per source file).
+static __device__ unsigned int g_timeout;
+__device__ __forceinline__ void mark_timeout() { atomicOr(&g_timeout, 1u); }
+// Reads and clears it; PB_DEVICE with its text where it was set.
+static inline uint32_t take_status() {
+  unsigned int st = 0;
+  PB_CUDA(cudaMemcpyFromSymbol(&st, g_timeout, 4));
+  if (!st) return PB_OK;
+  const unsigned int zero = 0;
+  PB_CUDA(cudaMemcpyToSymbol(g_timeout, &zero, 4));
+  set_last_error("an attention pipeline timed out waiting for a copy or a product");
+  return PB_DEVICE;
+}
+
+// --------------------------------------------------------------- tensor maps (host)
+
+struct Maps {
+  CUtensorMap k, v;
+  uint32_t k_step, v_step;  // 0: one key head's rows serve all
+};
+
+using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                            const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                            CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+inline uint32_t encoder(Encode* out) {
+  static std::atomic<Encode> known{nullptr};
+  Encode found = known.load();
+  if (!found) {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult how;
+    PB_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &how));
+    if (how != cudaDriverEntryPointSuccess || !f) {
+      set_last_error("the driver has no cuTensorMapEncodeTiled");
+      return PB_DEVICE;
+    }
+    found = reinterpret_cast<Encode>(f);
+    known.store(found);
+  }
+  *out = found;
+  return PB_OK;
+}
+
+inline uint32_t encode_map(CUtensorMap* map, CUtensorMapDataType type, int rank, void* data, const cuuint64_t* dims,
+                           const cuuint64_t* strides, const cuuint32_t* box) {
+  Encode encode = nullptr;
+  uint32_t st = encoder(&encode);
+  if (st) return st;
+  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  const CUresult e = encode(map, type, rank, data, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (e == CUDA_SUCCESS) return PB_OK;
+  char text[96];
+  std::snprintf(text, sizeof text, "cuTensorMapEncodeTiled refused the keys or values (error %d)", (int)e);
+  set_last_error(text);
+  return PB_DEVICE;
+}
+
+// Keys and values of a cache layer: (element, slot, head, page), boxes of 64 elements
+// of one page's slots.
+template <class T>
+uint32_t cache_maps(const AttnArgs& a, uint32_t head_dim, uint32_t tile_keys, Maps* maps) {
+  const cuuint64_t dim = head_dim, size = a.cache.page_size;
+  const cuuint64_t dims[4] = {dim, size, a.cache.kv_heads, a.cache.pages};
+  const cuuint64_t strides[3] = {dim * 2, size * dim * 2, a.cache.kv_heads * size * dim * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)std::min<cuuint64_t>(size, tile_keys), 1, 1};
+  maps->k_step = maps->v_step = 1;
+  uint32_t st = encode_map(&maps->k, Format<T>::kMap, 4, a.cache.k, dims, strides, box);
+  if (!st) st = encode_map(&maps->v, Format<T>::kMap, 4, a.cache.v, dims, strides, box);
+  return st;
+}
+
+// Packed keys and values: (element, row, head), boxes of 64 elements of a tile's rows.
+template <class T>
+uint32_t rows_maps(const AttnArgs& a, uint32_t head_dim, uint32_t tile_keys, Maps* maps) {
+  auto one = [&](const pb_rows& r, CUtensorMap* map, uint32_t* step) {
+    const bool alone = a.kv_heads == 1 || r.head_stride == 0;
+    const cuuint64_t dims[3] = {head_dim, std::max(1u, a.kv_rows), alone ? 1 : a.kv_heads};
+    const cuuint64_t strides[2] = {std::max<cuuint64_t>(16, r.row_stride * 2), alone ? 16 : r.head_stride * 2};
+    const cuuint32_t box[3] = {64, tile_keys, 1};
+    *step = r.head_stride != 0;
+    return encode_map(map, Format<T>::kMap, 3, r.data, dims, strides, box);
+  };
+  uint32_t st = one(a.k, &maps->k, &maps->k_step);
+  if (!st) st = one(a.v, &maps->v, &maps->v_step);
+  return st;
+}
+
+}  // namespace paged
+}  // namespace pb
