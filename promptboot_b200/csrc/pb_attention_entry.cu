@@ -35,12 +35,11 @@ uint32_t check_scale(const char* who, float scale) {
   return PB_OK;
 }
 
-// Row groups of 16 that hold a sequence's rows of one key head on average (1, 2 or 4),
-// 0 where they are more than 64.
+// Row groups of 16 that hold a sequence's rows of one key head on average (1 or 2),
+// 0 where they are more than 32.
 uint32_t few_tiles(uint64_t rows, uint32_t seqs) {
   if (rows <= 16ull * seqs) return 1;
-  if (rows <= 32ull * seqs) return 2;
-  return rows <= 64ull * seqs ? 4 : 0;
+  return rows <= 32ull * seqs ? 2 : 0;
 }
 
 constexpr float kLog2E = 1.4426950408889634f;

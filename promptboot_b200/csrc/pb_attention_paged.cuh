@@ -91,27 +91,32 @@ __device__ __forceinline__ uint32_t sequence_work(const AttnArgs& a, const Seque
 }
 
 // Inclusive prefix of the sequences' work in shared memory; every thread of the
-// block calls it.  seqs <= PB_MAX_SEQS.
+// block calls it.  A thread takes consecutive sequences, so that one scan of the block
+// serves them all.  seqs <= PB_MAX_SEQS.
 template <bool kTree, int kRows, int kKeys, int kThreads>
 __device__ __forceinline__ void work_prefix(const AttnArgs& a, uint32_t* prefix) {
   __shared__ uint32_t warp_sum[kThreads / 32];
-  uint32_t base = 0;
-  for (uint32_t s0 = 0; s0 < a.seqs; s0 += kThreads) {
-    const uint32_t s = s0 + threadIdx.x;
-    uint32_t w = s < a.seqs ? sequence_work<kTree, kRows, kKeys>(a, load_sequence<kTree>(a, s)) : 0;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const uint32_t o = __shfl_up_sync(0xffffffffu, w, d);
-      if ((threadIdx.x & 31) >= d) w += o;
-    }
-    if ((threadIdx.x & 31) == 31) warp_sum[threadIdx.x >> 5] = w;
-    __syncthreads();
-    uint32_t before = base;
-    for (int i = 0; i < (int)(threadIdx.x >> 5); ++i) before += warp_sum[i];
-    if (s < a.seqs) prefix[s] = before + w;
-    for (int i = 0; i < kThreads / 32; ++i) base += warp_sum[i];
-    __syncthreads();
+  const uint32_t each = ceil_div(a.seqs, kThreads), first = threadIdx.x * each;
+  const uint32_t last = min(a.seqs, first + each);
+  uint32_t sum = 0;
+#pragma unroll 4
+  for (uint32_t s = first; s < last; ++s) {
+    sum += sequence_work<kTree, kRows, kKeys>(a, load_sequence<kTree>(a, s));
+    prefix[s] = sum;
   }
+  uint32_t scan = sum;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const uint32_t o = __shfl_up_sync(0xffffffffu, scan, d);
+    if ((threadIdx.x & 31) >= d) scan += o;
+  }
+  if ((threadIdx.x & 31) == 31) warp_sum[threadIdx.x >> 5] = scan;
+  __syncthreads();
+  uint32_t before = scan - sum;
+  for (int i = 0; i < (int)(threadIdx.x >> 5); ++i) before += warp_sum[i];
+  if (before)
+    for (uint32_t s = first; s < last; ++s) prefix[s] += before;
+  __syncthreads();
 }
 
 // The sequence that holds item x of the prefix, and x within it.
@@ -194,57 +199,74 @@ __host__ __device__ constexpr size_t partial_words() {
 }
 
 // Joins the partials of the segments that crossed CTA runs: weights 2^(m_i - m),
-// in the order of the runs, so the result does not depend on timing.  One CTA per
-// (possible segment, kDim / 4 threads per row x 256 / (kDim / 4) rows).
+// in the order of the runs, so the result does not depend on timing.  A segment
+// is joined by the CTAs (four at most, so that one wave of them holds all) of the edge
+// at the end of the run in which it begins.  A thread has four elements of a row and
+// loads eight partials at a time: latency is what there is to save here.
 template <class T, int kDim, int kRows, int kKeys, int kLeast>
 __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ AttnArgs a, uint32_t grid) {
   extern __shared__ uint32_t prefix[];
   work_prefix<true, kRows, kKeys, 256>(a, prefix);
-  pdl_wait();  // the partials
-  const uint32_t total = prefix[a.seqs - 1];
-  if (total == 0) return;
-  const Share<kLeast> share(total, grid);
-  constexpr int kPerRow = kDim / 4, kStep = 256 / kPerRow;
-  // gridDim.x CTAs walk the runs' boundaries: a segment that crosses them is joined
-  // by the CTA of the run in which it begins.
-  for (uint32_t c = blockIdx.x; c + 1 < share.ctas; c += gridDim.x) {
-    const uint32_t edge = share.start(c + 1);
-    uint32_t x = edge;
-    const uint32_t seq = find_sequence(prefix, a.seqs, x);
-    const Sequence s = load_sequence<true>(a, seq);
-    const uint32_t tiles = max(1u, ceil_div(s.len, kKeys));
-    const uint32_t begin = edge - x % tiles;
-    // begins at the edge, or in an earlier run than c
-    if (begin == edge || begin < share.start(c)) continue;
-    const uint32_t segment = x / tiles, last = share.holder(begin + tiles - 1);
-    const uint32_t row_tiles = ceil_div(s.t * a.group, kRows);
-    const uint32_t head = segment / row_tiles, row_tile = segment % row_tiles;
-    const int chunk = (threadIdx.x % kPerRow) * 4;
-    for (uint32_t r = blockIdx.y * kStep + threadIdx.x / kPerRow; r < kRows; r += gridDim.y * kStep) {
-      const uint32_t row = row_tile * kRows + r;
-      if (row >= s.t * a.group) break;
-      float m = -INFINITY;
-      for (uint32_t p = c; p <= last; ++p)
-        m = fmaxf(m, a.partial[partial_of(p, p == c) * partial_words<kRows, kDim>() + kRows * kDim + r]);
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-      float l = 0.f;
-      for (uint32_t p = c; p <= last; ++p) {
-        const float* rec = a.partial + partial_of(p, p == c) * partial_words<kRows, kDim>();
-        const float mp = rec[kRows * kDim + r];
-        const float w = mp == -INFINITY ? 0.f : exp2f(mp - m);
-        const float4 v = *reinterpret_cast<const float4*>(rec + r * kDim + chunk);
-        if (mp != -INFINITY) {  // a run that a row saw nothing of
-          o.x = __fmaf_rn(w, v.x, o.x); o.y = __fmaf_rn(w, v.y, o.y);
-          o.z = __fmaf_rn(w, v.z, o.z); o.w = __fmaf_rn(w, v.w, o.w);
-          l = __fmaf_rn(w, rec[kRows * kDim + kRows + r], l);
+  const uint32_t total = prefix[a.seqs - 1], c = blockIdx.x;
+  const Share<kLeast> share(max(1u, total), grid);
+  bool mine = total > 0 && c + 1 < share.ctas;
+  uint32_t edge = 0, begin = 0, seq = 0, x = 0, tiles = 1;
+  Sequence s{};
+  if (mine) {
+    x = edge = share.start(c + 1);
+    seq = find_sequence(prefix, a.seqs, x);
+    s = load_sequence<true>(a, seq);
+    tiles = max(1u, ceil_div(s.len, kKeys));
+    begin = edge - x % tiles;
+    mine = begin != edge && begin >= share.start(c);  // else it begins at the edge, or in an earlier run
+  }
+  pdl_wait();  // the partials; also in a CTA that has none, for what comes after this launch
+  if (!mine) return;
+  constexpr int kPerRow = kDim / 4, kStep = 256 / kPerRow, kBatch = 8;
+  const uint32_t last = share.holder(begin + tiles - 1);
+  const uint32_t row_tiles = ceil_div(s.t * a.group, kRows);
+  const uint32_t head = x / tiles / row_tiles, row_tile = x / tiles % row_tiles;
+  const int chunk = (threadIdx.x % kPerRow) * 4;
+  for (uint32_t r = blockIdx.y * kStep + threadIdx.x / kPerRow; r < kRows; r += gridDim.y * kStep) {
+    const uint32_t row = row_tile * kRows + r;
+    if (row >= s.t * a.group) return;
+    float m = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (uint32_t p0 = c; p0 <= last; p0 += kBatch) {
+      float mp[kBatch], lp[kBatch];
+      float4 op[kBatch];
+      float to = m;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        mp[i] = -INFINITY;
+        if (p0 + i <= last) {
+          const float* rec = a.partial + partial_of(p0 + i, p0 + i == c) * partial_words<kRows, kDim>();
+          mp[i] = rec[kRows * kDim + r];
+          lp[i] = rec[kRows * kDim + kRows + r];
+          op[i] = *reinterpret_cast<const float4*>(rec + r * kDim + chunk);
         }
       }
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      const uint32_t token = row / a.group, h = head * a.group + row % a.group;
-      T* out = static_cast<T*>(a.out.data) + (uint64_t)(s.q0 + token) * a.out.row_stride +
-               h * a.out.head_stride + chunk;
-      store4(out, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) to = fmaxf(to, mp[i]);
+      const float old = m == -INFINITY ? 0.f : exp2f(m - to);
+      m = to;
+      l = __fmul_rn(l, old);
+      o.x = __fmul_rn(o.x, old); o.y = __fmul_rn(o.y, old);
+      o.z = __fmul_rn(o.z, old); o.w = __fmul_rn(o.w, old);
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        if (mp[i] == -INFINITY) continue;  // no run, or one of which the row saw nothing
+        const float w = exp2f(mp[i] - m);
+        o.x = __fmaf_rn(w, op[i].x, o.x); o.y = __fmaf_rn(w, op[i].y, o.y);
+        o.z = __fmaf_rn(w, op[i].z, o.z); o.w = __fmaf_rn(w, op[i].w, o.w);
+        l = __fmaf_rn(w, lp[i], l);
+      }
     }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const uint32_t token = row / a.group, h = head * a.group + row % a.group;
+    T* out = static_cast<T*>(a.out.data) + (uint64_t)(s.q0 + token) * a.out.row_stride +
+             h * a.out.head_stride + chunk;
+    store4(out, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
   }
 }
 
@@ -252,7 +274,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ At
 template <class T, int kDim, int kRows, int kKeys, int kLeast>
 uint32_t launch_combine(const AttnArgs& a, uint32_t grid, cudaStream_t s) {
   constexpr int kStep = 256 / (kDim / 4);
-  const dim3 join(std::min<uint32_t>(grid, 1024), kRows > kStep ? std::min(4, kRows / kStep) : 1);
+  const dim3 join(grid, std::min(4, (kRows + kStep - 1) / kStep));
   PB_CUDA(launch_pdl(combine_kernel<T, kDim, kRows, kKeys, kLeast>, join, 256, a.seqs * 4, s, a, grid));
   return PB_OK;
 }

@@ -49,66 +49,98 @@ struct KeepArgs {
   uint64_t layer_bytes;
   uint32_t layers, pages, page_size, kv_heads, row_words;
   const uint32_t *tables, *contexts, *counts, *nodes;
-  uint32_t table_width, nodes_width, seqs;
-  uint64_t columns;  // seqs * layers * 2 * kv_heads * row_words
+  uint32_t table_width, nodes_width;
+  uint32_t columns;  // layers * 2 * kv_heads * row_words
 };
 
-// One thread per (sequence, layer, keys or values, head, 16-byte word of a row):
-// it makes all of its column's moves by itself, so the moves of a sequence need no
-// order between threads.  Within a column the kept node indices n_i ascend and
-// n_i >= i, so target i never equals the source of a later move (n_k > n_i >= i):
-// sources are read kBatch at a time before their targets are written.
-constexpr int kBatch = 8;
-__global__ void __launch_bounds__(128) keep_kernel(KeepArgs a) {
-  const uint64_t t = (uint64_t)blockIdx.x * 128 + threadIdx.x;
-  if (t >= a.columns) return;
-  const uint32_t word = (uint32_t)(t % a.row_words);
-  uint64_t rest = t / a.row_words;
-  const uint32_t head = (uint32_t)(rest % a.kv_heads);
-  rest /= a.kv_heads;
-  const uint32_t side = (uint32_t)(rest & 1);
-  rest >>= 1;
-  const uint32_t layer = (uint32_t)(rest % a.layers);
-  const uint32_t seq = (uint32_t)(rest / a.layers);
-  uint4* base = reinterpret_cast<uint4*>((side ? a.v : a.k) + layer * a.layer_bytes) + word;
+// One CTA per sequence and 128 of its columns (layer, keys or values, head, 16-byte
+// word of a row).  Its threads first work out the moves together, each a source and a
+// target row, then each makes all moves of its column by itself, so that the moves
+// need no order between threads.  Within a column the kept node indices n_i ascend
+// and n_i >= i, so target i never equals the source of a later move (n_k > n_i >= i):
+// sources are read kBatch at a time before their targets are written.  Bound by the
+// latency of its three dependent loads (node, page, row) where it is small, else by
+// memory.
+constexpr int kBatch = 8, kMoves = 128;
+__global__ void __launch_bounds__(128) keep_kernel(const __grid_constant__ KeepArgs a) {
+  __shared__ uint32_t sources[kMoves], targets[kMoves];  // rows of head 0 in units of page slots; PB_NONE: no move
+  __shared__ uint32_t warp_top[4], warp_moves[4];
+  const uint32_t seq = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t column = blockIdx.x * 128 + tid;
   const uint32_t* table = a.tables + (uint64_t)seq * a.table_width;
   const uint32_t* nodes = a.nodes + (uint64_t)seq * a.nodes_width;
-  const uint64_t context = a.contexts[seq];
   const uint64_t reach = (uint64_t)a.table_width * a.page_size;
-  const uint32_t count = min(a.counts[seq], a.nodes_width);
-  auto row = [&](uint64_t position) -> uint4* {
-    if (position >= reach) return nullptr;
-    const uint32_t page = table[position / a.page_size];
-    if (page >= a.pages) return nullptr;
-    return base + (((uint64_t)page * a.kv_heads + head) * a.page_size + position % a.page_size) *
-                      a.row_words;
-  };
-  int64_t last = -1;  // the node before
-  for (uint32_t i0 = 0; i0 < count; i0 += kBatch) {
-    uint4 w[kBatch];
-    uint4* to[kBatch];
+  const uint32_t word = column % a.row_words;
+  uint32_t rest = column / a.row_words;
+  const uint32_t head = rest % a.kv_heads;
+  rest /= a.kv_heads;
+  uint4* base = reinterpret_cast<uint4*>((rest & 1 ? a.v : a.k) + (rest >> 1) * a.layer_bytes) +
+                (uint64_t)head * a.page_size * a.row_words + word;
+  int64_t top = -1;  // the largest node so far
+  uint32_t count = 0xffffffffu;
+  for (uint32_t i0 = 0; i0 < a.nodes_width && i0 < count; i0 += kMoves) {
+    const uint32_t i = i0 + tid;
+    const int64_t n = i < a.nodes_width ? (int64_t)nodes[i] : -1;
+    const uint64_t context = a.contexts[seq];
+    count = a.counts[seq];
+    // the largest node before this one, over the warp and then the block
+    int64_t before = n;
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      const uint32_t i = i0 + j;
-      to[j] = nullptr;
-      if (i < count) {
-        const int64_t n = nodes[i];
-        if (n > last && n >= (int64_t)i) {
-          last = n;
-          if (n != (int64_t)i) {
-            const uint4* from = row(context + (uint64_t)n);
-            uint4* target = row(context + i);
-            if (from && target) {
-              w[j] = *from;
-              to[j] = target;
-            }
-          }
-        }
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t o = __shfl_up_sync(0xffffffffu, before, d);
+      if (lane >= d) before = max(before, o);
+    }
+    __syncthreads();  // the moves before have been read
+    if (lane == 31) warp_top[warp] = (uint32_t)max((int64_t)0, before + 1);
+    int64_t up_to = __shfl_up_sync(0xffffffffu, before, 1);
+    if (lane == 0) up_to = -1;
+    __syncthreads();
+    up_to = max(up_to, top);
+    for (uint32_t w = 0; w < 4; ++w) {
+      const int64_t x = (int64_t)warp_top[w] - 1;
+      if (w < warp) up_to = max(up_to, x);
+      top = max(top, x);
+    }
+    bool move = i < count && i < a.nodes_width && n > (int64_t)i && n > up_to;  // n = i stays where it is
+    uint32_t from = PB_NONE, to = PB_NONE;
+    if (move && context + (uint64_t)n < reach) {
+      const uint64_t src = context + (uint64_t)n, dst = context + i;
+      const uint32_t p0 = table[src / a.page_size], p1 = table[dst / a.page_size];
+      if (p0 < a.pages && p1 < a.pages) {
+        from = p0 * a.page_size + (uint32_t)(src % a.page_size);
+        to = p1 * a.page_size + (uint32_t)(dst % a.page_size);
       }
     }
+    // only the moves, in their order
+    move = from != PB_NONE;
+    const uint32_t vote = __ballot_sync(0xffffffffu, move);
+    if (lane == 0) warp_moves[warp] = __popc(vote);
+    __syncthreads();
+    uint32_t at = __popc(vote & ((1u << lane) - 1u)), moves = 0;
+    for (uint32_t w = 0; w < 4; ++w) {
+      if (w < warp) at += warp_moves[w];
+      moves += warp_moves[w];
+    }
+    if (move) {
+      sources[at] = from;
+      targets[at] = to;
+    }
+    __syncthreads();
+    if (column < a.columns) {
+      auto row = [&](uint32_t spot) -> uint4* {
+        const uint32_t page = spot / a.page_size;
+        return base + ((uint64_t)page * a.kv_heads * a.page_size + spot % a.page_size) * a.row_words;
+      };
+      for (uint32_t m0 = 0; m0 < moves; m0 += kBatch) {
+        uint4 w[kBatch];
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j)
-      if (to[j]) *to[j] = w[j];
+        for (int j = 0; j < kBatch; ++j)
+          if (m0 + j < moves) w[j] = *row(sources[m0 + j]);
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j)
+          if (m0 + j < moves) *row(targets[m0 + j]) = w[j];
+      }
+    }
   }
 }
 
@@ -185,11 +217,19 @@ uint32_t pb_cache_keep_device(const pb_cache* cache, uint32_t seqs, const uint32
   a.layers = cache->layers; a.pages = cache->pages; a.page_size = cache->page_size;
   a.kv_heads = cache->kv_heads; a.row_words = cache->head_dim * bytes / 16;
   a.tables = tables; a.contexts = contexts; a.counts = counts; a.nodes = nodes;
-  a.table_width = table_width; a.nodes_width = nodes_width; a.seqs = seqs;
-  a.columns = (uint64_t)seqs * a.layers * 2 * a.kv_heads * a.row_words;
-  const uint64_t grid = (a.columns + 127) / 128;
-  if (grid > 0x7fffffffu) return pb::paged::refuse(PB_CAPACITY, who, "too many sequences");
-  pb::keep_kernel<<<(uint32_t)grid, 128, 0, (cudaStream_t)stream>>>(a);
+  a.table_width = table_width; a.nodes_width = nodes_width;
+  const uint64_t columns = (uint64_t)a.layers * 2 * a.kv_heads * a.row_words;
+  if (columns >= 1u << 31) return pb::paged::refuse(PB_CAPACITY, who, "too many layers");
+  a.columns = (uint32_t)columns;
+  // grid.y holds 65535 sequences: further ones in further launches
+  for (uint32_t s0 = 0; s0 < seqs; s0 += 65535) {
+    const uint32_t n = std::min<uint32_t>(65535, seqs - s0);
+    pb::keep_kernel<<<dim3((a.columns + 127) / 128, n), 128, 0, (cudaStream_t)stream>>>(a);
+    a.tables += (uint64_t)n * table_width;
+    a.contexts += n;
+    a.counts += n;
+    a.nodes += (uint64_t)n * nodes_width;
+  }
   PB_CUDA(cudaGetLastError());
   return PB_OK;
 }
