@@ -252,8 +252,8 @@ attention_few_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__
           for (int r = 0; r < kShare; r += 32) {
             const int key = k0 + r + lane;
             if (r + lane < kShare)
-              if (clean_value_row<F, kDim, C::kBlock>(smem + st * 2 * C::kTile + C::kTile, key, tile * kKeys + key >= s.len))
-                *dirty = pieces;
+              clean_value_row<F, kDim, C::kBlock>(smem + st * 2 * C::kTile + C::kTile, key, tile * kKeys + key >= s.len,
+                                                  dirty, pieces);
           }
           __syncwarp();
         }
@@ -411,9 +411,8 @@ uint32_t launch(const AttnArgs& a, cudaStream_t s) {
 
 template <class T>
 uint32_t by_size(const AttnArgs& a, uint32_t head_dim, uint32_t tiles, cudaStream_t s) {
-  if (head_dim == 64)
-    return tiles == 1 ? launch<T, 64, 1>(a, s) : tiles == 2 ? launch<T, 64, 2>(a, s) : launch<T, 64, 4>(a, s);
-  return tiles == 1 ? launch<T, 128, 1>(a, s) : tiles == 2 ? launch<T, 128, 2>(a, s) : launch<T, 128, 4>(a, s);
+  if (head_dim == 64) return tiles == 1 ? launch<T, 64, 1>(a, s) : launch<T, 64, 2>(a, s);
+  return tiles == 1 ? launch<T, 128, 1>(a, s) : launch<T, 128, 2>(a, s);
 }
 
 }  // namespace
