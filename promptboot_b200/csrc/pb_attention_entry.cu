@@ -89,8 +89,8 @@ uint64_t pb_tree_attention_workspace(uint32_t type, uint32_t head_dim, uint32_t 
   if (pb::paged::check_heads("pb_tree_attention_workspace", type, head_dim, q_heads, kv_heads, seqs, rows))
     return 0;
   if (pb::paged::type_bytes(type) == 2) {
-    const uint32_t all = rows * (q_heads / kv_heads), tiles = pb::paged::few_tiles(all, seqs);
-    return (tiles ? pb::paged::few_tree_words(head_dim, tiles) : pb::paged::tc_tree_words(head_dim, all, seqs)) * 4;
+    const uint32_t tiles = pb::paged::few_tiles(rows * (q_heads / kv_heads), seqs);
+    return (tiles ? pb::paged::few_tree_words(head_dim, tiles) : pb::paged::tc_tree_words(head_dim)) * 4;
   }
   return pb::paged::simt_tree_words(head_dim, rows * (q_heads / kv_heads), seqs) * 4;
 }

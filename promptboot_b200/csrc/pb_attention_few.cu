@@ -252,8 +252,8 @@ attention_few_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__
           for (int r = 0; r < kShare; r += 32) {
             const int key = k0 + r + lane;
             if (r + lane < kShare)
-              clean_value_row<F, kDim, C::kBlock>(smem + st * 2 * C::kTile + C::kTile, key, tile * kKeys + key >= s.len,
-                                                  dirty, pieces);
+              if (clean_value_row<F, kDim, C::kBlock>(smem + st * 2 * C::kTile + C::kTile, key, tile * kKeys + key >= s.len))
+                *dirty = pieces;
           }
           __syncwarp();
         }

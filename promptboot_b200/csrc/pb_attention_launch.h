@@ -19,7 +19,7 @@ uint64_t simt_tree_words(uint32_t head_dim, uint32_t rows, uint32_t seqs);
 // up since the last look.
 uint32_t tc_prompt(const AttnArgs& a, uint32_t type, uint32_t head_dim, cudaStream_t s);
 uint32_t tc_tree(const AttnArgs& a, uint32_t type, uint32_t head_dim, cudaStream_t s);
-uint64_t tc_tree_words(uint32_t head_dim, uint32_t rows, uint32_t seqs);
+uint64_t tc_tree_words(uint32_t head_dim);
 uint32_t tc_status();
 
 // Tree attention of 16-bit elements with 16 * tiles rows at most on average per

@@ -8,17 +8,14 @@
 // The weights' sum adds the unrounded weights, so P's rounding is one more half
 // step of the type per weight and averages out over the keys.
 //
-// A CTA has kGroups row tiles, which share the K and V tiles that pass by.  Each has
-// four softmax warps, one row per thread (TMEM lane = row), and a warp that issues its
-// MMAs; one more warp brings K and V tiles by TMA (128-byte swizzle) into rings of
-// kStages.  S, P and O have TMEM columns of their own: the scores of the next tile go
-// out as soon as those of this one are in registers, under its exponentials.
-//
-// Bound by the softmax warps: per key and row an exponential (16 a cycle and SM) and
-// some five other instructions, in dependent chains that one or two warps per
-// scheduler leave half idle (50% issue).  So three row tiles at heads of 64 (480 of
-// 512 TMEM columns, one CTA per SM, three softmax warps per scheduler) where a sequence
-// fills them, else one row tile and two CTAs per SM.
+// Warps: 0..3 softmax, one row per thread (TMEM lane = row); 4 issues the MMAs;
+// 5 brings K and V tiles by TMA (128-byte swizzle) into rings of kStages.  S has two
+// buffers in TMEM, P takes the place of the upper half of the scores it comes from: the
+// scores of tile j + 2 go out when the products of tile j are done, a tile ahead of
+// their softmax, which therefore seldom waits.  256 TMEM columns, so two CTAs share an
+// SM and one's products run under the other's exponentials.  (Four CTAs of one score
+// buffer each measured the same at heads of 64: the SM's 16 exponentials a cycle bind
+// both.)
 //
 // The running maximum is the one in use until a row's true maximum passes it by
 // 2^kSlack: O is rescaled (through registers) only then, seldom after the first
@@ -36,29 +33,26 @@ namespace paged {
 
 namespace {
 
-constexpr int kRowTile = 128;  // rows of one MMA
-constexpr int kKeys = 64;
+constexpr int kThreads = 192;
+constexpr int kRows = 128;
 constexpr int kLeast = 2;
 
-template <int kDim, int kGroups>
+template <int kDim>
 struct Tc {
-  static constexpr int kRows = kGroups * kRowTile;
-  static constexpr int kThreads = 32 * (5 * kGroups + 1);
-  static constexpr int kCtas = kGroups == 1 ? 2 : 1;  // per SM
-  static constexpr int kStages = kGroups > 1 ? 5 : kDim == 64 ? 4 : 2;
-  static constexpr int kHalves = kDim / 64;            // 128-byte column blocks of a row
-  static constexpr int kQBlock = kRowTile * 128;
-  static constexpr int kQ = kHalves * kQBlock;         // Q of one row tile
-  static constexpr int kBlock = kKeys * 128;           // one column block of a K or V tile
+  static constexpr int kKeys = 64;
+  static constexpr int kStages = kDim == 64 ? 4 : 2;
+  static constexpr int kHalves = kDim / 64;           // 128-byte column blocks of a row
+  static constexpr int kQBlock = kRows * 128;
+  static constexpr int kBlock = kKeys * 128;          // one column block of a K or V tile
   static constexpr int kTile = kHalves * kBlock;
-  static constexpr int kKOff = kGroups * kQ;
+  static constexpr int kKOff = kHalves * kQBlock;
   static constexpr int kVOff = kKOff + kStages * kTile;
   static constexpr int kBarOff = kVOff + kStages * kTile;
-  static constexpr int kBars = 4 * kStages + 6 * kGroups;
+  static constexpr int kBars = 4 * kStages + 6;
   static constexpr int kPrefixOff = kBarOff + kBars * 8 + 16;
-  static constexpr int kPCol = kKeys, kOCol = kKeys + kKeys / 2, kGroupCols = kOCol + kDim;
-  static constexpr int kCols = kCtas == 2 ? 256 : 512;
-  static_assert(kGroups * kGroupCols <= kCols, "TMEM columns");
+  static constexpr int kOCol = 2 * kKeys;             // S and P: [0, 64) and [64, 128)
+  static constexpr int kCols = 256;
+  static_assert(kOCol + kDim <= kCols, "TMEM columns");
   static size_t bytes(uint32_t seqs) { return 1024 + kPrefixOff + (size_t)seqs * 4; }
 };
 
@@ -173,27 +167,31 @@ __device__ __forceinline__ uint32_t seen32(const RowView& r, uint32_t key) {
   return m;
 }
 
-template <class T, int kDim, int kGroups, bool kTree>
-__global__ void __launch_bounds__(Tc<kDim, kGroups>::kThreads, Tc<kDim, kGroups>::kCtas)
+template <class T, int kDim, bool kTree>
+__global__ void __launch_bounds__(kThreads, 2)
 attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Maps maps) {
-  using C = Tc<kDim, kGroups>;
+  using C = Tc<kDim>;
   using F = Format<T>;
-  constexpr int kRows = C::kRows, kStages = C::kStages, kHalves = C::kHalves;
+  constexpr int kKeys = C::kKeys, kStages = C::kStages, kHalves = C::kHalves;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
   uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
   uint64_t* k_empty = k_full + kStages;
   uint64_t* v_full = k_empty + kStages;
   uint64_t* v_empty = v_full + kStages;
-  uint64_t* groups = v_empty + kStages;  // six per row tile
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(groups + 6 * kGroups);
+  uint64_t* q_full = v_empty + kStages;
+  uint64_t* p_full = q_full + 1;
+  uint64_t* o_full = p_full + 1;  // O holds the tile's products, its P is free
+  uint64_t* done = o_full + 1;    // O holds the piece's
+  uint64_t* s_full = done + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* dirty = abort_flag + 1;  // the last piece with a value that was taken out
   uint32_t* prefix = reinterpret_cast<uint32_t*>(smem + C::kPrefixOff);
 
   if (kTree) pdl_trigger();
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-  work_prefix<kTree, kRows, kKeys, C::kThreads>(a, prefix);
+  work_prefix<kTree, kRows, kKeys, kThreads>(a, prefix);
   const uint32_t total = prefix[a.seqs - 1];
   uint32_t next, end;
   if (kTree) {
@@ -208,22 +206,20 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     end = next + 1;
   }
 
-  if (warp == 0) tmem_alloc(tmem_slot, C::kCols);
-  if (tid == 32) {
+  if (warp == 4) tmem_alloc(tmem_slot, C::kCols);
+  if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&k_full[i], 1);
-      mbar_init(&k_empty[i], kGroups);
+      mbar_init(&k_empty[i], 1);
       mbar_init(&v_full[i], 1);
-      mbar_init(&v_empty[i], kGroups);
+      mbar_init(&v_empty[i], 1);
     }
-    for (int g = 0; g < kGroups; ++g) {
-      mbar_init(&groups[6 * g], 4);
-      mbar_init(&groups[6 * g + 1], 1);
-      mbar_init(&groups[6 * g + 2], 4);
-      mbar_init(&groups[6 * g + 3], 4);
-      mbar_init(&groups[6 * g + 4], 1);
-      mbar_init(&groups[6 * g + 5], 1);
-    }
+    mbar_init(q_full, kRows);
+    mbar_init(&s_full[0], 1);
+    mbar_init(&s_full[1], 1);
+    mbar_init(p_full, kRows);
+    mbar_init(o_full, 1);
+    mbar_init(done, 1);
     *abort_flag = 0;
     *dirty = 0;
     fence_barrier_init();
@@ -231,36 +227,20 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   tc_before_sync();
   __syncthreads();
   tc_after_sync();
+  const uint32_t tmem = *tmem_slot;
 
-  // The row tile of a softmax or MMA warp: its TMEM columns and barriers.
-  const int group = warp < 4 * kGroups ? warp >> 2 : min(warp - 4 * kGroups, kGroups - 1);
-  const uint32_t tmem = *tmem_slot + group * C::kGroupCols;
-  uint64_t* q_full = groups + 6 * group;  // Q is in shared memory
-  uint64_t* s_full = q_full + 1;          // S holds a tile's scores
-  uint64_t* s_free = q_full + 2;          // they are in registers
-  uint64_t* p_full = q_full + 3;          // P holds its weights
-  uint64_t* o_full = q_full + 4;          // O holds its products, P is free
-  uint64_t* drained = q_full + 5;         // on the way out: every issued MMA has ended
-
-  // The CTA's pieces, decoded alike by every role; and the last key tile that some row
-  // of this row tile sees.
+  // The CTA's pieces, decoded alike by every role.
   Sequence s;
   uint32_t rows;
   auto take = [&](Piece& p) { take_piece<kTree, kRows, kKeys>(a, prefix, next, end, p, s, rows); };
-  auto first_row = [&](const Piece& p) { return p.row_tile * kRows + group * kRowTile; };
-  auto tiles_of = [&](const Piece& p) {
-    const uint32_t r0 = first_row(p);
-    if (r0 >= rows) return p.tile0;
-    if (kTree) return p.tile1;
-    const uint32_t last = min(rows, r0 + kRowTile) - 1;
-    return min(p.tile1, ceil_div(row_view<false>(a, s, last / a.group).all, kKeys));
-  };
 
-  if (warp == 5 * kGroups) {
+  int k_brought = 0, v_brought = 0, o_commits = 0;  // tiles, for the way out
+
+  if (warp == 5) {
     const uint32_t leader = elect_one();
     const uint32_t size = kTree ? min(a.cache.page_size, (uint32_t)kKeys) : kKeys;  // keys of a box
     const uint32_t ka = smem_u32(smem) + C::kKOff, va = smem_u32(smem) + C::kVOff;
-    int q = 0, k_brought = 0, v_brought = 0;  // tiles so far
+    int q = 0;  // tiles so far
     bool stop = false;
     while (next < end && !stop) {
       Piece p;
@@ -305,114 +285,98 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         wait_drain(&v_full[i % kStages], (i / kStages) & 1, 50000000ull);
     }
     __syncwarp();
-  } else if (warp >= 4 * kGroups) {
+  } else if (warp == 4) {
     const uint32_t leader = elect_one();
-    constexpr uint32_t kBase = (1u << 4) | (F::kCode << 7) | (F::kCode << 10) | ((uint32_t)(kRowTile >> 4) << 24);
+    constexpr uint32_t kBase = (1u << 4) | (F::kCode << 7) | (F::kCode << 10) | ((uint32_t)(kRows >> 4) << 24);
     constexpr uint32_t kQk = kBase | ((uint32_t)(kKeys >> 3) << 17);
     constexpr uint32_t kPv = kBase | ((uint32_t)(kDim >> 3) << 17) | (1u << 16);  // V is N-major
-    const uint32_t qa = smem_u32(smem) + group * C::kQ;
-    const uint32_t ka = smem_u32(smem) + C::kKOff, va = smem_u32(smem) + C::kVOff;
-    int q = 0, t = 0, walked = 0;  // tiles that passed by; this row tile's; its pieces with tiles
+    const uint32_t qa = smem_u32(smem), ka = qa + C::kKOff, va = qa + C::kVOff;
+    int q = 0, pieces = 0;  // tiles and pieces so far
     bool stop = false;
     while (next < end && !stop) {
       Piece p;
       take(p);
-      const int n = (int)(p.tile1 - p.tile0), mine = (int)(tiles_of(p) - p.tile0);
-      auto scores = [&](int i) {  // S = Q K^T of tile i
-        const int st = (q + i) % kStages;
-        if (!wait_soon(&k_full[st], ((q + i) / kStages) & 1, abort_flag)) return false;
+      const int n = (int)(p.tile1 - p.tile0);
+      if (n <= 0) continue;
+      auto scores = [&](int t) {  // S = Q K^T
+        const int st = t % kStages;
+        if (!wait_soon(&k_full[st], (t / kStages) & 1, abort_flag)) return false;
         tc_after_sync();
 #pragma unroll
         for (int j = 0; j < kDim / 16; ++j)
-          mma_ss(leader, tmem, desc128(qa + j / 4 * C::kQBlock + j % 4 * 32, 16),
+          mma_ss(leader, tmem + (t & 1) * kKeys, desc128(qa + j / 4 * C::kQBlock + j % 4 * 32, 16),
                  desc128(ka + st * C::kTile + j / 4 * C::kBlock + j % 4 * 32, 16), kQk, j > 0);
-        commit_to(leader, s_full);
+        commit_to(leader, &s_full[t & 1]);
         commit_to(leader, &k_empty[st]);
         return true;
       };
-      if (mine > 0) {
-        if (!wait_soon(q_full, walked & 1, abort_flag) || !scores(0)) break;
-        ++walked;
-      }
-      for (int i = 0; i < mine; ++i, ++t) {
-        const int st = (q + i) % kStages;
-        if ((i + 1 < mine && (!wait_soon(s_free, t & 1, abort_flag) || !scores(i + 1))) ||
-            !wait_soon(p_full, t & 1, abort_flag) ||
-            !wait_soon(&v_full[st], ((q + i) / kStages) & 1, abort_flag)) {
+      if (!wait_soon(q_full, pieces & 1, abort_flag) || !scores(q) || (n > 1 && !scores(q + 1))) break;
+      ++pieces;
+      for (int i = 0; i < n; ++i, ++q) {
+        const int st = q % kStages;
+        if (!wait_soon(p_full, q & 1, abort_flag) || !wait_soon(&v_full[st], (q / kStages) & 1, abort_flag)) {
           stop = true;
           break;
         }
         tc_after_sync();
 #pragma unroll
         for (int j = 0; j < kKeys / 16; ++j)
-          mma_ts(leader, tmem + C::kOCol, tmem + C::kPCol + j * 8, desc128(va + st * C::kTile + j * 2048, C::kBlock),
-                 kPv, i > 0 || j > 0);
+          mma_ts(leader, tmem + C::kOCol, tmem + (q & 1) * kKeys + kKeys / 2 + j * 8,
+                 desc128(va + st * C::kTile + j * 2048, C::kBlock), kPv, i > 0 || j > 0);
         commit_to(leader, o_full);
         commit_to(leader, &v_empty[st]);
-      }
-      for (int i = max(0, mine); i < n && !stop; ++i) {  // tiles for the other row tiles alone
-        const int st = (q + i) % kStages;
-        stop = !wait_soon(&k_full[st], ((q + i) / kStages) & 1, abort_flag) ||
-               !wait_soon(&v_full[st], ((q + i) / kStages) & 1, abort_flag);
-        if (!stop && lane == 0) {
-          mbar_arrive(&k_empty[st]);
-          mbar_arrive(&v_empty[st]);
+        if (i + 1 == n) commit_to(leader, done);
+        o_commits = q + 1;
+        // The scores of the tile after the next take the place of this P, once it has
+        // been read.
+        if (!wait_soon(o_full, q & 1, abort_flag) || (i + 2 < n && !scores(q + 2))) {
+          stop = true;
+          break;
         }
-        __syncwarp();
       }
-      q += n;
     }
-    if (*abort_flag) {
-      commit_to(leader, drained);
-      wait_drain(drained, 0, 50000000ull);
-    }
+    if (*abort_flag && o_commits) wait_drain(o_full, (o_commits - 1) & 1, 50000000ull);  // issued MMAs end
     __syncwarp();
   } else {
-    const int me = tid & (kRowTile - 1);
-    const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16);  // this warp's lanes
-    uint8_t* q_tile = smem + group * C::kQ;
-    int q = 0, t = 0, pieces = 0;  // tiles that passed by; this row tile's; pieces
+    const uint32_t tl = tmem + ((uint32_t)(warp * 32) << 16);  // this warp's lanes
+    int q = 0, pieces = 0, walked = 0;  // tiles; pieces, and those with tiles
     bool stop = false;
     while (next < end && !stop) {
       Piece p;
       take(p);
       ++pieces;
-      const uint32_t row = first_row(p) + me, token = row / a.group;
+      const uint32_t row = p.row_tile * kRows + tid, token = row / a.group;
       const uint32_t head = p.head * a.group + row % a.group;
       const bool there = row < rows;
       // Rows past the last see everything: zeros times finite or other keys, never stored.
       const RowView view = there ? row_view<kTree>(a, s, token) : RowView{0xffffffffu, 0ull};
-      float m = -INFINITY;      // the maximum in use, in powers of two
-      uint64_t l2[2] = {0, 0};  // the sum of weights, in four parts
-      // Tiles from here on hold a key that some row of this row tile, of the CTA does not see.
-      auto blind = [&](uint32_t r) { return (kTree ? s.context : row_view<false>(a, s, r / a.group).all) / kKeys; };
-      const uint32_t tile1 = tiles_of(p), mask0 = p.tile0 < tile1 ? blind(first_row(p)) : 0;
-      if (p.tile0 < tile1) {
+      float m = -INFINITY;          // the maximum in use, in powers of two
+      uint64_t l2[2] = {0, 0};      // the sum of weights, in four parts
+      // Tiles from here on hold a key that some row does not see.
+      const uint32_t mask0 = (kTree ? s.context : row_view<false>(a, s, p.row_tile * kRows / a.group).all) / kKeys;
+      if (p.tile0 < p.tile1) {
         const T* src = static_cast<const T*>(a.q.data) + (uint64_t)(s.q0 + token) * a.q.row_stride +
                        (uint64_t)head * a.q.head_stride;
 #pragma unroll
         for (int c = 0; c < kDim / 8; ++c) {
           const uint4 w = there ? reinterpret_cast<const uint4*>(src)[c] : make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4*>(q_tile + c / 8 * C::kQBlock + me * 128 + ((c % 8) ^ (me & 7)) * 16) = w;
+          *reinterpret_cast<uint4*>(smem + c / 8 * C::kQBlock + tid * 128 + ((c % 8) ^ (tid & 7)) * 16) = w;
         }
         fence_async_smem();
         tc_before_sync();  // the piece before has been read from TMEM
-        __syncwarp();
-        if (lane == 0) mbar_arrive(q_full);
+        mbar_arrive(q_full);
       }
-      for (uint32_t tile = p.tile0; tile < tile1; ++tile, ++t) {
+      for (uint32_t tile = p.tile0; tile < p.tile1; ++tile, ++q) {
         const uint32_t key0 = tile * kKeys;
         const bool masked = tile >= mask0;
-        if (!wait_soon(s_full, t & 1, abort_flag)) { stop = true; break; }
+        const uint32_t sc = tl + (q & 1) * kKeys;
+        if (!wait_soon(&s_full[q & 1], (q >> 1) & 1, abort_flag)) { stop = true; break; }
         tc_after_sync();
         uint32_t v[2][32];
-        tmem_ld32(tl, v[0]);
-        tmem_ld32(tl + 32, v[1]);
+        tmem_ld32(sc, v[0]);
+        tmem_ld32(sc + 32, v[1]);
         tmem_wait(v[0]);
         tmem_wait(v[1]);
-        tc_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(s_free);
         if (masked) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
@@ -421,18 +385,14 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
             for (int i = 0; i < 32; ++i) v[c][i] = (seen >> i) & 1 ? v[c][i] : 0xff800000u;  // -inf
           }
         }
-        float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int i = 0; i < 64; i += 8)
 #pragma unroll
           for (int u = 0; u < 4; ++u)
-            top4[u] = max_nan(top4[u], __uint_as_float(v[i / 32][i % 32 + 2 * u]),
-                              __uint_as_float(v[i / 32][i % 32 + 2 * u + 1]));
-        const float top =
-            __fmul_rn(max_nan(max_nan(top4[0], top4[1], top4[2]), top4[3], top4[3]), a.scale_log2);
-        // P and O are free when the products before are done.
-        if (t > 0 && !wait_soon(o_full, (t - 1) & 1, abort_flag)) { stop = true; break; }
-        tc_after_sync();
+            t[u] = max_nan(t[u], __uint_as_float(v[i / 32][i % 32 + 2 * u]),
+                           __uint_as_float(v[i / 32][i % 32 + 2 * u + 1]));
+        const float top = __fmul_rn(max_nan(max_nan(t[0], t[1], t[2]), t[3], t[3]), a.scale_log2);
         float keep = 1.f;
         if (!(top < INFINITY)) {
           m = NAN;  // a score that is not a number or +inf: so is the row
@@ -443,6 +403,8 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
           m = top;
         }
         if (__any_sync(0xffffffffu, keep != 1.f)) {  // never in a piece's first tile
+          if (!wait_soon(o_full, (q - 1) & 1, abort_flag)) { stop = true; break; }
+          tc_after_sync();
           uint32_t o[16];
 #pragma unroll
           for (int c = 0; c < kDim; c += 16) {
@@ -457,8 +419,6 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         }
         const float base = F::kRaise - (m == -INFINITY ? 0.f : m);
         const uint64_t scale2 = pk(a.scale_log2, a.scale_log2), base2 = pk(base, base);
-        // One exponential in four through the polynomial; all through the unit where keys
-        // are masked, whose weight has to be zero.
         auto weigh = [&](auto mixed) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
@@ -472,32 +432,30 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
               unpk(y, y0, y1);
               w[i / 2] = Elements<T>::pair(y0, y1);
             }
-            tmem_st16(tl + C::kPCol + 16 * c, w);
+            tmem_st16(sc + kKeys / 2 + 16 * c, w);  // over scores that have been read
           }
         };
         if (masked) weigh(std::false_type{});
         else weigh(std::true_type{});
         if (masked) {
           // Value rows of this tile, one per thread: zero past the keys, and without
-          // what is not finite (row tiles that share them find the same).
-          const int at = q + (int)(tile - p.tile0);
-          if (!wait_soon(&v_full[at % kStages], (at / kStages) & 1, abort_flag)) { stop = true; break; }
-          if (me < kKeys)
-            clean_value_row<F, kDim, C::kBlock>(smem + C::kVOff + at % kStages * C::kTile, me, key0 + me >= s.len,
-                                                dirty, pieces);
+          // what is not finite.
+          if (!wait_soon(&v_full[q % kStages], (q / kStages) & 1, abort_flag)) { stop = true; break; }
+          if (tid < kKeys &&
+              clean_value_row<F, kDim, C::kBlock>(smem + C::kVOff + (q % kStages) * C::kTile, tid, key0 + tid >= s.len))
+            *dirty = pieces;
           fence_async_smem();
         }
         tmem_wait_st();
         tc_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(p_full);
+        mbar_arrive(p_full);
       }
-      q += (int)(p.tile1 - p.tile0);
       if (stop) break;
 
       // The piece is done: O / l, or O with its maximum and sum.
-      if (p.tile0 < tile1) {
-        if (!wait_soon(o_full, (t - 1) & 1, abort_flag)) break;
+      if (p.tile0 < p.tile1) {
+        if (!wait_soon(done, walked & 1, abort_flag)) break;
+        ++walked;
         tc_after_sync();
       }
       float part[4];
@@ -507,13 +465,12 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       const float inv = l == 0.f ? 0.f : __frcp_rn(l);
       T* out = static_cast<T*>(a.out.data) + (uint64_t)(s.q0 + token) * a.out.row_stride +
                (uint64_t)head * a.out.head_stride;
-      const int in_tile = group * kRowTile + me;
       float* rec = kTree && p.partial >= 0 ? a.partial + (size_t)p.partial * partial_words<kRows, kDim>() : nullptr;
-      const bool mend = *dirty >= pieces;  // a later piece's: nothing to add here, which does no harm
+      const bool mend = *dirty == pieces;
 #pragma unroll
       for (int c = 0; c < kDim; c += 32) {
         uint32_t v[32];
-        if (p.tile0 < tile1) {
+        if (p.tile0 < p.tile1) {
           tmem_ld32(tl + C::kOCol + c, v);
           tmem_wait(v);
         } else {
@@ -523,7 +480,7 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         if (!there) continue;
         if (mend) {
           // A weight is positive: what is not finite passes through the sum as it is.
-          for (uint32_t key = max(p.tile0, blind(p.row_tile * kRows)) * kKeys; key < min(tile1 * kKeys, s.len); ++key) {
+          for (uint32_t key = max(p.tile0, mask0) * kKeys; key < min(p.tile1 * kKeys, s.len); ++key) {
             if (!view.sees(key)) continue;
             const T* from;
             if (kTree) {
@@ -545,7 +502,7 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         if (rec) {
 #pragma unroll
           for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<uint4*>(rec + in_tile * kDim + c + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            *reinterpret_cast<uint4*>(rec + tid * kDim + c + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
         } else {
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
@@ -557,8 +514,8 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         }
       }
       if (there && rec) {
-        rec[kRows * kDim + in_tile] = m == -INFINITY ? m : m - F::kRaise;
-        rec[kRows * kDim + kRows + in_tile] = l;
+        rec[kRows * kDim + tid] = m == -INFINITY ? m : m - F::kRaise;
+        rec[kRows * kDim + kRows + tid] = l;
       }
     }
   }
@@ -567,13 +524,16 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   __syncthreads();
   tc_after_sync();
   if (*abort_flag && tid == 0) mark_timeout();
-  if (warp == 0) tmem_dealloc(*tmem_slot, C::kCols);
+  tc_before_sync();
+  __syncthreads();
+  tc_after_sync();
+  if (warp == 4) tmem_dealloc(tmem, C::kCols);
 }
 
-template <class T, int kDim, int kGroups, bool kTree>
-uint32_t launch(const AttnArgs& a, cudaStream_t s) {
-  using C = Tc<kDim, kGroups>;
-  auto kernel = attention_tc_kernel<T, kDim, kGroups, kTree>;
+template <class T, int kDim, bool kTree>
+uint32_t launch(const AttnArgs& a, uint32_t grid, cudaStream_t s) {
+  using C = Tc<kDim>;
+  auto kernel = attention_tc_kernel<T, kDim, kTree>;
   static std::atomic<uint64_t> configured{0};
   if (attribute_needed(configured)) {
     PB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::bytes(PB_MAX_SEQS)));
@@ -581,40 +541,32 @@ uint32_t launch(const AttnArgs& a, cudaStream_t s) {
     attribute_done(configured);
   }
   Maps maps{};
-  uint32_t st = kTree ? cache_maps<T>(a, kDim, kKeys, &maps) : rows_maps<T>(a, kDim, kKeys, &maps);
+  uint32_t st = kTree ? cache_maps<T>(a, kDim, C::kKeys, &maps) : rows_maps<T>(a, kDim, C::kKeys, &maps);
   if (st) return st;
-  const uint32_t grid = kTree ? tree_ctas(C::kCtas) : (a.q_rows * a.group / C::kRows + a.seqs) * a.kv_heads;
-  kernel<<<grid, C::kThreads, C::bytes(a.seqs), s>>>(a, maps);
+  kernel<<<grid, kThreads, C::bytes(a.seqs), s>>>(a, maps);
   PB_CUDA(cudaGetLastError());
-  return kTree ? launch_combine<T, kDim, C::kRows, kKeys, kLeast>(a, grid, s) : PB_OK;
-}
-
-// Three row tiles a CTA where the rows of a sequence and key head fill two on average.
-bool wide(uint32_t head_dim, uint64_t rows, uint32_t seqs) {
-  return head_dim == 64 && rows >= 2ull * kRowTile * seqs;
-}
-
-template <class T, bool kTree>
-uint32_t by_size(const AttnArgs& a, uint32_t head_dim, cudaStream_t s) {
-  if (head_dim == 128) return launch<T, 128, 1, kTree>(a, s);
-  return wide(head_dim, (uint64_t)a.q_rows * a.group, a.seqs) ? launch<T, 64, 3, kTree>(a, s)
-                                                              : launch<T, 64, 1, kTree>(a, s);
+  return kTree ? launch_combine<T, kDim, kRows, C::kKeys, kLeast>(a, grid, s) : PB_OK;
 }
 
 }  // namespace
 
 uint32_t tc_prompt(const AttnArgs& a, uint32_t type, uint32_t head_dim, cudaStream_t s) {
-  return type == PB_TYPE_F16 ? by_size<__half, false>(a, head_dim, s) : by_size<__nv_bfloat16, false>(a, head_dim, s);
+  const uint32_t grid = (a.q_rows * a.group / kRows + a.seqs) * a.kv_heads;
+  if (type == PB_TYPE_F16)
+    return head_dim == 64 ? launch<__half, 64, false>(a, grid, s) : launch<__half, 128, false>(a, grid, s);
+  return head_dim == 64 ? launch<__nv_bfloat16, 64, false>(a, grid, s)
+                        : launch<__nv_bfloat16, 128, false>(a, grid, s);
 }
 
-uint64_t tc_tree_words(uint32_t head_dim, uint32_t rows, uint32_t seqs) {
-  // CTAs x rows: three row tiles have one CTA per SM, one has two
-  return wide(head_dim, rows, seqs) ? (uint64_t)tree_ctas(1) * 2 * 3 * kRowTile * (head_dim + 2)
-                                    : (uint64_t)tree_ctas(2) * 2 * kRowTile * (head_dim + 2);
+uint64_t tc_tree_words(uint32_t head_dim) {
+  return (uint64_t)tree_ctas(2) * 2 * kRows * (head_dim + 2);
 }
 
 uint32_t tc_tree(const AttnArgs& a, uint32_t type, uint32_t head_dim, cudaStream_t s) {
-  return type == PB_TYPE_F16 ? by_size<__half, true>(a, head_dim, s) : by_size<__nv_bfloat16, true>(a, head_dim, s);
+  const uint32_t grid = tree_ctas(2);
+  if (type == PB_TYPE_F16)
+    return head_dim == 64 ? launch<__half, 64, true>(a, grid, s) : launch<__half, 128, true>(a, grid, s);
+  return head_dim == 64 ? launch<__nv_bfloat16, 64, true>(a, grid, s) : launch<__nv_bfloat16, 128, true>(a, grid, s);
 }
 
 uint32_t tc_status() { return take_status(); }

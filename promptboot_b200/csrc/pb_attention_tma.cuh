@@ -89,32 +89,25 @@ __device__ __forceinline__ float max_nan(float a, float b, float c) {
 
 // Value row `key` of a tile in shared memory (column blocks of 128 bytes, kBlock
 // apart, 128-byte swizzle): zeroed where it is past the keys; else what is not finite
-// is zeroed, after *flag has been set to `mark`, so that a warp that finds the value
-// gone finds the flag set.
+// is zeroed.  Whether there was any.
 template <class F, int kDim, int kBlock>
-__device__ __forceinline__ void clean_value_row(uint8_t* tile, int key, bool past, volatile int* flag, int mark) {
+__device__ __forceinline__ bool clean_value_row(uint8_t* tile, int key, bool past) {
+  bool found = false;
 #pragma unroll 4
   for (int c = 0; c < kDim / 8; ++c) {
     uint4* word = reinterpret_cast<uint4*>(tile + c / 8 * kBlock + key * 128 + ((c % 8) ^ (key & 7)) * 16);
-    if (past) {
-      *word = make_uint4(0, 0, 0, 0);
-      continue;
-    }
-    uint4 x = *word;
+    uint4 x = past ? make_uint4(0, 0, 0, 0) : *word;
     uint32_t* u = reinterpret_cast<uint32_t*>(&x);
-    bool found = false;
+    bool write = past;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t e = u[i] & F::kExponents;
-      if ((e & 0xffffu) == (F::kExponents & 0xffffu)) { u[i] &= 0xffff0000u; found = true; }
-      if ((e >> 16) == (F::kExponents >> 16)) { u[i] &= 0xffffu; found = true; }
+      if ((e & 0xffffu) == (F::kExponents & 0xffffu)) { u[i] &= 0xffff0000u; found = write = true; }
+      if ((e >> 16) == (F::kExponents >> 16)) { u[i] &= 0xffffu; found = write = true; }
     }
-    if (found) {
-      *flag = mark;
-      __threadfence_block();
-      *word = x;
-    }
+    if (write) *word = x;
   }
+  return found;
 }
 
 // Set where a bounded wait of a kernel gave up (one word per source file).
