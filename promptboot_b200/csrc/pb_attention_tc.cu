@@ -48,7 +48,7 @@ struct Tc {
   static constexpr int kKOff = kHalves * kQBlock;
   static constexpr int kVOff = kKOff + kStages * kTile;
   static constexpr int kBarOff = kVOff + kStages * kTile;
-  static constexpr int kBars = 4 * kStages + 6;
+  static constexpr int kBars = 4 * kStages + 11;
   static constexpr int kPrefixOff = kBarOff + kBars * 8 + 16;
   static constexpr int kOCol = 2 * kKeys;             // S and P: [0, 64) and [64, 128)
   static constexpr int kCols = 256;
@@ -153,6 +153,32 @@ __device__ __forceinline__ uint64_t exp2_poly(uint64_t x) {
   unpk(t, t0, t1);
   return pk_u(__float_as_uint(y0) + (__float_as_uint(t0) << 23), __float_as_uint(y1) + (__float_as_uint(t1) << 23));
 }
+// Asks for the index of a CTA of this launch that has not begun, which then never does
+// (16 bytes at `to`, completing on bar); and what the answer was.
+__device__ __forceinline__ void cancel_one(uint32_t leader, uint4* to, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "setp.ne.b32 e, %2, 0;\n\t"
+      "@e clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];\n\t}"
+      ::"r"(smem_u32(to)), "r"(smem_u32(bar)), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ bool cancelled(const uint4* answer, uint32_t& cta) {
+  uint32_t is, x;
+  asm volatile(
+      "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t.reg .b32 y, z, w;\n\t"
+      "ld.shared.b128 h, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "mov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, y, z, w}, h;\n\t}"
+      : "=r"(is), "=r"(x)
+      : "r"(smem_u32(answer))
+      : "memory");
+  cta = x;
+  return is != 0;
+}
+
 // Which of the 32 keys from `key` on a row sees.
 __device__ __forceinline__ uint32_t seen32(const RowView& r, uint32_t key) {
   const uint32_t below = r.all > key ? r.all - key : 0;
@@ -180,11 +206,13 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   uint64_t* v_full = k_empty + kStages;
   uint64_t* v_empty = v_full + kStages;
   uint64_t* q_full = v_empty + kStages;
-  uint64_t* p_full = q_full + 1;
-  uint64_t* o_full = p_full + 1;  // O holds the tile's products, its P is free
+  uint64_t* p_full = q_full + 1;  // one per score buffer: a warp may be a tile ahead of another
+  uint64_t* o_full = p_full + 2;  // O holds the tile's products, its P is free
   uint64_t* done = o_full + 1;    // O holds the piece's
   uint64_t* s_full = done + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 2);
+  uint64_t* unit_full = s_full + 2;  // prompts: the next unit is known
+  uint64_t* unit_empty = unit_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(unit_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* dirty = abort_flag + 1;  // the last piece with a value that was taken out
   uint32_t* prefix = reinterpret_cast<uint32_t*>(smem + C::kPrefixOff);
@@ -217,9 +245,14 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     mbar_init(q_full, kRows);
     mbar_init(&s_full[0], 1);
     mbar_init(&s_full[1], 1);
-    mbar_init(p_full, kRows);
+    mbar_init(&p_full[0], kRows);
+    mbar_init(&p_full[1], kRows);
     mbar_init(o_full, 1);
     mbar_init(done, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&unit_full[i], 1);
+      mbar_init(&unit_empty[i], kThreads / 32);
+    }
     *abort_flag = 0;
     *dirty = 0;
     fence_barrier_init();
@@ -229,10 +262,26 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   tc_after_sync();
   const uint32_t tmem = *tmem_slot;
 
-  // The CTA's pieces, decoded alike by every role.
+  // The CTA's pieces, decoded alike by every role.  Prompts: one unit after another, of
+  // those that no CTA has begun, by cancelling the launch of its CTA; asked for while the
+  // unit before is worked on.
+  __shared__ alignas(16) uint4 answer[2];
   Sequence s;
   uint32_t rows;
+  int unit = 0;
+  bool have = true;
   auto take = [&](Piece& p) { take_piece<kTree, kRows, kKeys>(a, prefix, next, end, p, s, rows); };
+  auto further = [&] {
+    if (kTree) return next < end;
+    const int slot = unit & 1;
+    if (!wait_soon(&unit_full[slot], (unit >> 1) & 1, abort_flag)) return false;
+    const bool more = cancelled(&answer[slot], next);
+    fence_async_smem();  // read before the next answer is written
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&unit_empty[slot]);
+    ++unit;
+    return more && next < total;
+  };
 
   int k_brought = 0, v_brought = 0, o_commits = 0;  // tiles, for the way out
 
@@ -242,9 +291,16 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     const uint32_t ka = smem_u32(smem) + C::kKOff, va = smem_u32(smem) + C::kVOff;
     int q = 0;  // tiles so far
     bool stop = false;
-    while (next < end && !stop) {
+    int asked = 0;
+    for (; have && !stop; have = further()) {
       Piece p;
       take(p);
+      if (!kTree) {
+        if (!wait_soon(&unit_empty[unit & 1], ((unit >> 1) & 1) ^ 1, abort_flag)) break;
+        expect_tx(leader, &unit_full[unit & 1], 16);
+        cancel_one(leader, &answer[unit & 1], &unit_full[unit & 1]);
+        asked = unit + 1;
+      }
       auto boxes = [&](uint32_t tile) { return min((uint32_t)kKeys / size, ceil_div(s.len - tile * kKeys, size)); };
       auto page_of = [&](uint32_t tile) {  // of box `lane` of a tile
         const uint32_t key = tile * kKeys + lane * size;
@@ -278,7 +334,8 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         page = ahead;
       }
     }
-    if (*abort_flag) {  // every copy lands before the CTA may exit
+    if (*abort_flag) {  // every copy and answer lands before the CTA may exit
+      if (asked) wait_drain(&unit_full[(asked - 1) & 1], ((asked - 1) >> 1) & 1, 50000000ull);
       for (int i = max(0, k_brought - kStages); i < k_brought; ++i)
         wait_drain(&k_full[i % kStages], (i / kStages) & 1, 50000000ull);
       for (int i = max(0, v_brought - kStages); i < v_brought; ++i)
@@ -293,7 +350,7 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     const uint32_t qa = smem_u32(smem), ka = qa + C::kKOff, va = qa + C::kVOff;
     int q = 0, pieces = 0;  // tiles and pieces so far
     bool stop = false;
-    while (next < end && !stop) {
+    for (; have && !stop; have = further()) {
       Piece p;
       take(p);
       const int n = (int)(p.tile1 - p.tile0);
@@ -314,7 +371,7 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       ++pieces;
       for (int i = 0; i < n; ++i, ++q) {
         const int st = q % kStages;
-        if (!wait_soon(p_full, q & 1, abort_flag) || !wait_soon(&v_full[st], (q / kStages) & 1, abort_flag)) {
+        if (!wait_soon(&p_full[q & 1], (q >> 1) & 1, abort_flag) || !wait_soon(&v_full[st], (q / kStages) & 1, abort_flag)) {
           stop = true;
           break;
         }
@@ -341,7 +398,7 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     const uint32_t tl = tmem + ((uint32_t)(warp * 32) << 16);  // this warp's lanes
     int q = 0, pieces = 0, walked = 0;  // tiles; pieces, and those with tiles
     bool stop = false;
-    while (next < end && !stop) {
+    for (; have && !stop; have = further()) {
       Piece p;
       take(p);
       ++pieces;
@@ -448,7 +505,7 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         }
         tmem_wait_st();
         tc_before_sync();
-        mbar_arrive(p_full);
+        mbar_arrive(&p_full[q & 1]);
       }
       if (stop) break;
 

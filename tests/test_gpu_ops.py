@@ -470,6 +470,26 @@ def test_tree_attention_of_long_and_of_many_contexts(dtype, seqs, nodes):
     assert torch.equal(got, ops.tree_attention(*args, layer=1, workspace=work))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_gives_the_same_bits_every_time(dtype):
+    """Many calls on the same inputs: split contexts with several pieces per CTA, and
+    packed prompts with several units per CTA.  A lost wait shows here first."""
+    for seqs, nodes, dim, kv_heads, heads in ((16, 12, 128, 8, 32), (2, 48, 64, 2, 14), (60, 1, 64, 2, 14), (20, 5, 64, 2, 8)):
+        g, rng = gen(24), np.random.default_rng(seqs)
+        contexts = [int(c) for c in rng.integers(200, 3000 if seqs > 2 else 30000, seqs)]
+        cache, tables, _, _ = paged(g, rng, [c + nodes for c in contexts], 64, kv_heads, dim, dtype)
+        q = normal(g, seqs * nodes, heads, dim, dtype=dtype, scale=2.0)
+        visible = masks([b for _ in range(seqs) for b in random_tree(rng, nodes)])
+        args = (q, cache, tables, i32(contexts), starts([nodes] * seqs), visible)
+        want = ops.tree_attention(*args, layer=1)
+        assert all(torch.equal(want, ops.tree_attention(*args, layer=1)) for _ in range(400))
+    for tokens, dim in (([1200, 100, 1], 64), ([64] * 60, 128)):
+        g, n = gen(25), sum(tokens)
+        q, k, v = (normal(g, n, h, dim, dtype=dtype, scale=1.5) for h in (14, 2, 2))
+        want = ops.prompt_attention(q, k, v, starts(tokens))
+        assert all(torch.equal(want, ops.prompt_attention(q, k, v, starts(tokens))) for _ in range(400))
+
+
 # ------------------------------------------------------------------------- pages
 
 @pytest.mark.parametrize("dtype", TYPES)
