@@ -35,11 +35,12 @@ uint32_t check_scale(const char* who, float scale) {
   return PB_OK;
 }
 
-// Row groups of 16 that hold a sequence's rows of one key head on average (1 or 2),
-// 0 where they are more than 32.
-uint32_t few_tiles(uint64_t rows, uint32_t seqs) {
+// Row groups of 16 that hold a sequence's rows of one key head on average: 1, or 2 at
+// heads of 64 (at heads of 128 their sums would not fit the registers); 0 where they
+// are more.
+uint32_t few_tiles(uint32_t head_dim, uint64_t rows, uint32_t seqs) {
   if (rows <= 16ull * seqs) return 1;
-  return rows <= 32ull * seqs ? 2 : 0;
+  return head_dim == 64 && rows <= 32ull * seqs ? 2 : 0;
 }
 
 constexpr float kLog2E = 1.4426950408889634f;
@@ -89,7 +90,7 @@ uint64_t pb_tree_attention_workspace(uint32_t type, uint32_t head_dim, uint32_t 
   if (pb::paged::check_heads("pb_tree_attention_workspace", type, head_dim, q_heads, kv_heads, seqs, rows))
     return 0;
   if (pb::paged::type_bytes(type) == 2) {
-    const uint32_t tiles = pb::paged::few_tiles(rows * (q_heads / kv_heads), seqs);
+    const uint32_t tiles = pb::paged::few_tiles(head_dim, rows * (q_heads / kv_heads), seqs);
     return (tiles ? pb::paged::few_tree_words(head_dim, tiles) : pb::paged::tc_tree_words(head_dim)) * 4;
   }
   return pb::paged::simt_tree_words(head_dim, rows * (q_heads / kv_heads), seqs) * 4;
@@ -114,10 +115,10 @@ uint32_t pb_tree_attention_device(const pb_cache* cache, uint32_t layer, uint32_
   if ((st = pb::paged::check_rows(out, bytes, who, "out"))) return st;
   if (!tables || !table_width || !contexts || !offsets || !visible)
     return refuse(PB_CAPACITY, who, "an empty table or a NULL argument");
-  // Key tiles (of 32 keys at least, for row tiles of 16 at least) are counted in 32 bits.
+  // Key tiles (of 16 keys at least, for row tiles of 16 at least) are counted in 32 bits.
   const uint64_t group = q_heads / cache->kv_heads, reach = (uint64_t)table_width * cache->page_size;
   const uint64_t segments = (rows * group / 16 + seqs) * cache->kv_heads;
-  if (reach >= 1ull << 30 || segments * (reach / 32 + 1) >= 1ull << 31)
+  if (reach >= 1ull << 30 || segments * (reach / 16 + 1) >= 1ull << 31)
     return refuse(PB_CAPACITY, who, "the tables reach too far for so many sequences and rows");
   const uint64_t need = pb_tree_attention_workspace(cache->type, cache->head_dim, q_heads,
                                                     cache->kv_heads, seqs, rows);
@@ -134,7 +135,7 @@ uint32_t pb_tree_attention_device(const pb_cache* cache, uint32_t layer, uint32_
   a.scale_log2 = scale * pb::paged::kLog2E;
   a.partial = static_cast<float*>(workspace);
   if (bytes == 2) {
-    const uint32_t tiles = pb::paged::few_tiles(rows * (uint32_t)group, seqs);
+    const uint32_t tiles = pb::paged::few_tiles(cache->head_dim, rows * group, seqs);
     return tiles ? pb::paged::few_tree(a, cache->type, cache->head_dim, tiles, (cudaStream_t)stream)
                  : pb::paged::tc_tree(a, cache->type, cache->head_dim, (cudaStream_t)stream);
   }

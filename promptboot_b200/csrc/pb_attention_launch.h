@@ -23,7 +23,7 @@ uint64_t tc_tree_words(uint32_t head_dim);
 uint32_t tc_status();
 
 // Tree attention of 16-bit elements with 16 * tiles rows at most on average per
-// sequence and key head (tiles 1, 2 or 4).
+// sequence and key head (tiles 1, or 2 at heads of 64).
 uint32_t few_tree(const AttnArgs& a, uint32_t type, uint32_t head_dim, uint32_t tiles, cudaStream_t s);
 uint64_t few_tree_words(uint32_t head_dim, uint32_t tiles);
 uint32_t few_status();

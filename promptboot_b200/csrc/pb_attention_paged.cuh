@@ -7,8 +7,8 @@
 //
 // Prompts: one CTA per segment, the row tiles of a sequence from its end (the
 // longest) to its start.  Trees: all key tiles of all segments form one list,
-// which the CTAs share out evenly in consecutive runs whatever the sequences'
-// lengths are; a segment that crosses runs leaves one partial (weighted sum,
+// which is shared out evenly in consecutive runs, one to a CTA or a warp, whatever the
+// sequences' lengths are; a segment that crosses runs leaves one partial (weighted sum,
 // maximum, sum) per run in the workspace and combine_kernel joins them.
 #pragma once
 
@@ -31,7 +31,8 @@ struct AttnArgs {
   const unsigned long long* visible;
   uint32_t seqs, q_rows, kv_rows, kv_heads, group, table_width;
   float scale_log2;  // scale * log2(e): weights are powers of two
-  float* partial;
+  float* partial;    // trees: two records a run
+  struct Join* joins;  // and what is to be joined where a run ends
 };
 
 // One sequence: its rows of q, its keys, and how many of them every row sees.
@@ -131,18 +132,19 @@ __device__ __forceinline__ uint32_t find_sequence(const uint32_t* prefix, uint32
   return lo;
 }
 
-// The trees' list of `total` key tiles over `grid` CTAs, at least kLeast tiles
-// each: CTA c takes [start(c), start(c + 1)), and tile x belongs to CTA holder(x).
+// The trees' list of `total` key tiles in `most` runs, at least kLeast tiles each: run
+// c is [start(c), start(c + 1)), and tile x is in run holder(x).  A run is a CTA's, or
+// a warp's in pb_attention_few.cu.
 template <int kLeast>
 struct Share {
-  uint32_t total, ctas;
-  __device__ __forceinline__ Share(uint32_t total_, uint32_t grid)
-      : total(total_), ctas(min(grid, max(1u, total_ / kLeast))) {}
+  uint32_t total, runs;
+  __device__ __forceinline__ Share(uint32_t total_, uint32_t most)
+      : total(total_), runs(min(most, max(1u, total_ / kLeast))) {}
   __device__ __forceinline__ uint32_t start(uint32_t c) const {
-    return (uint32_t)((uint64_t)c * total / ctas);
+    return (uint32_t)((uint64_t)c * total / runs);
   }
   __device__ __forceinline__ uint32_t holder(uint32_t x) const {
-    return (uint32_t)((((uint64_t)x + 1) * ctas - 1) / total);
+    return (uint32_t)((((uint64_t)x + 1) * runs - 1) / total);
   }
 };
 
@@ -153,10 +155,13 @@ struct Piece {
   int partial;  // workspace record, -1: the whole segment, straight to out
 };
 
-// Takes the next piece of a CTA's items [next, end).
+// The partial of run c for a segment that began before it, or that begins in it.
+__device__ __forceinline__ int partial_of(uint32_t run, bool begins) { return (int)(2 * run + begins); }
+
+// Takes the next piece of run `run`'s items [next, end).
 template <bool kTree, int kRows, int kKeys>
-__device__ __forceinline__ void take_piece(const AttnArgs& a, const uint32_t* prefix, uint32_t& next, uint32_t end,
-                                           Piece& p, Sequence& s, uint32_t& rows) {
+__device__ __forceinline__ void take_piece(const AttnArgs& a, const uint32_t* prefix, uint32_t run, uint32_t& next,
+                                           uint32_t end, Piece& p, Sequence& s, uint32_t& rows) {
   uint32_t x = next;
   p.seq = find_sequence(prefix, a.seqs, x);
   s = load_sequence<kTree>(a, p.seq);
@@ -169,7 +174,7 @@ __device__ __forceinline__ void take_piece(const AttnArgs& a, const uint32_t* pr
     p.tile1 = min(tiles, p.tile0 + (end - next));
     p.head = x / tiles / row_tiles;
     p.row_tile = x / tiles % row_tiles;
-    if (p.tile0 > 0 || p.tile1 < tiles) p.partial = (int)(2 * blockIdx.x + (p.tile0 == 0));
+    if (p.tile0 > 0 || p.tile1 < tiles) p.partial = partial_of(run, p.tile0 == 0);
     next += p.tile1 - p.tile0;
     if (s.len == 0) p.tile1 = p.tile0 = 0;  // nothing to see
   } else {
@@ -181,9 +186,6 @@ __device__ __forceinline__ void take_piece(const AttnArgs& a, const uint32_t* pr
     ++next;
   }
 }
-
-// The partial of CTA c for a segment that began before it, or that begins in it.
-__device__ __forceinline__ int partial_of(uint32_t cta, bool begins) { return (int)(2 * cta + begins); }
 
 // Four consecutive elements, rounded once.
 __device__ __forceinline__ void store4(float* out, float4 y) { *reinterpret_cast<float4*>(out) = y; }
@@ -198,48 +200,57 @@ __host__ __device__ constexpr size_t partial_words() {
   return (size_t)kRows * (kDim + 2);
 }
 
-// Joins the partials of the segments that crossed CTA runs: weights 2^(m_i - m),
-// in the order of the runs, so the result does not depend on timing.  A segment
-// is joined by the CTAs (four at most, so that one wave of them holds all) of the edge
-// at the end of the run in which it begins.  A thread has four elements of a row and
-// loads eight partials at a time: latency is what there is to save here.
-template <class T, int kDim, int kRows, int kKeys, int kLeast>
-__global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ AttnArgs a, uint32_t grid) {
-  extern __shared__ uint32_t prefix[];
-  work_prefix<true, kRows, kKeys, 256>(a, prefix);
-  const uint32_t total = prefix[a.seqs - 1], c = blockIdx.x;
-  const Share<kLeast> share(max(1u, total), grid);
-  bool mine = total > 0 && c + 1 < share.ctas;
-  uint32_t edge = 0, begin = 0, seq = 0, x = 0, tiles = 1;
-  Sequence s{};
-  if (mine) {
-    x = edge = share.start(c + 1);
-    seq = find_sequence(prefix, a.seqs, x);
-    s = load_sequence<true>(a, seq);
-    tiles = max(1u, ceil_div(s.len, kKeys));
-    begin = edge - x % tiles;
-    mine = begin != edge && begin >= share.start(c);  // else it begins at the edge, or in an earlier run
+// The segment that begins in a run and goes on in the next: its last run, the rows of
+// its sequence from q0 on, its head and row tile.  last PB_NONE: there is none.
+struct alignas(16) Join {
+  uint32_t last, q0, rows, head, row_tile;
+};
+
+// Notes the segment that crosses the end of run `run` (one thread of it, every run of
+// the launch).
+template <int kRows, int kKeys, int kLeast>
+__device__ __forceinline__ void note_join(const AttnArgs& a, const uint32_t* prefix, const Share<kLeast>& share,
+                                          uint32_t run) {
+  Join j{PB_NONE, 0, 0, 0, 0};
+  if (share.total > 0 && run + 1 < share.runs) {
+    const uint32_t edge = share.start(run + 1);
+    uint32_t x = edge;
+    const Sequence s = load_sequence<true>(a, find_sequence(prefix, a.seqs, x));
+    const uint32_t tiles = max(1u, ceil_div(s.len, kKeys)), begin = edge - x % tiles;
+    if (begin != edge && begin >= share.start(run)) {  // else it begins at the edge, or in an earlier run
+      const uint32_t rows = s.t * a.group, row_tiles = ceil_div(rows, kRows);
+      j = {share.holder(begin + tiles - 1), s.q0, rows, x / tiles / row_tiles, x / tiles % row_tiles};
+    }
   }
-  pdl_wait();  // the partials; also in a CTA that has none, for what comes after this launch
-  if (!mine) return;
-  constexpr int kPerRow = kDim / 4, kStep = 256 / kPerRow, kBatch = 8;
-  const uint32_t last = share.holder(begin + tiles - 1);
-  const uint32_t row_tiles = ceil_div(s.t * a.group, kRows);
-  const uint32_t head = x / tiles / row_tiles, row_tile = x / tiles % row_tiles;
+  a.joins[run] = j;
+}
+
+// Joins the partials of the segments that crossed runs: weights 2^(m_i - m), in the
+// order of the runs, so the result does not depend on timing.  A segment is joined by
+// the CTAs of the run in which it begins.  A thread has four elements of a row and loads
+// four or eight partials at a time: latency is what there is to save here.
+constexpr int kCombine = 128;  // threads
+template <class T, int kDim, int kRows>
+__global__ void __launch_bounds__(kCombine) combine_kernel(const __grid_constant__ AttnArgs a) {
+  pdl_wait();  // the notes and the partials
+  const uint32_t c = blockIdx.x;
+  const Join j = a.joins[c];
+  if (j.last == PB_NONE) return;
+  constexpr int kPerRow = kDim / 4, kStep = kCombine / kPerRow, kBatch = kRows > 32 ? 8 : 4;
   const int chunk = (threadIdx.x % kPerRow) * 4;
   for (uint32_t r = blockIdx.y * kStep + threadIdx.x / kPerRow; r < kRows; r += gridDim.y * kStep) {
-    const uint32_t row = row_tile * kRows + r;
-    if (row >= s.t * a.group) return;
+    const uint32_t row = j.row_tile * kRows + r;
+    if (row >= j.rows) return;
     float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (uint32_t p0 = c; p0 <= last; p0 += kBatch) {
+    for (uint32_t p0 = c; p0 <= j.last; p0 += kBatch) {
       float mp[kBatch], lp[kBatch];
       float4 op[kBatch];
       float to = m;
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
         mp[i] = -INFINITY;
-        if (p0 + i <= last) {
+        if (p0 + i <= j.last) {
           const float* rec = a.partial + partial_of(p0 + i, p0 + i == c) * partial_words<kRows, kDim>();
           mp[i] = rec[kRows * kDim + r];
           lp[i] = rec[kRows * kDim + kRows + r];
@@ -263,20 +274,29 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ At
       }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    const uint32_t token = row / a.group, h = head * a.group + row % a.group;
-    T* out = static_cast<T*>(a.out.data) + (uint64_t)(s.q0 + token) * a.out.row_stride +
+    const uint32_t token = row / a.group, h = j.head * a.group + row % a.group;
+    T* out = static_cast<T*>(a.out.data) + (uint64_t)(j.q0 + token) * a.out.row_stride +
              h * a.out.head_stride + chunk;
     store4(out, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
   }
 }
 
 // The trees' second launch, which may begin while the first ends.
-template <class T, int kDim, int kRows, int kKeys, int kLeast>
-uint32_t launch_combine(const AttnArgs& a, uint32_t grid, cudaStream_t s) {
-  constexpr int kStep = 256 / (kDim / 4);
-  const dim3 join(grid, std::min(4, (kRows + kStep - 1) / kStep));
-  PB_CUDA(launch_pdl(combine_kernel<T, kDim, kRows, kKeys, kLeast>, join, 256, a.seqs * 4, s, a, grid));
+template <class T, int kDim, int kRows>
+uint32_t launch_combine(const AttnArgs& a, uint32_t runs, cudaStream_t s) {
+  constexpr int kStep = kCombine / (kDim / 4);
+  const dim3 join(runs, kRows > 32 ? kRows / kStep : 1);
+  PB_CUDA(launch_pdl(combine_kernel<T, kDim, kRows>, join, kCombine, 0, s, a));
   return PB_OK;
+}
+
+// Words of a tree's workspace: two partials and a note per run.
+inline uint64_t tree_words(uint64_t runs, uint64_t rows, uint64_t head_dim) {
+  return runs * (2 * rows * (head_dim + 2) + sizeof(Join) / 4);
+}
+// Places them; the partials first.
+inline void place_workspace(AttnArgs& a, uint64_t runs, uint64_t rows, uint64_t head_dim) {
+  a.joins = reinterpret_cast<Join*>(a.partial + runs * 2 * rows * (head_dim + 2));
 }
 
 }  // namespace paged

@@ -49,9 +49,10 @@ __global__ void __launch_bounds__(kThreads) attention_simt_kernel(const __grid_c
 
   uint32_t next, end;  // this CTA's items: one segment, or a run of key tiles
   if (kTree) {
-    if (total == 0) return;
     const Share<kLeast> share(total, gridDim.x);
-    if (blockIdx.x >= share.ctas) return;
+    if (threadIdx.x == kThreads - 1) note_join<kRows, kKeys>(a, prefix, share, blockIdx.x);
+    if (total == 0) return;
+    if (blockIdx.x >= share.runs) return;
     next = share.start(blockIdx.x);
     end = share.start(blockIdx.x + 1);
   } else {
@@ -64,9 +65,10 @@ __global__ void __launch_bounds__(kThreads) attention_simt_kernel(const __grid_c
     Piece p;
     Sequence s;
     uint32_t rows;
-    take_piece<kTree, kRows, kKeys>(a, prefix, next, end, p, s, rows);
+    take_piece<kTree, kRows, kKeys>(a, prefix, blockIdx.x, next, end, p, s, rows);
     __syncthreads();  // the piece before is done with shared memory
     constexpr int kWords = kDim / 4;
+#pragma unroll 2
     for (int i = threadIdx.x; i < kRows * kWords; i += kThreads) {
       const int r = i / kWords, c = i % kWords * 4;
       const uint32_t row = p.row_tile * kRows + r;
@@ -97,6 +99,7 @@ __global__ void __launch_bounds__(kThreads) attention_simt_kernel(const __grid_c
     for (uint32_t tile = p.tile0; tile < p.tile1; ++tile) {
       const uint32_t key0 = tile * kKeys;
       __syncthreads();
+#pragma unroll 4
       for (int i = threadIdx.x; i < kKeys * kWords; i += kThreads) {
         const int j = i / kWords, c = i % kWords * 4;
         const uint32_t key = key0 + j;
@@ -238,7 +241,7 @@ __global__ void __launch_bounds__(kThreads) attention_simt_kernel(const __grid_c
 }
 
 template <int kDim, int kRpt, bool kTree>
-uint32_t launch(const AttnArgs& a, uint32_t grid, cudaStream_t s) {
+uint32_t launch(AttnArgs a, uint32_t grid, cudaStream_t s) {
   using C = Simt<kDim, kRpt>;
   auto kernel = attention_simt_kernel<kDim, kRpt, kTree>;
   static std::atomic<uint64_t> configured{0};
@@ -247,9 +250,10 @@ uint32_t launch(const AttnArgs& a, uint32_t grid, cudaStream_t s) {
                                  (int)C::bytes(PB_MAX_SEQS)));
     attribute_done(configured);
   }
+  if (kTree) place_workspace(a, grid, C::kRows, kDim);
   kernel<<<grid, kThreads, C::bytes(a.seqs), s>>>(a);
   PB_CUDA(cudaGetLastError());
-  return kTree ? launch_combine<float, kDim, C::kRows, C::kKeys, kLeast>(a, grid, s) : PB_OK;
+  return kTree ? launch_combine<float, kDim, C::kRows>(a, grid, s) : PB_OK;
 }
 
 constexpr int kFewRpt = 2, kManyRpt = 8;  // 16 or 64 rows of a tile
@@ -258,7 +262,11 @@ constexpr int kFewRpt = 2, kManyRpt = 8;  // 16 or 64 rows of a tile
 
 uint32_t simt_prompt(const AttnArgs& a, uint32_t head_dim, cudaStream_t s) {
   const uint32_t rows = a.q_rows * a.group;
-  const uint32_t grid = (rows / (8 * kManyRpt) + a.seqs) * a.kv_heads;
+  // Row tiles of 16 where tiles of 64 would leave SMs without work.
+  const bool small = (uint64_t)rows * a.kv_heads < 64ull * tree_ctas(1);
+  const uint32_t grid = (rows / (small ? 8 * kFewRpt : 8 * kManyRpt) + a.seqs) * a.kv_heads;
+  if (small)
+    return head_dim == 64 ? launch<64, kFewRpt, false>(a, grid, s) : launch<128, kFewRpt, false>(a, grid, s);
   return head_dim == 64 ? launch<64, kManyRpt, false>(a, grid, s) : launch<128, kManyRpt, false>(a, grid, s);
 }
 
@@ -267,7 +275,7 @@ static bool few(uint32_t rows, uint32_t seqs) { return rows <= 16 * seqs; }
 
 uint64_t simt_tree_words(uint32_t head_dim, uint32_t rows, uint32_t seqs) {
   const uint32_t tile = few(rows, seqs) ? 8 * kFewRpt : 8 * kManyRpt;
-  return (uint64_t)tree_ctas(4) * 2 * tile * (head_dim + 2);
+  return tree_words(tree_ctas(4), tile, head_dim);
 }
 
 uint32_t simt_tree(const AttnArgs& a, uint32_t head_dim, cudaStream_t s) {

@@ -223,9 +223,11 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   const uint32_t total = prefix[a.seqs - 1];
   uint32_t next, end;
   if (kTree) {
-    if (total == 0) return;
     const Share<kLeast> share(total, gridDim.x);
-    if (blockIdx.x >= share.ctas) return;
+    if (total == 0 || blockIdx.x >= share.runs) {
+      if (tid == 0) note_join<kRows, kKeys>(a, prefix, share, blockIdx.x);
+      return;
+    }
     next = share.start(blockIdx.x);
     end = share.start(blockIdx.x + 1);
   } else {
@@ -270,7 +272,7 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   uint32_t rows;
   int unit = 0;
   bool have = true;
-  auto take = [&](Piece& p) { take_piece<kTree, kRows, kKeys>(a, prefix, next, end, p, s, rows); };
+  auto take = [&](Piece& p) { take_piece<kTree, kRows, kKeys>(a, prefix, blockIdx.x, next, end, p, s, rows); };
   auto further = [&] {
     if (kTree) return next < end;
     const int slot = unit & 1;
@@ -334,6 +336,8 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         page = ahead;
       }
     }
+    if (kTree && lane == 0)  // under the last tiles of the others
+      note_join<kRows, kKeys>(a, prefix, Share<kLeast>(total, gridDim.x), blockIdx.x);
     if (*abort_flag) {  // every copy and answer lands before the CTA may exit
       if (asked) wait_drain(&unit_full[(asked - 1) & 1], ((asked - 1) >> 1) & 1, 50000000ull);
       for (int i = max(0, k_brought - kStages); i < k_brought; ++i)
@@ -588,7 +592,7 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
 }
 
 template <class T, int kDim, bool kTree>
-uint32_t launch(const AttnArgs& a, uint32_t grid, cudaStream_t s) {
+uint32_t launch(AttnArgs a, uint32_t grid, cudaStream_t s) {
   using C = Tc<kDim>;
   auto kernel = attention_tc_kernel<T, kDim, kTree>;
   static std::atomic<uint64_t> configured{0};
@@ -600,9 +604,10 @@ uint32_t launch(const AttnArgs& a, uint32_t grid, cudaStream_t s) {
   Maps maps{};
   uint32_t st = kTree ? cache_maps<T>(a, kDim, C::kKeys, &maps) : rows_maps<T>(a, kDim, C::kKeys, &maps);
   if (st) return st;
+  if (kTree) place_workspace(a, grid, kRows, kDim);
   kernel<<<grid, kThreads, C::bytes(a.seqs), s>>>(a, maps);
   PB_CUDA(cudaGetLastError());
-  return kTree ? launch_combine<T, kDim, kRows, C::kKeys, kLeast>(a, grid, s) : PB_OK;
+  return kTree ? launch_combine<T, kDim, kRows>(a, grid, s) : PB_OK;
 }
 
 }  // namespace
@@ -615,9 +620,7 @@ uint32_t tc_prompt(const AttnArgs& a, uint32_t type, uint32_t head_dim, cudaStre
                         : launch<__nv_bfloat16, 128, false>(a, grid, s);
 }
 
-uint64_t tc_tree_words(uint32_t head_dim) {
-  return (uint64_t)tree_ctas(2) * 2 * kRows * (head_dim + 2);
-}
+uint64_t tc_tree_words(uint32_t head_dim) { return tree_words(tree_ctas(2), kRows, head_dim); }
 
 uint32_t tc_tree(const AttnArgs& a, uint32_t type, uint32_t head_dim, cudaStream_t s) {
   const uint32_t grid = tree_ctas(2);
