@@ -69,6 +69,7 @@ uint32_t pb_prompt_attention_device(uint32_t type, uint32_t head_dim, uint32_t q
     return refuse(PB_CAPACITY, who, "other key rows than q rows need kv_offsets");
   if (!q_offsets) return refuse(PB_CAPACITY, who, "q_offsets is NULL");
   if ((st = pb::paged::check_rows(q, bytes, who, "q"))) return st;
+  if (!kv_rows) k = v = q;  // not read: without key rows they may be NULL
   if ((st = pb::paged::check_rows(k, bytes, who, "k"))) return st;
   if ((st = pb::paged::check_rows(v, bytes, who, "v"))) return st;
   if ((st = pb::paged::check_rows(out, bytes, who, "out"))) return st;

@@ -115,25 +115,27 @@ attention_few_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__
       page = (int)a.tables[(uint64_t)l_seq * a.table_width + key / a.cache.page_size];
   };
   auto send = [&] {  // sends for tile `load`
+    while (load < end && (load - seg0) * kKeys >= l_len) {  // no keys, no tile to wait for
+      ++load;
+      look();
+    }
     if (load >= end) return;
     const uint32_t key = (load - seg0) * kKeys;
-    if (key < l_len) {  // a segment without keys has one empty tile
-      const int st = loaded % kStages;
-      const uint32_t count = min((uint32_t)kKeys / size, ceil_div(l_len - key, size));
-      const uint32_t to = smem_u32(ring) + st * 2 * C::kTile;
-      expect_tx(leader, &full[st], 2 * count * size * kHalves * 128);
-      for (uint32_t b = 0; b < count; ++b) {
-        const int at = __shfl_sync(0xffffffffu, page, b);
+    const int st = loaded % kStages;
+    const uint32_t count = min((uint32_t)kKeys / size, ceil_div(l_len - key, size));
+    const uint32_t to = smem_u32(ring) + st * 2 * C::kTile;
+    expect_tx(leader, &full[st], 2 * count * size * kHalves * 128);
+    for (uint32_t b = 0; b < count; ++b) {
+      const int at = __shfl_sync(0xffffffffu, page, b);
 #pragma unroll
-        for (int c = 0; c < kHalves; ++c) {
-          tma_4d(leader, to + c * C::kBlock + b * size * 128, &maps.k, c * 64, (int)(key % a.cache.page_size),
-                 (int)l_head, at, &full[st]);
-          tma_4d(leader, to + C::kTile + c * C::kBlock + b * size * 128, &maps.v, c * 64,
-                 (int)(key % a.cache.page_size), (int)l_head, at, &full[st]);
-        }
+      for (int c = 0; c < kHalves; ++c) {
+        tma_4d(leader, to + c * C::kBlock + b * size * 128, &maps.k, c * 64, (int)(key % a.cache.page_size),
+               (int)l_head, at, &full[st]);
+        tma_4d(leader, to + C::kTile + c * C::kBlock + b * size * 128, &maps.v, c * 64,
+               (int)(key % a.cache.page_size), (int)l_head, at, &full[st]);
       }
-      ++loaded;
     }
+    ++loaded;
     ++load;
     look();
   };

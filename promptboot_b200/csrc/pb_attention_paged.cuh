@@ -176,7 +176,6 @@ __device__ __forceinline__ void take_piece(const AttnArgs& a, const uint32_t* pr
     p.row_tile = x / tiles % row_tiles;
     if (p.tile0 > 0 || p.tile1 < tiles) p.partial = partial_of(run, p.tile0 == 0);
     next += p.tile1 - p.tile0;
-    if (s.len == 0) p.tile1 = p.tile0 = 0;  // nothing to see
   } else {
     p.head = x % a.kv_heads;
     p.row_tile = row_tiles - 1 - x / a.kv_heads;
@@ -185,6 +184,10 @@ __device__ __forceinline__ void take_piece(const AttnArgs& a, const uint32_t* pr
     p.tile1 = ceil_div(row_view<false>(a, s, last / a.group).all, kKeys);
     ++next;
   }
+  // Offsets that do not ascend can make the work overflow its counters: what is then no
+  // segment has no rows and no tiles.
+  if (p.row_tile >= row_tiles || p.head >= a.kv_heads) rows = 0;
+  if (rows == 0 || s.len == 0) p.tile1 = p.tile0 = 0;  // nothing to see
 }
 
 // Four consecutive elements, rounded once.
@@ -217,10 +220,11 @@ __device__ __forceinline__ void note_join(const AttnArgs& a, const uint32_t* pre
     uint32_t x = edge;
     const Sequence s = load_sequence<true>(a, find_sequence(prefix, a.seqs, x));
     const uint32_t tiles = max(1u, ceil_div(s.len, kKeys)), begin = edge - x % tiles;
-    if (begin != edge && begin >= share.start(run)) {  // else it begins at the edge, or in an earlier run
-      const uint32_t rows = s.t * a.group, row_tiles = ceil_div(rows, kRows);
-      j = {share.holder(begin + tiles - 1), s.q0, rows, x / tiles / row_tiles, x / tiles % row_tiles};
-    }
+    const uint32_t rows = s.t * a.group, row_tiles = max(1u, ceil_div(rows, kRows));
+    const uint32_t head = x / tiles / row_tiles;
+    // else it begins at the edge, or in an earlier run (or is none: see take_piece)
+    if (begin != edge && begin >= share.start(run) && head < a.kv_heads)
+      j = {min(share.holder(begin + tiles - 1), share.runs - 1), s.q0, rows, head, x / tiles % row_tiles};
   }
   a.joins[run] = j;
 }

@@ -189,7 +189,7 @@ uint32_t pb_cache_copy_pages_device(const pb_cache* cache, uint32_t n, const uin
   const uint32_t page_words = cache->kv_heads * cache->page_size * cache->head_dim * bytes / 16;
   const uint32_t unroll = page_words % 128 == 0 ? 4 : 1;
   const uint64_t units = (uint64_t)n * cache->layers * 2 * (page_words / (32 * unroll));
-  const uint32_t grid = (uint32_t)std::min<uint64_t>((units + 7) / 8, 148 * 8);
+  const uint32_t grid = (uint32_t)std::min<uint64_t>((units + 7) / 8, 0x7fffffffu);
   auto* k = static_cast<uint8_t*>(cache->k);
   auto* v = static_cast<uint8_t*>(cache->v);
   auto kernel = unroll == 4 ? pb::copy_pages_kernel<4> : pb::copy_pages_kernel<1>;

@@ -297,6 +297,46 @@ def test_prompt_attention_of_stacked_views_and_a_given_scale(dtype):
         check_heads(by_head.transpose(0, 1)[rows], q[rows], k[rows], v[rows], causal(t, t), 0.3, dtype)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_prompt_attention_of_keys_by_head_and_of_one_expanded_head(dtype):
+    g = gen(13)
+    q = normal(g, 200, 4, 64, dtype=dtype)
+    k, v = (normal(g, 2, 200, 64, dtype=dtype).transpose(0, 1) for _ in range(2))  # stored [heads, rows, dim]
+    got = ops.prompt_attention(q, k, v, starts([150, 50]))
+    assert torch.equal(got, ops.prompt_attention(q, k.contiguous(), v.contiguous(), starts([150, 50])))
+    one = k[:, :1].expand(200, 4, 64)  # a head stride of zero
+    got = ops.prompt_attention(q, one, v[:, 1:].expand(200, 4, 64), starts([150, 50]))
+    want = ops.prompt_attention(q, k[:, :1].contiguous(), v[:, 1:].contiguous(), starts([150, 50]))
+    # four key heads or one with four query heads: the same sums over other row tiles
+    at = 0
+    for t in (150, 50):
+        check_heads(got[at:at + t], q[at:at + t], one[at:at + t], v[at:at + t, 1:].expand(t, 4, 64), causal(t, t), 0.125, dtype)
+        check_heads(want[at:at + t], q[at:at + t], k[at:at + t, :1], v[at:at + t, 1:], causal(t, t), 0.125, dtype)
+        at += t
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_prompt_attention_without_keys_is_zero(dtype):
+    g = gen(14)
+    q, none = normal(g, 30, 4, 64, dtype=dtype), normal(g, 1, 2, 64, dtype=dtype)[:0]
+    assert not ops.prompt_attention(q, none, none, starts([10, 20]), kv_offsets=starts([0, 0])).any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_with_offsets_that_do_not_ascend_stays_in_its_buffers(dtype):
+    """Results are those of the sequences that are there; the others have no rows."""
+    g, rng = gen(15), np.random.default_rng(15)
+    q, k, v = (normal(g, 64, h, 64, dtype=dtype) for h in (4, 2, 2))
+    out = torch.full_like(q, 3.0)
+    ops.prompt_attention(q, k, v, i32([60, 20, 20, 64, 10]), out=out)  # 60..20 and 64..10 are none
+    assert torch.equal(out[20:], ops.prompt_attention(q[20:], k[20:], v[20:], i32([0, 44]))) and (out[:20] == 3.0).all()
+    cache, tables, _, _ = paged(g, rng, [40, 40, 40], 16, 2, 64, dtype)
+    visible = masks([1] * 64)
+    out = torch.full_like(q, 3.0)
+    ops.tree_attention(q, cache, tables, i32([39, 39, 39]), i32([5, 3, 4, 2]), visible, layer=1, out=out)
+    assert (out[:3] == 3.0).all() and (out[4:] == 3.0).all() and not (out[3] == 3.0).any()
+
+
 def test_prompt_attention_cuts_offsets_at_the_rows():
     g = gen(11)
     q, k, v = (normal(g, 40, 2, 64) for _ in range(3))
@@ -604,6 +644,38 @@ def test_operators_on_a_side_stream_and_in_graphs():
     want = chain()
     for out in outs:
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_first_calls_of_a_process_may_be_captured():
+    """Nothing has to be set up before a capture."""
+    import subprocess
+    import sys
+    code = """
+import torch
+from promptboot_b200 import ops
+i = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+q, k = torch.randn(4, 2, 64, device="cuda").bfloat16(), torch.randn(4, 1, 64, device="cuda").bfloat16()
+cache = ops.PageCache.empty(1, 4, 1, 16, 64)
+cache.k.zero_(); cache.v.fill_(1.0)
+offsets, tables, contexts, one, at = i([0, 4]), i([[0, 1]]), i([9]), torch.ones(4, dtype=torch.int64, device="cuda"), i([0, 1, 2, 3])
+slots, pairs, counts, nodes = i([-1] * 4), i([[0, 2]]), i([1]), i([[0]])
+plan = ops.Rotary(64)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    a = plan.apply_to_cache(q, k, k, at, cache, slots)
+    b = ops.prompt_attention(a, k, k, offsets)
+    c = ops.tree_attention(a, cache, tables, contexts, offsets, one)
+    d = ops.prompt_attention(q.float(), k.float(), k.float(), offsets)
+    cache.copy_pages(pairs)
+    cache.keep(tables, contexts, counts, nodes)
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(c, torch.ones_like(c)) and torch.equal(b, ops.prompt_attention(a, k, k, offsets))
+from promptboot_b200 import _lib
+assert _lib.load().pb_attention_status(None) == 0
+"""
+    assert subprocess.run([sys.executable, "-c", code], timeout=120).returncode == 0
 
 
 # ---------------------------------------------------------------- the run of them
