@@ -43,6 +43,13 @@ uint32_t few_tiles(uint32_t head_dim, uint64_t rows, uint32_t seqs) {
   return head_dim == 64 && rows <= 32ull * seqs ? 2 : 0;
 }
 
+// Row tile of the binary32 kernel for few rows that holds a sequence's rows of one key
+// head on average, 0 where they are more than 16.
+uint32_t few32_rows(uint64_t rows, uint32_t seqs) {
+  if (rows <= 8ull * seqs) return 8;
+  return rows <= 16ull * seqs ? 16 : 0;
+}
+
 constexpr float kLog2E = 1.4426950408889634f;
 
 }  // namespace
@@ -90,11 +97,13 @@ uint64_t pb_tree_attention_workspace(uint32_t type, uint32_t head_dim, uint32_t 
                                      uint32_t kv_heads, uint32_t seqs, uint32_t rows) {
   if (pb::paged::check_heads("pb_tree_attention_workspace", type, head_dim, q_heads, kv_heads, seqs, rows))
     return 0;
-  if (pb::paged::type_bytes(type) == 2) {
-    const uint32_t tiles = pb::paged::few_tiles(head_dim, rows * (q_heads / kv_heads), seqs);
-    return (tiles ? pb::paged::few_tree_words(head_dim, tiles) : pb::paged::tc_tree_words(head_dim)) * 4;
+  const uint64_t all = (uint64_t)rows * (q_heads / kv_heads);
+  if (type == PB_TYPE_F32) {
+    const uint32_t tile = pb::paged::few32_rows(all, seqs);
+    return (tile ? pb::paged::few32_tree_words(head_dim, tile) : pb::paged::simt_tree_words(head_dim)) * 4;
   }
-  return pb::paged::simt_tree_words(head_dim, rows * (q_heads / kv_heads), seqs) * 4;
+  const uint32_t tiles = pb::paged::few_tiles(head_dim, all, seqs);
+  return (tiles ? pb::paged::few_tree_words(head_dim, tiles) : pb::paged::tc_tree_words(head_dim)) * 4;
 }
 
 uint32_t pb_tree_attention_device(const pb_cache* cache, uint32_t layer, uint32_t q_heads,
@@ -116,9 +125,9 @@ uint32_t pb_tree_attention_device(const pb_cache* cache, uint32_t layer, uint32_
   if ((st = pb::paged::check_rows(out, bytes, who, "out"))) return st;
   if (!tables || !table_width || !contexts || !offsets || !visible)
     return refuse(PB_CAPACITY, who, "an empty table or a NULL argument");
-  // Key tiles (of 16 keys at least, for row tiles of 16 at least) are counted in 32 bits.
+  // Key tiles (of 16 keys at least, for row tiles of 8 at least) are counted in 32 bits.
   const uint64_t group = q_heads / cache->kv_heads, reach = (uint64_t)table_width * cache->page_size;
-  const uint64_t segments = (rows * group / 16 + seqs) * cache->kv_heads;
+  const uint64_t segments = (rows * group / 8 + seqs) * cache->kv_heads;
   if (reach >= 1ull << 30 || segments * (reach / 16 + 1) >= 1ull << 31)
     return refuse(PB_CAPACITY, who, "the tables reach too far for so many sequences and rows");
   const uint64_t need = pb_tree_attention_workspace(cache->type, cache->head_dim, q_heads,
@@ -140,13 +149,15 @@ uint32_t pb_tree_attention_device(const pb_cache* cache, uint32_t layer, uint32_
     return tiles ? pb::paged::few_tree(a, cache->type, cache->head_dim, tiles, (cudaStream_t)stream)
                  : pb::paged::tc_tree(a, cache->type, cache->head_dim, (cudaStream_t)stream);
   }
+  if (const uint32_t tile = pb::paged::few32_rows(rows * group, seqs))
+    return pb::paged::few32_tree(a, cache->head_dim, tile, (cudaStream_t)stream);
   return pb::paged::simt_tree(a, cache->head_dim, (cudaStream_t)stream);
 }
 
 uint32_t pb_attention_status(void* stream) {
   PB_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
-  const uint32_t a = pb::paged::tc_status(), b = pb::paged::few_status();
-  return a ? a : b;
+  const uint32_t a = pb::paged::tc_status(), b = pb::paged::few_status(), c = pb::paged::few32_status();
+  return a ? a : b ? b : c;
 }
 
 }  // extern "C"

@@ -89,59 +89,8 @@ attention_few_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__
   uint32_t next = run < share.runs ? share.start(run) : total;
   const uint32_t end = run < share.runs ? share.start(run + 1) : total;
 
-  // This warp's ring.  Tile `load` of the list goes to stage loaded % kStages; its
-  // segment, (sequence, head) with tile 0 at seg0, is decoded where it changes; the page
-  // ids of a tile are fetched when the one before is sent for.
-  uint64_t* full = bars + warp * kStages;
-  uint8_t* ring = smem + warp * kStages * 2 * C::kTile;
-  const uint32_t leader = elect_one();
-  const uint32_t size = min(a.cache.page_size, (uint32_t)kKeys);  // keys of a box
-  uint32_t load = next, seg0 = 0, seg1 = 0, l_seq = 0, l_head = 0, l_len = 0;
-  int loaded = 0, page = 0;
-  auto look = [&] {  // decodes tile `load` and fetches its page ids
-    if (load >= end) return;
-    if (load >= seg1) {
-      uint32_t x = load;
-      l_seq = find_sequence(prefix, a.seqs, x);
-      const Sequence q = load_sequence<true>(a, l_seq);
-      const uint32_t tiles = max(1u, ceil_div(q.len, kKeys)), segment = x / tiles;
-      l_len = q.len;
-      l_head = segment / ceil_div(q.t * a.group, kRows);
-      seg0 = load - x % tiles;
-      seg1 = seg0 + tiles;
-    }
-    const uint32_t key = (load - seg0) * kKeys + lane * size;
-    if (lane * size < kKeys && key < l_len)
-      page = (int)a.tables[(uint64_t)l_seq * a.table_width + key / a.cache.page_size];
-  };
-  auto send = [&] {  // sends for tile `load`
-    while (load < end && (load - seg0) * kKeys >= l_len) {  // no keys, no tile to wait for
-      ++load;
-      look();
-    }
-    if (load >= end) return;
-    const uint32_t key = (load - seg0) * kKeys;
-    const int st = loaded % kStages;
-    const uint32_t count = min((uint32_t)kKeys / size, ceil_div(l_len - key, size));
-    const uint32_t to = smem_u32(ring) + st * 2 * C::kTile;
-    expect_tx(leader, &full[st], 2 * count * size * kHalves * 128);
-    for (uint32_t b = 0; b < count; ++b) {
-      const int at = __shfl_sync(0xffffffffu, page, b);
-#pragma unroll
-      for (int c = 0; c < kHalves; ++c) {
-        tma_4d(leader, to + c * C::kBlock + b * size * 128, &maps.k, c * 64, (int)(key % a.cache.page_size),
-               (int)l_head, at, &full[st]);
-        tma_4d(leader, to + C::kTile + c * C::kBlock + b * size * 128, &maps.v, c * 64,
-               (int)(key % a.cache.page_size), (int)l_head, at, &full[st]);
-      }
-    }
-    ++loaded;
-    ++load;
-    look();
-  };
-  look();
-#pragma unroll
-  for (int i = 0; i < kStages; ++i) send();
+  TileRing<T, kRows, kKeys, kHalves, kStages> ring(a, maps, prefix, bars + warp * kStages,
+                                                   smem + warp * kStages * 2 * C::kTile, next, end);
   if (lane == 0) note_join<kRows, kKeys>(a, prefix, share, run);
 
   const int r0 = lane >> 2, c0 = (lane & 3) * 2;  // this thread's fragment row (and + 8) and column
@@ -188,10 +137,9 @@ attention_few_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__
     const uint32_t mask0 = s.context / kKeys;  // tiles from here on hold a key that some row does not see
 
     for (uint32_t tile = p.tile0; tile < p.tile1; ++tile) {
-      const int st = used % kStages;
-      if (!wait_soon(&full[st], (used / kStages) & 1, abort_flag)) { stop = true; break; }
-      ++used;
-      const uint32_t kt = smem_u32(ring) + st * 2 * C::kTile, vt = kt + C::kTile;
+      if (!wait_soon(&ring.full[used % kStages], (used / kStages) & 1, abort_flag)) { stop = true; break; }
+      uint8_t* tile_keys = ring.keys(used++);
+      const uint32_t kt = smem_u32(tile_keys), vt = kt + C::kTile;
       float sc[kTiles][kKeys / 8][4];
 #pragma unroll
       for (int g = 0; g < kTiles; ++g)
@@ -275,7 +223,7 @@ attention_few_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__
       if (masked) {
         // The tile's value rows: zero past the keys, and without what is not finite.
         mend |= __any_sync(0xffffffffu, lane < kKeys && clean_value_row<F, kDim, C::kBlock>(
-                                            ring + st * 2 * C::kTile + C::kTile, lane, key0 + lane >= s.len));
+                                            tile_keys + C::kTile, lane, key0 + lane >= s.len));
       }
 #pragma unroll
       for (int j = 0; j < kKeys / 16; ++j) {
@@ -293,7 +241,7 @@ attention_few_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__
       }
       if (masked) fence_async_smem();  // cleaned rows before the next copy over them
       __syncwarp();
-      send();
+      ring.send();
     }
 
     if (stop) break;
@@ -348,9 +296,7 @@ attention_few_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__
       }
     }
   }
-  // After a wait that gave up, copies may be under way: they land before the CTA exits.
-  for (int i = max(used, loaded - kStages); i < loaded; ++i)
-    wait_drain(&full[i % kStages], (i / kStages) & 1, 50000000ull);
+  if (stop) ring.drain(used);
   __syncthreads();
   if (*abort_flag && tid == 0) mark_timeout();
 }

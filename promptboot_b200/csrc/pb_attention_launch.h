@@ -9,11 +9,11 @@ namespace paged {
 // CTAs that share a tree call's key tiles: so many on each SM of the current device.
 uint32_t tree_ctas(uint32_t per_sm);
 
-// Prompt attention; tree attention and the words of its workspace, for rows =
-// q_rows * group: binary32 elements on the CUDA cores.
+// Prompt attention; tree attention and the words of its workspace: binary32 elements
+// on the CUDA cores.
 uint32_t simt_prompt(const AttnArgs& a, uint32_t head_dim, cudaStream_t s);
 uint32_t simt_tree(const AttnArgs& a, uint32_t head_dim, cudaStream_t s);
-uint64_t simt_tree_words(uint32_t head_dim, uint32_t rows, uint32_t seqs);
+uint64_t simt_tree_words(uint32_t head_dim);
 
 // The same on the tensor cores, for 16-bit elements; whether a wait of theirs gave
 // up since the last look.
@@ -27,6 +27,11 @@ uint32_t tc_status();
 uint32_t few_tree(const AttnArgs& a, uint32_t type, uint32_t head_dim, uint32_t tiles, cudaStream_t s);
 uint64_t few_tree_words(uint32_t head_dim, uint32_t tiles);
 uint32_t few_status();
+
+// The same of binary32 elements, with row tiles of 8 or 16.
+uint32_t few32_tree(const AttnArgs& a, uint32_t head_dim, uint32_t tile_rows, cudaStream_t s);
+uint64_t few32_tree_words(uint32_t head_dim, uint32_t tile_rows);
+uint32_t few32_status();
 
 }  // namespace paged
 }  // namespace pb

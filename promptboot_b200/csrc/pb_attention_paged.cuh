@@ -232,7 +232,7 @@ __device__ __forceinline__ void note_join(const AttnArgs& a, const uint32_t* pre
 // Joins the partials of the segments that crossed runs: weights 2^(m_i - m), in the
 // order of the runs, so the result does not depend on timing.  A segment is joined by
 // the CTAs of the run in which it begins.  A thread has four elements of a row and loads
-// four or eight partials at a time: latency is what there is to save here.
+// eight partials at a time: latency is what there is to save here.
 constexpr int kCombine = 128;  // threads
 template <class T, int kDim, int kRows>
 __global__ void __launch_bounds__(kCombine) combine_kernel(const __grid_constant__ AttnArgs a) {
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(kCombine) combine_kernel(const __grid_constant
   const uint32_t c = blockIdx.x;
   const Join j = a.joins[c];
   if (j.last == PB_NONE) return;
-  constexpr int kPerRow = kDim / 4, kStep = kCombine / kPerRow, kBatch = kRows > 32 ? 8 : 4;
+  constexpr int kPerRow = kDim / 4, kStep = kCombine / kPerRow, kBatch = 8;
   const int chunk = (threadIdx.x % kPerRow) * 4;
   for (uint32_t r = blockIdx.y * kStep + threadIdx.x / kPerRow; r < kRows; r += gridDim.y * kStep) {
     const uint32_t row = j.row_tile * kRows + r;

@@ -270,18 +270,10 @@ uint32_t simt_prompt(const AttnArgs& a, uint32_t head_dim, cudaStream_t s) {
   return head_dim == 64 ? launch<64, kManyRpt, false>(a, grid, s) : launch<128, kManyRpt, false>(a, grid, s);
 }
 
-// Row tiles of 16 where a sequence has no more rows than that on average.
-static bool few(uint32_t rows, uint32_t seqs) { return rows <= 16 * seqs; }
-
-uint64_t simt_tree_words(uint32_t head_dim, uint32_t rows, uint32_t seqs) {
-  const uint32_t tile = few(rows, seqs) ? 8 * kFewRpt : 8 * kManyRpt;
-  return tree_words(tree_ctas(4), tile, head_dim);
-}
+uint64_t simt_tree_words(uint32_t head_dim) { return tree_words(tree_ctas(4), 8 * kManyRpt, head_dim); }
 
 uint32_t simt_tree(const AttnArgs& a, uint32_t head_dim, cudaStream_t s) {
   const uint32_t grid = tree_ctas(4);
-  if (few(a.q_rows * a.group, a.seqs))
-    return head_dim == 64 ? launch<64, kFewRpt, true>(a, grid, s) : launch<128, kFewRpt, true>(a, grid, s);
   return head_dim == 64 ? launch<64, kManyRpt, true>(a, grid, s) : launch<128, kManyRpt, true>(a, grid, s);
 }
 

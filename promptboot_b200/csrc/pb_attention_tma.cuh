@@ -13,6 +13,11 @@ namespace paged {
 template <class T>
 struct Format;
 template <>
+struct Format<float> {
+  static constexpr CUtensorMapDataType kMap = CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+  static constexpr float kSlack = 8.f;
+};
+template <>
 struct Format<__half> {
   static constexpr uint32_t kCode = 0;  // instruction descriptor
   static constexpr CUtensorMapDataType kMap = CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
@@ -110,6 +115,83 @@ __device__ __forceinline__ bool clean_value_row(uint8_t* tile, int key, bool pas
   return found;
 }
 
+struct Maps {
+  CUtensorMap k, v;
+  uint32_t k_step, v_step;  // 0: one key head's rows serve all
+};
+
+// A warp's ring of key and value tiles over its run [begin, end) of a tree's tile list,
+// which it fills itself: tile `load` goes to stage loaded % kStages, keys first, in
+// column blocks of 128 bytes (kBlocks of them) of kKeys rows.  Its segment, (sequence,
+// head) with tile 0 at seg0, is decoded where it changes; the page ids of a tile are
+// fetched when the one before is sent for.
+template <class T, int kRows, int kKeys, int kBlocks, int kStages>
+struct TileRing {
+  static constexpr int kBlock = kKeys * 128, kTile = kBlocks * kBlock;
+  const AttnArgs& a;
+  const Maps& maps;
+  const uint32_t* prefix;
+  uint64_t* full;  // one barrier per stage
+  uint8_t* ring;
+  uint32_t leader, size, load, end, seg0 = 0, seg1 = 0, seq = 0, head = 0, len = 0;
+  int lane, loaded = 0, page = 0;
+
+  __device__ __forceinline__ TileRing(const AttnArgs& a_, const Maps& maps_, const uint32_t* prefix_, uint64_t* full_,
+                                      uint8_t* ring_, uint32_t begin, uint32_t end_)
+      : a(a_), maps(maps_), prefix(prefix_), full(full_), ring(ring_), leader(elect_one()),
+        size(min(a_.cache.page_size, (uint32_t)kKeys)), load(begin), end(end_), lane(threadIdx.x & 31) {
+    look();
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) send();
+  }
+  __device__ __forceinline__ uint8_t* keys(int tile) const { return ring + tile % kStages * 2 * kTile; }
+  __device__ __forceinline__ void look() {  // decodes tile `load` and fetches its page ids
+    if (load >= end) return;
+    if (load >= seg1) {
+      uint32_t x = load;
+      seq = find_sequence(prefix, a.seqs, x);
+      const Sequence q = load_sequence<true>(a, seq);
+      const uint32_t tiles = max(1u, ceil_div(q.len, kKeys));
+      len = q.len;
+      head = x / tiles / max(1u, ceil_div(q.t * a.group, kRows));
+      seg0 = load - x % tiles;
+      seg1 = seg0 + tiles;
+    }
+    const uint32_t key = (load - seg0) * kKeys + lane * size;
+    if (lane * size < kKeys && key < len)
+      page = (int)a.tables[(uint64_t)seq * a.table_width + key / a.cache.page_size];
+  }
+  __device__ __forceinline__ void send() {  // sends for tile `load`
+    while (load < end && (load - seg0) * kKeys >= len) {  // no keys, no tile to wait for
+      ++load;
+      look();
+    }
+    if (load >= end) return;
+    const uint32_t key = (load - seg0) * kKeys, slot = key % a.cache.page_size;
+    uint64_t* bar = &full[loaded % kStages];
+    const uint32_t count = min((uint32_t)kKeys / size, ceil_div(len - key, size));
+    const uint32_t to = smem_u32(keys(loaded));
+    expect_tx(leader, bar, 2 * count * size * kBlocks * 128);
+    for (uint32_t b = 0; b < count; ++b) {
+      const int at = __shfl_sync(0xffffffffu, page, b);
+#pragma unroll
+      for (int c = 0; c < kBlocks; ++c) {
+        const int x = c * (int)(128 / sizeof(T));
+        tma_4d(leader, to + c * kBlock + b * size * 128, &maps.k, x, (int)slot, (int)head, at, bar);
+        tma_4d(leader, to + kTile + c * kBlock + b * size * 128, &maps.v, x, (int)slot, (int)head, at, bar);
+      }
+    }
+    ++loaded;
+    ++load;
+    look();
+  }
+  // On the way out: what was sent for after `used` tiles lands before the CTA exits.
+  __device__ __forceinline__ void drain(int used) {
+    for (int i = max(used, loaded - kStages); i < loaded; ++i)
+      wait_drain(&full[i % kStages], (i / kStages) & 1, 50000000ull);
+  }
+};
+
 // Set where a bounded wait of a kernel gave up (one word per source file).
 static __device__ unsigned int g_timeout;
 __device__ __forceinline__ void mark_timeout() { atomicOr(&g_timeout, 1u); }
@@ -125,11 +207,6 @@ static inline uint32_t take_status() {
 }
 
 // --------------------------------------------------------------- tensor maps (host)
-
-struct Maps {
-  CUtensorMap k, v;
-  uint32_t k_step, v_step;  // 0: one key head's rows serve all
-};
 
 using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                             const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -169,14 +246,14 @@ inline uint32_t encode_map(CUtensorMap* map, CUtensorMapDataType type, int rank,
   return PB_DEVICE;
 }
 
-// Keys and values of a cache layer: (element, slot, head, page), boxes of 64 elements
-// of one page's slots.
+// Keys and values of a cache layer: (element, slot, head, page), boxes of 128 bytes of
+// one page's slots.
 template <class T>
 uint32_t cache_maps(const AttnArgs& a, uint32_t head_dim, uint32_t tile_keys, Maps* maps) {
   const cuuint64_t dim = head_dim, size = a.cache.page_size;
   const cuuint64_t dims[4] = {dim, size, a.cache.kv_heads, a.cache.pages};
-  const cuuint64_t strides[3] = {dim * 2, size * dim * 2, a.cache.kv_heads * size * dim * 2};
-  const cuuint32_t box[4] = {64, (cuuint32_t)std::min<cuuint64_t>(size, tile_keys), 1, 1};
+  const cuuint64_t strides[3] = {dim * sizeof(T), size * dim * sizeof(T), a.cache.kv_heads * size * dim * sizeof(T)};
+  const cuuint32_t box[4] = {128 / sizeof(T), (cuuint32_t)std::min<cuuint64_t>(size, tile_keys), 1, 1};
   maps->k_step = maps->v_step = 1;
   uint32_t st = encode_map(&maps->k, Format<T>::kMap, 4, a.cache.k, dims, strides, box);
   if (!st) st = encode_map(&maps->v, Format<T>::kMap, 4, a.cache.v, dims, strides, box);
