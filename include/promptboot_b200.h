@@ -361,8 +361,8 @@ PB_API uint32_t pb_rotary_device(const pb_rotary *rotary, uint32_t type, uint32_
                                  const pb_rows *k, const pb_rows *k_out, void *stream);
 /* The same, with k turned and v as it is written to `layer` of the cache, whose
  * type, heads and head_dim they have, at slots_device[row] = page * page_size +
- * slot in the page.  A slot outside the cache (PB_NONE) writes no k and v; the
- * same slot twice holds either row. */
+ * slot in the page.  A slot outside the cache (PB_NONE) writes no k and v; of
+ * rows with the same slot it holds a mix. */
 PB_API uint32_t pb_rotary_cache_device(const pb_rotary *rotary, uint32_t rows,
                                        const uint32_t *positions_device, uint32_t q_heads,
                                        const pb_rows *q, const pb_rows *q_out, const pb_rows *k,
@@ -409,7 +409,8 @@ PB_API uint32_t pb_tree_attention_device(const pb_cache *cache, uint32_t layer, 
                                          void *workspace, uint64_t workspace_bytes, void *stream);
 
 /* Waits for `stream` and reports a prompt or tree attention whose kernel gave up
- * waiting for a copy or a product (PB_DEVICE, once; its outputs are not complete). */
+ * waiting for a copy or a product (PB_DEVICE, once; its outputs are not complete).
+ * Not to be called while a graph is captured. */
 PB_API uint32_t pb_attention_status(void *stream);
 
 /* Copies page pairs[2 i] to page pairs[2 i + 1] for i < n, keys and values of
@@ -420,8 +421,8 @@ PB_API uint32_t pb_cache_copy_pages_device(const pb_cache *cache, uint32_t n,
 /* Keeps the accepted nodes of drafted trees: for every layer, position contexts
  * [s] + nodes[s * nodes_width + i] moves to contexts[s] + i, for i < counts[s]
  * (cut at nodes_width).  nodes ascend within a sequence; an entry below its own
- * index, below the one before it, or past the table, and a page id outside the
- * cache, is left out.  The pages that are written belong to one sequence each. */
+ * index, not above all those before it, or past the table, and a page id outside
+ * the cache, is left out.  The pages that are written belong to one sequence each. */
 PB_API uint32_t pb_cache_keep_device(const pb_cache *cache, uint32_t seqs,
                                      const uint32_t *tables_device, uint32_t table_width,
                                      const uint32_t *contexts_device,

@@ -64,7 +64,8 @@ struct KeepArgs {
 constexpr int kBatch = 8, kMoves = 128;
 __global__ void __launch_bounds__(128) keep_kernel(const __grid_constant__ KeepArgs a) {
   __shared__ uint32_t sources[kMoves], targets[kMoves];  // rows of head 0 in units of page slots; PB_NONE: no move
-  __shared__ uint32_t warp_top[4], warp_moves[4];
+  __shared__ int64_t warp_top[4];
+  __shared__ uint32_t warp_moves[4];
   const uint32_t seq = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t column = blockIdx.x * 128 + tid;
   const uint32_t* table = a.tables + (uint64_t)seq * a.table_width;
@@ -91,15 +92,14 @@ __global__ void __launch_bounds__(128) keep_kernel(const __grid_constant__ KeepA
       if (lane >= d) before = max(before, o);
     }
     __syncthreads();  // the moves before have been read
-    if (lane == 31) warp_top[warp] = (uint32_t)max((int64_t)0, before + 1);
+    if (lane == 31) warp_top[warp] = before;
     int64_t up_to = __shfl_up_sync(0xffffffffu, before, 1);
     if (lane == 0) up_to = -1;
     __syncthreads();
     up_to = max(up_to, top);
     for (uint32_t w = 0; w < 4; ++w) {
-      const int64_t x = (int64_t)warp_top[w] - 1;
-      if (w < warp) up_to = max(up_to, x);
-      top = max(top, x);
+      if (w < warp) up_to = max(up_to, warp_top[w]);
+      top = max(top, warp_top[w]);
     }
     bool move = i < count && i < a.nodes_width && n > (int64_t)i && n > up_to;  // n = i stays where it is
     uint32_t from = PB_NONE, to = PB_NONE;

@@ -8,7 +8,8 @@ current torch stream, and returns at once.  Index tensors are contiguous int32
 (or uint32), -1 standing for none; head tensors are [rows, heads, head_dim] of
 float32, float16 or bfloat16 with a contiguous last dimension, any other strides a
 multiple of 16 bytes, so that views of a stacked q/k/v projection serve as they
-are.  Refused arguments raise OperatorError.
+are.  Refused arguments raise OperatorError.  There are no gradients: a tensor that
+asks for one is refused unless grad mode is off.
 """
 from __future__ import annotations
 
@@ -75,6 +76,8 @@ def _heads(t, dtype, device, name):
         raise OperatorError(f"{name} must be [rows, heads, head_dim] with a contiguous last dimension")
     if t.dtype is not dtype or t.get_device() != device:
         raise OperatorError(f"{name} has another type or device")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise OperatorError(f"{name} asks for a gradient, which the serving operators do not have")
     return _Rows(t.data_ptr(), s[0], s[1])
 
 
@@ -271,6 +274,13 @@ def tree_attention(q, cache, tables, contexts, offsets, visible, layer=0, scale=
     _call(device, _lib.load().pb_tree_attention_device, _ref(cache._c), layer, heads, seqs, rows, _ref(q_in),
           _ref(to), a, width, b, c, d, dim ** -0.5 if scale is None else scale, workspace.data_ptr(), workspace.numel())
     return out
+
+
+def attention_status(device=None):
+    """Waits for the device's current stream and raises DeviceError where an attention
+    on that device gave up waiting since the last call (its outputs are not complete)."""
+    device = torch.cuda.current_device() if device is None else torch.device(device).index or 0
+    _call(device, _lib.load().pb_attention_status)
 
 
 class PagePool:

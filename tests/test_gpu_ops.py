@@ -494,6 +494,26 @@ def test_tree_attention_tables_that_end_and_pages_outside_the_cache(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,heads,nodes", [(64, 3, 1), (64, 3, 5), (128, 5, 1), (128, 5, 3), (64, 3, 40)])
+def test_tree_attention_of_growing_and_of_falling_scores(dtype, dim, heads, nodes):
+    """The maximum moves in every tile, or in the first alone, by far more than the
+    sums could bear without being scaled; and all scores alike."""
+    g, rng = gen(24), np.random.default_rng(24)
+    n = 900
+    cache, tables, keys, values = paged(g, rng, [n + nodes] * 3, 16, 1, dim, dtype)
+    ramp = torch.linspace(-6, 6, n + nodes, device="cuda")[:, None, None].expand(-1, 1, dim).to(dtype)
+    for s, rows in enumerate([ramp, ramp.flip(0), ramp * 0 + 1]):
+        keys[s] = rows.contiguous()
+        ids = tables[s, :-(-(n + nodes) // 16)].long()
+        p = torch.arange(n + nodes, device="cuda")
+        cache.k[1][ids[p // 16], :, p % 16] = keys[s]
+    q = torch.ones(3 * nodes, heads, dim, device="cuda", dtype=dtype)
+    visible = [b for _ in range(3) for b in random_tree(rng, nodes)]
+    got = ops.tree_attention(q, cache, tables, i32([n] * 3), starts([nodes] * 3), masks(visible), layer=1, scale=0.7)
+    check_tree(got, q, [n] * 3, [nodes] * 3, visible, keys, values, 0.7, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("seqs,nodes", [(1, 1), (2, 48), (300, 1), (40, 3)])
 def test_tree_attention_of_long_and_of_many_contexts(dtype, seqs, nodes):
     """Contexts that are split over many CTAs, and more sequences than CTAs; the
@@ -595,6 +615,26 @@ def test_keep_leaves_out_entries_that_are_no_path():
     move(want, before, 15, 12)
     assert torch.equal(cache.k, want)
     assert torch.equal(cache.v, want + 1)
+
+
+def test_keep_of_long_rows_with_entries_that_stand_for_none():
+    """-1 is above every node: what stands behind it is left out, within 32 entries and
+    beyond; a row of more than 128 entries goes on where it stopped."""
+    g = gen(31)
+    cache = ops.PageCache.empty(1, 40, 1, 16, 16, torch.float32)
+    cache.k.copy_(normal(g, *cache.k.shape))
+    cache.v.copy_(cache.k + 1)
+    before = cache.k.clone()
+    tables = torch.arange(40, dtype=torch.int32, device="cuda").view(2, 20)
+    path = list(range(3, 203))
+    rows = [path, path[:31] + [-1] + path[32:]]
+    cache.keep(tables, i32([7, 7]), i32([200, 200]), i32(rows))
+    want = before.clone()
+    for s, count in enumerate([200, 31]):
+        for i in range(count):
+            a, b = 10 + i, 7 + i
+            want[0, 20 * s + b // 16, :, b % 16] = before[0, 20 * s + a // 16, :, a % 16]
+    assert torch.equal(cache.k, want) and torch.equal(cache.v, want + 1)
 
 
 # ------------------------------------------------------------- streams and graphs
@@ -804,3 +844,14 @@ def test_refusals_launch_nothing():
         stack = torch.zeros(4, 6, 64, device="cuda")
         ops.Rotary(64).apply(stack[:, :2], stack[:, 2:3], i32([0, 1, 2, 3]), q_out=stack.view(-1)[:512].view(4, 2, 64))
     assert ops.prompt_attention(q[:0], k[:0], k[:0], i32([0, 0])).shape == (0, 2, 64)
+
+
+def test_tensors_that_ask_for_gradients_are_refused_and_the_status_is_clean():
+    q = torch.zeros(4, 2, 64, device="cuda", requires_grad=True)
+    k = torch.zeros(4, 2, 64, device="cuda")
+    with pytest.raises(ops.OperatorError, match="gradient"):
+        ops.prompt_attention(q, k, k, i32([0, 4]))
+    with torch.no_grad():
+        assert not ops.prompt_attention(q, k, k, i32([0, 4])).any()
+    ops.attention_status()
+    ops.attention_status("cuda:0")
