@@ -125,10 +125,11 @@ uint32_t pb_tree_attention_device(const pb_cache* cache, uint32_t layer, uint32_
   if ((st = pb::paged::check_rows(out, bytes, who, "out"))) return st;
   if (!tables || !table_width || !contexts || !offsets || !visible)
     return refuse(PB_CAPACITY, who, "an empty table or a NULL argument");
-  // Key tiles (of 16 keys at least, for row tiles of 8 at least) are counted in 32 bits.
+  // Key tiles are counted in 32 bits: of `least` keys or more, for row tiles of `least` or more.
   const uint64_t group = q_heads / cache->kv_heads, reach = (uint64_t)table_width * cache->page_size;
-  const uint64_t segments = (rows * group / 8 + seqs) * cache->kv_heads;
-  if (reach >= 1ull << 30 || segments * (reach / 16 + 1) >= 1ull << 31)
+  const uint32_t least = bytes == 4 ? 8 : 16;
+  const uint64_t segments = (rows * group / least + seqs) * cache->kv_heads;
+  if (reach >= 1ull << 30 || segments * (reach / least + 1) >= 1ull << 31)
     return refuse(PB_CAPACITY, who, "the tables reach too far for so many sequences and rows");
   const uint64_t need = pb_tree_attention_workspace(cache->type, cache->head_dim, q_heads,
                                                     cache->kv_heads, seqs, rows);

@@ -1,14 +1,16 @@
 // Tree attention of few rows per sequence and key head in binary32 (products and
 // sums too): the counterpart of pb_attention_few.cu on the CUDA cores.
 //
-// Each warp walks a run of tiles of 16 KB of keys and values through a ring of its own
-// (128-byte swizzle).  Scores: a lane has a key (at heads of 128 half of one) and all
-// rows, whose queries it reads from shared memory, the same word for every lane.
-// Weights go through shared memory; values: a lane has kDim / 32 elements and all rows.
-// The running maximum moves only where a score passes it by more than kSlack, so that
-// it takes the warp's shuffles seldom.  Per tile some 1000 multiply-adds a lane against
-// 16 KB from memory: the SM's four schedulers keep up with twice its share of the
-// memory's rate at 8 rows, and with all of it at 16.
+// Each warp walks a run of tiles through a ring of its own (128-byte swizzle).  Scores:
+// a lane has a key, or half of one, and all rows, whose queries it reads from shared
+// memory, the same word for every lane.  Weights go through shared memory; values: a
+// lane has kDim / 32 elements and all rows.  The running maximum moves only where a
+// score passes it by more than kSlack, so that it takes the warp's shuffles seldom.
+//
+// Bound by the latency of a warp's chain through a tile, with two or three warps to a
+// scheduler (a third of its issue slots): 69 us for 256 single tokens over 512 to 1024
+// positions, 14 heads of 64 to 2 (2.95 TB/s), 210 us for 16 over 6000, 32 heads of 128
+// to 8 (3.5 TB/s).  The first took 138 us on row tiles of 16 of pb_attention_simt.cu.
 #include "pb_attention_launch.h"
 #include "pb_attention_tma.cuh"
 
@@ -16,18 +18,22 @@ namespace pb {
 namespace paged {
 namespace {
 
-constexpr int kWarps = 5;  // what shared memory holds
-constexpr int kThreads = kWarps * 32;
-constexpr int kLeast = 2;
 constexpr int kStages = 2;
 
 template <int kDim, int kRows>
 struct Few32 {
-  static constexpr int kSplit = kDim / 64;             // lanes of a key
+  // Ten warps with tiles of 8 KB of keys and values, or five with tiles of 16: ten are
+  // faster where their sums leave the registers (64 x 8: 69 against 77 us for 256 single
+  // tokens, 2.95 TB/s), five else (128 x 16: 209 against 233 us for 64 x 4 nodes).
+  static constexpr bool kMany = kDim == 64 && kRows == 8;
+  static constexpr int kWarps = kMany ? 10 : 5;
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kLeast = kMany ? 4 : 2;         // tiles of a run
+  static constexpr int kSplit = kMany ? 2 : kDim / 64; // lanes of a key
   static constexpr int kKeys = 32 / kSplit;
   static constexpr int kBlocks = kDim / 32;            // 128-byte column blocks of a row
   static constexpr int kBlock = kKeys * 128;
-  static constexpr int kTile = kBlocks * kBlock;       // K or V: 8 KB
+  static constexpr int kTile = kBlocks * kBlock;       // K or V
   static constexpr int kQOff = kWarps * kStages * 2 * kTile;
   static constexpr int kQ = kRows * kDim * 4;
   static constexpr int kPOff = kQOff + kWarps * kQ;
@@ -38,10 +44,10 @@ struct Few32 {
 };
 
 template <int kDim, int kRows>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Few32<kDim, kRows>::kThreads, 1)
 attention_few32_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Maps maps) {
   using C = Few32<kDim, kRows>;
-  constexpr int kKeys = C::kKeys, kSplit = C::kSplit, kE = kDim / 32;  // elements of a lane
+  constexpr int kKeys = C::kKeys, kSplit = C::kSplit, kWarps = C::kWarps, kE = kDim / 32;  // elements of a lane
   extern __shared__ uint8_t raw[];
   uint8_t* smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
@@ -57,9 +63,9 @@ attention_few32_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
     *abort_flag = 0;
     fence_barrier_init();
   }
-  work_prefix<true, kRows, kKeys, kThreads>(a, prefix);  // ends with a barrier of the block
+  work_prefix<true, kRows, kKeys, C::kThreads>(a, prefix);  // ends with a barrier of the block
   const uint32_t total = prefix[a.seqs - 1];
-  const Share<kLeast> share(total, gridDim.x * kWarps);
+  const Share<C::kLeast> share(total, gridDim.x * kWarps);
   const uint32_t run = blockIdx.x * kWarps + warp;
   uint32_t next = run < share.runs ? share.start(run) : total;
   const uint32_t end = run < share.runs ? share.start(run + 1) : total;
@@ -67,7 +73,7 @@ attention_few32_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
                                                          smem + warp * kStages * 2 * C::kTile, next, end);
   if (lane == 0) note_join<kRows, kKeys>(a, prefix, share, run);
 
-  const int key = lane / kSplit, half = lane % kSplit;  // of the scores
+  const int key = lane / kSplit, part = lane % kSplit;  // of the scores
   const int d0 = lane * kE;                             // of the values
   Sequence s;
   uint32_t rows;
@@ -107,9 +113,9 @@ attention_few32_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
 #pragma unroll
       for (int r = 0; r < kRows; ++r) x[r] = 0.f;
 #pragma unroll 4
-      for (int i = 0; i < 16; ++i) {
-        // the halves of a key take their words in another order: their banks differ
-        const int j = half ? i ^ 4 : i, block = half * 2 + j / 8, chunk = j % 8;
+      for (int i = 0; i < C::kBlocks / kSplit * 8; ++i) {
+        // the parts of a key take their words in other orders: their banks differ
+        const int chunk = i % 8 ^ (part * (8 / kSplit)), block = part * (C::kBlocks / kSplit) + i / 8;
         const float4 k4 = *reinterpret_cast<const float4*>(kt + block * C::kBlock + key * 128 + ((chunk ^ (key & 7)) * 16));
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
@@ -126,7 +132,8 @@ attention_few32_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
       uint32_t seen = 0xffffffffu;  // rows that see this lane's key
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
-        if (kSplit > 1) x[r] += __shfl_xor_sync(0xffffffffu, x[r], 1);
+#pragma unroll
+        for (int d = 1; d < kSplit; d <<= 1) x[r] += __shfl_xor_sync(0xffffffffu, x[r], d);
         x[r] = __fmul_rn(x[r], a.scale_log2);
         if (masked) {
           const uint32_t row = first + r;
@@ -161,10 +168,10 @@ attention_few32_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
         const float w = exp2_fast(x[r] - (m[r] == -INFINITY ? 0.f : m[r]));
-        if (half == 0) l[r] += w;
+        if (part == 0) l[r] += w;
         x[r] = (seen >> r) & 1 ? w : -0.f;
       }
-      if (half == 0) {
+      if (part == 0) {
 #pragma unroll
         for (int r = 0; r < kRows; r += 4)
           *reinterpret_cast<float4*>(ps + key * kRows + r) = make_float4(x[r], x[r + 1], x[r + 2], x[r + 3]);
@@ -251,16 +258,17 @@ uint32_t launch(AttnArgs a, cudaStream_t s) {
   uint32_t st = cache_maps<float>(a, kDim, C::kKeys, &maps);
   if (st) return st;
   const uint32_t grid = tree_ctas(1);
-  place_workspace(a, grid * kWarps, kRows, kDim);
-  kernel<<<grid, kThreads, C::bytes(a.seqs), s>>>(a, maps);
+  place_workspace(a, grid * C::kWarps, kRows, kDim);
+  kernel<<<grid, C::kThreads, C::bytes(a.seqs), s>>>(a, maps);
   PB_CUDA(cudaGetLastError());
-  return launch_combine<float, kDim, kRows>(a, grid * kWarps, s);
+  return launch_combine<float, kDim, kRows>(a, grid * C::kWarps, s);
 }
 
 }  // namespace
 
 uint64_t few32_tree_words(uint32_t head_dim, uint32_t tile_rows) {
-  return tree_words((uint64_t)tree_ctas(1) * kWarps, tile_rows, head_dim);
+  const uint32_t warps = head_dim == 64 && tile_rows == 8 ? Few32<64, 8>::kWarps : Few32<64, 16>::kWarps;
+  return tree_words((uint64_t)tree_ctas(1) * warps, tile_rows, head_dim);
 }
 
 uint32_t few32_tree(const AttnArgs& a, uint32_t head_dim, uint32_t tile_rows, cudaStream_t s) {
