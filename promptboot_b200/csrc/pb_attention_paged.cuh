@@ -288,8 +288,10 @@ __global__ void __launch_bounds__(kCombine) combine_kernel(const __grid_constant
 // The trees' second launch, which may begin while the first ends.
 template <class T, int kDim, int kRows>
 uint32_t launch_combine(const AttnArgs& a, uint32_t runs, cudaStream_t s) {
-  constexpr int kStep = kCombine / (kDim / 4);
-  const dim3 join(runs, kRows > 32 ? kRows / kStep : 1);
+  constexpr uint32_t kStep = kCombine / (kDim / 4);
+  // CTAs for the rows that a sequence has on average; those of longer ones take turns.
+  const uint32_t mean = (uint32_t)(((uint64_t)a.q_rows * a.group + a.seqs - 1) / a.seqs);
+  const dim3 join(runs, kRows > 32 ? std::max(1u, std::min<uint32_t>(kRows, mean) / kStep) : 1);
   PB_CUDA(launch_pdl(combine_kernel<T, kDim, kRows>, join, kCombine, 0, s, a));
   return PB_OK;
 }

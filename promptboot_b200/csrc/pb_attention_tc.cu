@@ -22,8 +22,8 @@
 // row tile where the exponentials (16 a cycle and SM) need 512: measured with two, three
 // and four softmax warps per scheduler, the schedulers issue 0.55 instructions a cycle
 // and no more, since the packed products and the maxima share register ports (a pair of
-// them takes 3.25 cycles, each alone 2).  One prompt of 16384 (14 heads of 64): 0.63 ms
-// alone, 770 TFLOP/s; a packed prompt of 4096 at 32 heads of 128: 714 TFLOP/s.  Three
+// them takes 3.25 cycles, each alone 2).  One prompt of 16384 (14 heads of 64): 0.62 ms
+// alone, 775 TFLOP/s; a packed prompt of 4096 at 32 heads of 128: 714 TFLOP/s.  Three
 // row tiles a CTA that share the key tiles gained 5% there and lost as much on ragged
 // batches; four CTAs an SM with one score buffer each, and weights formed with the
 // maximum of the tile before, measured the same or worse.
