@@ -222,8 +222,9 @@ attention_few_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__
         }
       if (masked) {
         // The tile's value rows: zero past the keys, and without what is not finite.
-        mend |= __any_sync(0xffffffffu, lane < kKeys && clean_value_row<F, kDim, C::kBlock>(
-                                            tile_keys + C::kTile, lane, key0 + lane >= s.len));
+        mend |= __any_sync(0xffffffffu, clean_value_row<F, kDim, C::kBlock, 32 / kKeys>(
+                                            tile_keys + C::kTile, lane % kKeys, lane / kKeys,
+                                            key0 + lane % kKeys >= s.len));
       }
 #pragma unroll
       for (int j = 0; j < kKeys / 16; ++j) {

@@ -23,7 +23,7 @@
 // and four softmax warps per scheduler, the schedulers issue 0.55 instructions a cycle
 // and no more, since the packed products and the maxima share register ports (a pair of
 // them takes 3.25 cycles, each alone 2).  One prompt of 16384 (14 heads of 64): 0.62 ms
-// alone, 775 TFLOP/s; a packed prompt of 4096 at 32 heads of 128: 714 TFLOP/s.  Three
+// alone, 778 TFLOP/s; one of 4096 at 32 heads of 128: 131 us, 1045 TFLOP/s.  Three
 // row tiles a CTA that share the key tiles gained 5% there and lost as much on ragged
 // batches; four CTAs an SM with one score buffer each, and weights formed with the
 // maximum of the tile before, measured the same or worse.
@@ -513,11 +513,13 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         if (masked) weigh(std::false_type{});
         else weigh(std::true_type{});
         if (masked) {
-          // Value rows of this tile, one per thread: zero past the keys, and without
+          // Value rows of this tile, half a row per thread: zero past the keys, and without
           // what is not finite.
           if (!wait_soon(&v_full[q % kStages], (q / kStages) & 1, abort_flag)) { stop = true; break; }
-          if (tid < kKeys &&
-              clean_value_row<F, kDim, C::kBlock>(smem + C::kVOff + (q % kStages) * C::kTile, tid, key0 + tid >= s.len))
+          static_assert(2 * kKeys == kRows, "two threads to a value row");
+          const int key = tid % kKeys;
+          if (clean_value_row<F, kDim, C::kBlock, 2>(smem + C::kVOff + (q % kStages) * C::kTile, key, tid / kKeys,
+                                                     key0 + key >= s.len))
             *dirty = pieces;
           fence_async_smem();
         }

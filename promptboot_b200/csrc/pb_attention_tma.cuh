@@ -92,27 +92,42 @@ __device__ __forceinline__ float max_nan(float a, float b, float c) {
   return y;
 }
 
-// Value row `key` of a tile in shared memory (column blocks of 128 bytes, kBlock
-// apart, 128-byte swizzle): zeroed where it is past the keys; else what is not finite
-// is zeroed.  Whether there was any.
-template <class F, int kDim, int kBlock>
-__device__ __forceinline__ bool clean_value_row(uint8_t* tile, int key, bool past) {
-  bool found = false;
-#pragma unroll 4
-  for (int c = 0; c < kDim / 8; ++c) {
-    uint4* word = reinterpret_cast<uint4*>(tile + c / 8 * kBlock + key * 128 + ((c % 8) ^ (key & 7)) * 16);
-    uint4 x = past ? make_uint4(0, 0, 0, 0) : *word;
-    uint32_t* u = reinterpret_cast<uint32_t*>(&x);
-    bool write = past;
+// Part `part` of kParts of value row `key` of a tile in shared memory (column blocks of
+// 128 bytes, kBlock apart, 128-byte swizzle): zeroed where it is past the keys; else
+// what is not finite is zeroed.  Whether there was any.
+template <class F, int kDim, int kBlock, int kParts>
+__device__ __forceinline__ bool clean_value_row(uint8_t* tile, int key, int part, bool past) {
+  constexpr int kWords = kDim / 8 / kParts;
+  constexpr uint32_t kLowest = (F::kExponents & (0u - F::kExponents)) * 0x10001u;
+  auto word = [&](int i) {
+    const int c = part * kWords + i;
+    return reinterpret_cast<uint4*>(tile + c / 8 * kBlock + key * 128 + ((c % 8) ^ (key & 7)) * 16);
+  };
+  uint32_t full = 0;  // all exponent bits set: one more carries into the sign's place
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t e = u[i] & F::kExponents;
-      if ((e & 0xffffu) == (F::kExponents & 0xffffu)) { u[i] &= 0xffff0000u; found = write = true; }
-      if ((e >> 16) == (F::kExponents >> 16)) { u[i] &= 0xffffu; found = write = true; }
+  for (int i = 0; i < kWords; ++i) {
+    if (past) {
+      *word(i) = make_uint4(0, 0, 0, 0);
+    } else {
+      const uint4 x = *word(i);
+      full |= ((x.x & F::kExponents) + kLowest) | ((x.y & F::kExponents) + kLowest) |
+              ((x.z & F::kExponents) + kLowest) | ((x.w & F::kExponents) + kLowest);
     }
-    if (write) *word = x;
   }
-  return found;
+  if (!(full & 0x80008000u)) return false;
+#pragma unroll 1
+  for (int i = 0; i < kWords; ++i) {
+    uint4 x = *word(i);
+    uint32_t* u = reinterpret_cast<uint32_t*>(&x);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t e = u[k] & F::kExponents;
+      if ((e & 0xffffu) == (F::kExponents & 0xffffu)) u[k] &= 0xffff0000u;
+      if ((e >> 16) == (F::kExponents >> 16)) u[k] &= 0xffffu;
+    }
+    *word(i) = x;
+  }
+  return true;
 }
 
 struct Maps {
