@@ -9,7 +9,9 @@
 // step of the type per weight and averages out over the keys.
 //
 // Warps: 0..3 softmax, one row per thread (TMEM lane = row); 4 issues the MMAs;
-// 5 brings K and V tiles by TMA (128-byte swizzle) into rings of kStages.  S has two
+// 5 brings K and V tiles by TMA (128-byte swizzle) into rings of kStages, and Q, as soon
+// as its place is free, so that a unit's first scores are formed under the weights and
+// the way out of the one before (24 ragged prompts: 163 -> 144 us).  S has two
 // buffers in TMEM, P takes the place of the upper half of the scores it comes from: the
 // scores of tile j + 2 go out when the products of tile j are done, a tile ahead of
 // their softmax, which therefore seldom waits.  256 TMEM columns, so two CTAs share an
@@ -22,8 +24,8 @@
 // row tile where the exponentials (16 a cycle and SM) need 512: measured with two, three
 // and four softmax warps per scheduler, the schedulers issue 0.55 instructions a cycle
 // and no more, since the packed products and the maxima share register ports (a pair of
-// them takes 3.25 cycles, each alone 2).  One prompt of 16384 (14 heads of 64): 0.62 ms
-// alone, 778 TFLOP/s; one of 4096 at 32 heads of 128: 131 us, 1045 TFLOP/s.  Three
+// them takes 3.25 cycles, each alone 2).  One prompt of 16384 (14 heads of 64): 0.61 ms
+// alone, 783 TFLOP/s; one of 4096 at 32 heads of 128: 127 us, 1080 TFLOP/s.  Three
 // row tiles a CTA that share the key tiles gained 5% there and lost as much on ragged
 // batches; four CTAs an SM with one score buffer each, and weights formed with the
 // maximum of the tile before, measured the same or worse.
@@ -225,7 +227,9 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   uint64_t* unit_empty = unit_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(unit_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* dirty = abort_flag + 1;  // the last piece with a value that was taken out
+  // The last even and odd piece with a value that was taken out: a warp may be in a piece
+  // while another ends the one before.
+  volatile int* dirty = abort_flag + 1;
   uint32_t* prefix = reinterpret_cast<uint32_t*>(smem + C::kPrefixOff);
 
   if (kTree) pdl_trigger();
@@ -255,7 +259,7 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       mbar_init(&v_full[i], 1);
       mbar_init(&v_empty[i], 1);
     }
-    mbar_init(q_full, kRows);
+    mbar_init(q_full, 32);
     mbar_init(&s_full[0], 1);
     mbar_init(&s_full[1], 1);
     mbar_init(&p_full[0], kRows);
@@ -267,7 +271,7 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       mbar_init(&unit_empty[i], kThreads / 32);
     }
     *abort_flag = 0;
-    *dirty = 0;
+    dirty[0] = dirty[1] = 0;
     fence_barrier_init();
   }
   tc_before_sync();
@@ -305,6 +309,26 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     int q = 0;  // tiles so far
     bool stop = false;
     int asked = 0;
+    const uint32_t inverse = 0xffffffffu / a.group + 1;  // x / group of x below 2048
+    // Sends for a piece's rows of Q, eight lanes to 128 bytes of a row.
+    auto bring_q = [&](const Piece& p) {
+      const uint32_t first = p.row_tile * kRows, token0 = first / a.group, rest = first % a.group;
+      const T* from = static_cast<const T*>(a.q.data) + (uint64_t)(s.q0 + token0) * a.q.row_stride +
+                      (uint64_t)(p.head * a.group) * a.q.head_stride + lane % 8 * 8;
+      const uint32_t to = smem_u32(smem);
+#pragma unroll 4
+      for (uint32_t r = lane / 8; r < kRows; r += 4) {
+        const uint32_t x = rest + r, t = a.group == 1 ? x : __umulhi(x, inverse), h = x - t * a.group;
+        const bool there = first + r < rows;  // else zeros
+        const T* row = from + (uint64_t)t * a.q.row_stride + (uint64_t)h * a.q.head_stride;
+#pragma unroll
+        for (int c = 0; c < kHalves; ++c)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                           to + c * C::kQBlock + r * 128 + ((lane % 8) ^ (r % 8)) * 16),
+                       "l"(there ? static_cast<const void*>(row + c * 64) : a.q.data), "r"(there ? 16 : 0)
+                       : "memory");
+      }
+    };
     for (; have && !stop; have = further()) {
       Piece p;
       take(p);
@@ -321,6 +345,10 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                    ? (int)a.tables[(uint64_t)p.seq * a.table_width + key / a.cache.page_size] : 0;
       };
       int page = page_of(p.tile0);
+      if (p.tile0 < p.tile1) {  // Q takes its place after the last scores of the piece before
+        if (q > 0 && !wait_soon(&k_empty[(q - 1) % kStages], ((q - 1) / kStages) & 1, abort_flag)) break;
+        bring_q(p);
+      }
       for (uint32_t tile = p.tile0; tile < p.tile1; ++tile, ++q) {
         const int st = q % kStages, ahead = page_of(tile + 1);
         const uint32_t key = tile * kKeys, count = boxes(tile);
@@ -341,6 +369,11 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         if (!wait_soon(&k_empty[st], ((q / kStages) & 1) ^ 1, abort_flag)) { stop = true; break; }
         bring(ka + st * C::kTile, &maps.k, maps.k_step, &k_full[st]);
         k_brought = q + 1;
+        if (tile == p.tile0) {
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          fence_async_smem();
+          mbar_arrive(q_full);
+        }
         if (!wait_soon(&v_empty[st], ((q / kStages) & 1) ^ 1, abort_flag)) { stop = true; break; }
         bring(va + st * C::kTile, &maps.v, maps.v_step, &v_full[st]);
         v_brought = q + 1;
@@ -349,6 +382,7 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     }
     if (kTree && lane == 0)  // under the last tiles of the others
       note_join<kRows, kKeys>(a, prefix, Share<kLeast>(total, gridDim.x), blockIdx.x);
+    asm volatile("cp.async.wait_all;" ::: "memory");
     if (*abort_flag) {  // every copy and answer lands before the CTA may exit
       if (asked) wait_drain(&unit_full[(asked - 1) & 1], ((asked - 1) >> 1) & 1, 50000000ull);
       for (int i = max(0, k_brought - kStages); i < k_brought; ++i)
@@ -426,18 +460,6 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       uint64_t l2[2] = {0, 0};      // the sum of weights, in four parts
       // Tiles from here on hold a key that some row does not see.
       const uint32_t mask0 = (kTree ? s.context : row_view<false>(a, s, p.row_tile * kRows / a.group).all) / kKeys;
-      if (p.tile0 < p.tile1) {
-        const T* src = static_cast<const T*>(a.q.data) + (uint64_t)(s.q0 + token) * a.q.row_stride +
-                       (uint64_t)head * a.q.head_stride;
-#pragma unroll
-        for (int c = 0; c < kDim / 8; ++c) {
-          const uint4 w = there ? reinterpret_cast<const uint4*>(src)[c] : make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4*>(smem + c / 8 * C::kQBlock + tid * 128 + ((c % 8) ^ (tid & 7)) * 16) = w;
-        }
-        fence_async_smem();
-        tc_before_sync();  // the piece before has been read from TMEM
-        mbar_arrive(q_full);
-      }
       for (uint32_t tile = p.tile0; tile < p.tile1; ++tile, ++q) {
         const uint32_t key0 = tile * kKeys;
         const bool masked = tile >= mask0;
@@ -520,7 +542,7 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
           const int key = tid % kKeys;
           if (clean_value_row<F, kDim, C::kBlock, 2>(smem + C::kVOff + (q % kStages) * C::kTile, key, tid / kKeys,
                                                      key0 + key >= s.len))
-            *dirty = pieces;
+            dirty[pieces & 1] = pieces;
           fence_async_smem();
         }
         tmem_wait_st();
@@ -543,7 +565,7 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       T* out = static_cast<T*>(a.out.data) + (uint64_t)(s.q0 + token) * a.out.row_stride +
                (uint64_t)head * a.out.head_stride;
       float* rec = kTree && p.partial >= 0 ? a.partial + (size_t)p.partial * partial_words<kRows, kDim>() : nullptr;
-      const bool mend = *dirty == pieces;
+      const bool mend = dirty[pieces & 1] == pieces;
 #pragma unroll
       for (int c = 0; c < kDim; c += 32) {
         uint32_t v[32];

@@ -285,6 +285,31 @@ def test_prompt_attention_infinite_value_reaches_its_component():
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 14, 2), (128, 32, 8)])
+def test_prompt_attention_of_many_short_prompts_with_infinite_values(dtype, dim, heads, kv_heads):
+    """More units than the GPU holds, half of them with a value that is not finite: it
+    reaches its component in the rows that see it and changes no other bit, whatever the
+    units before and after are doing."""
+    g, rng = gen(25), np.random.default_rng(25)
+    lengths = [int(n) for n in rng.integers(1, 120, 200)]
+    first = np.concatenate([[0], np.cumsum(lengths)])
+    n = int(first[-1])
+    q, k, v = (normal(g, n, h, dim, dtype=dtype) for h in (heads, kv_heads, kv_heads))
+    want = ops.prompt_attention(q, k, v, starts(lengths))
+    check_heads(want[:lengths[0]], q[:lengths[0]], k[:lengths[0]], v[:lengths[0]], causal(lengths[0], lengths[0]),
+                dim ** -0.5, dtype)
+    hit = torch.zeros_like(want, dtype=torch.bool)
+    for s in range(0, 200, 2):
+        at, c = int(first[s]) + int(rng.integers(lengths[s])), s % dim
+        v[at, :, c] = math.inf
+        hit[at:int(first[s + 1]), :, c] = True
+    for _ in range(10):
+        got = ops.prompt_attention(q, k, v, starts(lengths))
+        assert torch.equal(got.isinf(), hit)
+        assert torch.equal(got[~hit], want[~hit])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_prompt_attention_of_stacked_views_and_a_given_scale(dtype):
     g = gen(10)
     stacked = normal(g, 300, 18, 64, dtype=dtype)
