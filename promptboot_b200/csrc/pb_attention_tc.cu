@@ -25,7 +25,7 @@
 // and four softmax warps per scheduler, the schedulers issue 0.55 instructions a cycle
 // and no more, since the packed products and the maxima share register ports (a pair of
 // them takes 3.25 cycles, each alone 2).  One prompt of 16384 (14 heads of 64): 0.61 ms
-// alone, 783 TFLOP/s; one of 4096 at 32 heads of 128: 127 us, 1080 TFLOP/s.  Three
+// alone, 784 TFLOP/s; one of 4096 at 32 heads of 128: 125 us, 1100 TFLOP/s.  Three
 // row tiles a CTA that share the key tiles gained 5% there and lost as much on ragged
 // batches; four CTAs an SM with one score buffer each, and weights formed with the
 // maximum of the tile before, measured the same or worse.
@@ -204,6 +204,24 @@ __device__ __forceinline__ uint32_t seen32(const RowView& r, uint32_t key) {
     m |= (uint32_t)(r.bits << below);
   }
   return m;
+}
+
+// Turns the four words of each of four neighbouring lanes: lane j's w[i] becomes lane
+// i's w[j].
+__device__ __forceinline__ void across_quads(uint4 (&w)[4], int lane) {
+  auto swap = [&](uint4& low, uint4& high, int with) {
+    const bool up = lane & with;
+    uint4 x = up ? low : high;
+    x.x = __shfl_xor_sync(0xffffffffu, x.x, with);
+    x.y = __shfl_xor_sync(0xffffffffu, x.y, with);
+    x.z = __shfl_xor_sync(0xffffffffu, x.z, with);
+    x.w = __shfl_xor_sync(0xffffffffu, x.w, with);
+    (up ? low : high) = x;
+  };
+  swap(w[0], w[1], 1);
+  swap(w[2], w[3], 1);
+  swap(w[0], w[2], 2);
+  swap(w[1], w[3], 2);
 }
 
 template <class T, int kDim, bool kTree>
@@ -565,6 +583,10 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       T* out = static_cast<T*>(a.out.data) + (uint64_t)(s.q0 + token) * a.out.row_stride +
                (uint64_t)head * a.out.head_stride;
       float* rec = kTree && p.partial >= 0 ? a.partial + (size_t)p.partial * partial_words<kRows, kDim>() : nullptr;
+      T* quad[4];  // the rows of four neighbouring threads, whose stores then fill 64 bytes of a row
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        quad[i] = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, (unsigned long long)out, (lane & ~3) + i));
       const bool mend = dirty[pieces & 1] == pieces;
 #pragma unroll
       for (int c = 0; c < kDim; c += 32) {
@@ -576,8 +598,7 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = 0;
         }
-        if (!there) continue;
-        if (mend) {
+        if (mend && there) {
           // A weight is positive: what is not finite passes through the sum as it is.
           for (uint32_t key = max(p.tile0, mask0) * kKeys; key < min(p.tile1 * kKeys, s.len); ++key) {
             if (!view.sees(key)) continue;
@@ -599,17 +620,24 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
           }
         }
         if (rec) {
+          if (there) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<uint4*>(rec + tid * kDim + c + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<uint4*>(rec + tid * kDim + c + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+          }
         } else {
+          uint4 w[4];
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) {
+          for (int i = 0; i < 4; ++i) {
             float y[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) y[u] = __fmul_rn(__uint_as_float(v[i + u]), inv);
-            *reinterpret_cast<uint4*>(out + c + i) = Elements<T>::store(y);
+            for (int u = 0; u < 8; ++u) y[u] = __fmul_rn(__uint_as_float(v[8 * i + u]), inv);
+            w[i] = Elements<T>::store(y);
           }
+          across_quads(w, lane);  // word `lane % 4` of the quad's four rows
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (row - lane % 4 + i < rows) *reinterpret_cast<uint4*>(quad[i] + c + lane % 4 * 8) = w[i];
         }
       }
       if (there && rec) {
