@@ -7,11 +7,11 @@
 // and out = o / l.
 //
 // The keys of the next tile are on their way while the weights are found and the values
-// added, its values while its scores are.  Bound by the multiply-adds and the reads of
-// shared memory that feed them (12 of 16 bytes to 128 multiply-adds of a thread): a
-// prompt of 2500 tokens, 14 heads of 64 to 2, takes 457 us, 25 TFLOP/s; trees of 8 nodes
-// over 8 x 22000 positions 213 us, 18 TFLOP/s (four CTAs an SM in the grid where three
-// or two fit: 258).
+// added, its values while its scores are.  Bound by the latency of a warp's chain and
+// the reads of shared memory that feed its multiply-adds.  Row tiles of 32, four CTAs an
+// SM: a prompt of 2500 tokens, 14 heads of 64 to 2, takes 370 us, 30 TFLOP/s (tiles of 64:
+// 394, of 16: 492); 8 of 2500 in all 112 (139, 126); trees of 8 nodes over 32 x 3000
+// positions, 32 heads of 128 to 8, 438 us, 23 TFLOP/s (886 with tiles of 64, half empty).
 #include "pb_attention_launch.h"
 
 namespace pb {
@@ -29,7 +29,7 @@ struct Simt {
   static constexpr int kKpt = kKeys / 16;
   static constexpr int kPad = kDim + 4;   // row pitch: 16-byte reads of 8 rows hit all banks once
   static constexpr int kPadP = kKeys + 4;
-  static constexpr int kCtas = kDim == 64 ? 3 : 2;  // per SM, by shared memory for row tiles of 64
+  static constexpr int kCtas = 4;        // per SM, by shared memory for row tiles of 32
   static constexpr int kWords = kRows * kPad + 2 * kKeys * kPad + kRows * kPadP;
   static size_t bytes(uint32_t seqs) { return (size_t)(kWords + seqs) * 4; }
 };
@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(kThreads, kTree ? Simt<kDim, kRpt>::kCtas : 1)
     uint32_t all_see = 0xffffffffu;  // keys that every row of this thread sees
 #pragma unroll
     for (int i = 0; i < kRpt; ++i) {
-      const uint32_t row = p.row_tile * kRows + ty * kRpt + i;
+      const uint32_t row = p.row_tile * kRows + ty + 8 * i;
       view[i] = row < rows ? row_view<kTree>(a, s, row / a.group) : RowView{0xffffffffu, 0ull};
       all_see = min(all_see, view[i].all);
     }
@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(kThreads, kTree ? Simt<kDim, kRpt>::kCtas : 1)
           kf[j] = *reinterpret_cast<const float4*>(ks + (tx + 16 * j) * C::kPad + c);
 #pragma unroll
         for (int i = 0; i < kRpt; ++i) {
-          const float4 qf = *reinterpret_cast<const float4*>(qs + (ty * kRpt + i) * C::kPad + c);
+          const float4 qf = *reinterpret_cast<const float4*>(qs + (ty + 8 * i) * C::kPad + c);
 #pragma unroll
           for (int j = 0; j < kKpt; ++j) {
             sc[i][j] = __fmaf_rn(qf.x, kf[j].x, sc[i][j]);
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(kThreads, kTree ? Simt<kDim, kRpt>::kCtas : 1)
           const bool seen = !masked || view[i].sees(key0 + tx + 16 * j);
           const float w = seen ? exp2f(__fsub_rn(sc[i][j], base)) : -0.f;
           l[i] += seen ? w : 0.f;
-          ps[(ty * kRpt + i) * C::kPadP + tx + 16 * j] = w;
+          ps[(ty + 8 * i) * C::kPadP + tx + 16 * j] = w;
         }
       }
       copies_wait();    // the values
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kThreads, kTree ? Simt<kDim, kRpt>::kCtas : 1)
               vf[u][c] = *reinterpret_cast<const float4*>(vs + (j + u) * C::kPad + c * 64 + tx * 4);
 #pragma unroll
           for (int i = 0; i < kRpt; ++i) {
-            const float4 w4 = *reinterpret_cast<const float4*>(ps + (ty * kRpt + i) * C::kPadP + j);
+            const float4 w4 = *reinterpret_cast<const float4*>(ps + (ty + 8 * i) * C::kPadP + j);
             const float w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, kTree ? Simt<kDim, kRpt>::kCtas : 1)
     for (int i = 0; i < kRpt; ++i) {
 #pragma unroll
       for (int d = 8; d; d >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], d);
-      const uint32_t r = ty * kRpt + i, row = p.row_tile * kRows + r;
+      const uint32_t r = ty + 8 * i, row = p.row_tile * kRows + r;
       if (row >= rows) continue;
       if (p.partial >= 0) {
         float* rec = a.partial + (size_t)p.partial * partial_words<kRows, kDim>();
@@ -284,13 +284,14 @@ uint32_t launch(AttnArgs a, uint32_t grid, cudaStream_t s) {
   return kTree ? launch_combine<float, kDim, C::kRows>(a, grid, s) : PB_OK;
 }
 
-constexpr int kFewRpt = 2, kManyRpt = 8;  // 16 or 64 rows of a tile
+constexpr int kTreeCtas = Simt<64, 4>::kCtas;
+constexpr int kFewRpt = 2, kManyRpt = 4;  // 16 or 32 rows of a tile
 
 }  // namespace
 
 uint32_t simt_prompt(const AttnArgs& a, uint32_t head_dim, cudaStream_t s) {
   const uint32_t rows = a.q_rows * a.group;
-  // Row tiles of 16 where tiles of 64 would leave SMs without work.
+  // Row tiles of 16 where there are no more than some two tiles of 32 to an SM.
   const bool small = (uint64_t)rows * a.kv_heads < 64ull * tree_ctas(1);
   const uint32_t grid = (rows / (small ? 8 * kFewRpt : 8 * kManyRpt) + a.seqs) * a.kv_heads;
   if (small)
@@ -298,14 +299,10 @@ uint32_t simt_prompt(const AttnArgs& a, uint32_t head_dim, cudaStream_t s) {
   return head_dim == 64 ? launch<64, kManyRpt, false>(a, grid, s) : launch<128, kManyRpt, false>(a, grid, s);
 }
 
-static uint32_t tree_grid(uint32_t head_dim) {
-  return tree_ctas(head_dim == 64 ? Simt<64, kManyRpt>::kCtas : Simt<128, kManyRpt>::kCtas);
-}
-
-uint64_t simt_tree_words(uint32_t head_dim) { return tree_words(tree_grid(head_dim), 8 * kManyRpt, head_dim); }
+uint64_t simt_tree_words(uint32_t head_dim) { return tree_words(tree_ctas(kTreeCtas), 8 * kManyRpt, head_dim); }
 
 uint32_t simt_tree(const AttnArgs& a, uint32_t head_dim, cudaStream_t s) {
-  const uint32_t grid = tree_grid(head_dim);
+  const uint32_t grid = tree_ctas(kTreeCtas);
   return head_dim == 64 ? launch<64, kManyRpt, true>(a, grid, s) : launch<128, kManyRpt, true>(a, grid, s);
 }
 
