@@ -711,6 +711,32 @@ def test_operators_on_a_side_stream_and_in_graphs():
         assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_calls_on_two_streams_at_once_give_the_bits_of_calls_in_turn(dtype):
+    g, rng = gen(26), np.random.default_rng(26)
+    jobs = []
+    for nodes, seqs, dim in ((1, 40, 64), (20, 6, 128)):
+        contexts = [int(c) for c in rng.integers(100, 3000, seqs)]
+        cache, tables, _, _ = paged(g, rng, [c + nodes for c in contexts], 32, 2, dim, dtype)
+        q = normal(g, seqs * nodes, 8, dim, dtype=dtype)
+        visible = [b for _ in range(seqs) for b in random_tree(rng, nodes)]
+        jobs.append(lambda q=q, cache=cache, args=(tables, i32(contexts), starts([nodes] * seqs), masks(visible)):
+                    ops.tree_attention(q, cache, *args, layer=1))
+    lengths = [int(n) for n in rng.integers(1, 200, 60)]
+    q, k, v = (normal(g, sum(lengths), h, 64, dtype=dtype) for h in (8, 2, 2))
+    jobs.append(lambda at=starts(lengths): ops.prompt_attention(q, k, v, at))
+    want = [job() for job in jobs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(60):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append((i % 3, jobs[i % 3]()))
+    torch.cuda.synchronize()
+    for j, y in got:
+        assert torch.equal(y, want[j])
+
+
 def test_first_calls_of_a_process_may_be_captured():
     """Nothing has to be set up before a capture."""
     import subprocess
