@@ -82,7 +82,7 @@ __device__ __forceinline__ RowView row_view(const AttnArgs& a, const Sequence& s
   return {seen > s.t ? seen - s.t : 0, 0ull};
 }
 
-__device__ __forceinline__ uint32_t ceil_div(uint32_t a, uint32_t b) { return (a + b - 1) / b; }
+__host__ __device__ __forceinline__ uint32_t ceil_div(uint32_t a, uint32_t b) { return (a + b - 1) / b; }
 
 // Segments (prompts) or key tiles (trees) of a sequence, per key head and in all.
 template <bool kTree, int kRows, int kKeys>
@@ -291,7 +291,7 @@ uint32_t launch_combine(const AttnArgs& a, uint32_t runs, cudaStream_t s) {
   constexpr uint32_t kStep = kCombine / (kDim / 4);
   // CTAs for the rows that a sequence has on average; those of longer ones take turns.
   const uint32_t mean = (uint32_t)(((uint64_t)a.q_rows * a.group + a.seqs - 1) / a.seqs);
-  const dim3 join(runs, kRows > 32 ? std::max(1u, std::min<uint32_t>(kRows, mean) / kStep) : 1);
+  const dim3 join(runs, std::max(1u, ceil_div(std::min<uint32_t>(kRows, mean), kStep)));
   PB_CUDA(launch_pdl(combine_kernel<T, kDim, kRows>, join, kCombine, 0, s, a));
   return PB_OK;
 }
