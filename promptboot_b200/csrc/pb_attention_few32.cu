@@ -137,7 +137,9 @@ attention_few32_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
         x[r] = __fmul_rn(x[r], a.scale_log2);
         if (masked) {
           const uint32_t row = first + r;
-          if (row < rows && !row_view<true>(a, s, row / a.group).sees(key0 + key)) {
+          // Rows past the last see nothing here: a slot without a key would else decide
+          // whether the maxima move, and with that how the other rows round.
+          if (row >= rows || !row_view<true>(a, s, row / a.group).sees(key0 + key)) {
             seen &= ~(1u << r);
             x[r] = -INFINITY;
           }

@@ -538,6 +538,24 @@ def test_tree_attention_of_growing_and_of_falling_scores(dtype, dim, heads, node
     check_tree(got, q, [n] * 3, [nodes] * 3, visible, keys, values, 0.7, dtype)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32])
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 14, 2), (64, 15, 1), (128, 6, 2), (128, 11, 1)])
+def test_tree_attention_of_few_rows_beside_slots_without_keys(dtype, dim, heads, kv_heads):
+    """Keys that end at every place of a tile: what the slots behind them hold changes no
+    bit."""
+    got = {}
+    for junk in (0.5, NAN, math.inf):
+        g, rng = gen(27), np.random.default_rng(27)
+        contexts = list(range(1, 68))
+        cache, tables, keys, values = paged(g, rng, [c + 1 for c in contexts], 16, kv_heads, dim, dtype, junk=junk)
+        q = normal(g, len(contexts), heads, dim, dtype=dtype, scale=2.0)
+        args = (q, cache, tables, i32(contexts), starts([1] * len(contexts)), masks([1] * len(contexts)))
+        got[junk] = ops.tree_attention(*args, layer=1)
+        assert all(torch.equal(got[junk], ops.tree_attention(*args, layer=1)) for _ in range(50))
+    check_tree(got[0.5], q, contexts, [1] * len(contexts), [1] * len(contexts), keys, values, dim ** -0.5, dtype)
+    assert torch.equal(got[0.5], got[NAN]) and torch.equal(got[0.5], got[math.inf])
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("seqs,nodes", [(1, 1), (2, 48), (300, 1), (40, 3)])
 def test_tree_attention_of_long_and_of_many_contexts(dtype, seqs, nodes):
