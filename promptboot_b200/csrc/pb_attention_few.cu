@@ -225,6 +225,7 @@ attention_few_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__
         mend |= __any_sync(0xffffffffu, clean_value_row<F, kDim, C::kBlock, 32 / kKeys>(
                                             tile_keys + C::kTile, lane % kKeys, lane / kKeys,
                                             key0 + lane % kKeys >= s.len));
+        __syncwarp();  // cleaned rows before other lanes read them (a vote orders no memory)
       }
 #pragma unroll
       for (int j = 0; j < kKeys / 16; ++j) {

@@ -538,11 +538,12 @@ def test_tree_attention_of_growing_and_of_falling_scores(dtype, dim, heads, node
     check_tree(got, q, [n] * 3, [nodes] * 3, visible, keys, values, 0.7, dtype)
 
 
-@pytest.mark.parametrize("dtype", [torch.float32])
-@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 14, 2), (64, 15, 1), (128, 6, 2), (128, 11, 1)])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 14, 2), (64, 15, 1), (64, 24, 1), (128, 6, 2), (128, 11, 1)])
 def test_tree_attention_of_few_rows_beside_slots_without_keys(dtype, dim, heads, kv_heads):
     """Keys that end at every place of a tile: what the slots behind them hold changes no
-    bit."""
+    bit, however often a tile's value rows are cleaned in shared memory by the lanes that
+    have them and read by others."""
     got = {}
     for junk in (0.5, NAN, math.inf):
         g, rng = gen(27), np.random.default_rng(27)
