@@ -62,7 +62,7 @@ struct Tc {
   static constexpr int kVOff = kKOff + kStages * kTile;
   static constexpr int kBarOff = kVOff + kStages * kTile;
   static constexpr int kBars = 4 * kStages + 11;
-  static constexpr int kPrefixOff = kBarOff + kBars * 8 + 16;
+  static constexpr int kPrefixOff = kBarOff + kBars * 8 + 24;
   static constexpr int kOCol = 2 * kKeys;             // S and P: [0, 64) and [64, 128)
   static constexpr int kCols = 256;
   static_assert(kOCol + kDim <= kCols, "TMEM columns");
@@ -245,8 +245,9 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   uint64_t* unit_empty = unit_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(unit_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  // The last even and odd piece with a value that was taken out: a warp may be in a piece
-  // while another ends the one before.
+  // Of four pieces in turn, the last with a value that was taken out: a warp may be in a
+  // piece while another ends the one before, or, where that one had no tiles and so made
+  // no warp wait for another, the one before that.
   volatile int* dirty = abort_flag + 1;
   uint32_t* prefix = reinterpret_cast<uint32_t*>(smem + C::kPrefixOff);
 
@@ -289,7 +290,7 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       mbar_init(&unit_empty[i], kThreads / 32);
     }
     *abort_flag = 0;
-    dirty[0] = dirty[1] = 0;
+    for (int i = 0; i < 4; ++i) dirty[i] = 0;
     fence_barrier_init();
   }
   tc_before_sync();
@@ -560,7 +561,7 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
           const int key = tid % kKeys;
           if (clean_value_row<F, kDim, C::kBlock, 2>(smem + C::kVOff + (q % kStages) * C::kTile, key, tid / kKeys,
                                                      key0 + key >= s.len))
-            dirty[pieces & 1] = pieces;
+            dirty[pieces & 3] = pieces;
           fence_async_smem();
         }
         tmem_wait_st();
@@ -587,7 +588,7 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         quad[i] = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, (unsigned long long)out, (lane & ~3) + i));
-      const bool mend = dirty[pieces & 1] == pieces;
+      const bool mend = dirty[pieces & 3] == pieces;
 #pragma unroll
       for (int c = 0; c < kDim; c += 32) {
         uint32_t v[32];

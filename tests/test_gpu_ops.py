@@ -310,6 +310,33 @@ def test_prompt_attention_of_many_short_prompts_with_infinite_values(dtype, dim,
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_prompt_attention_of_prompts_without_keys_between_infinite_values(dtype, dim):
+    """A unit without key tiles makes no warp wait for another: what the unit before it
+    has still to write does not mix with the unit after it."""
+    g, rng = gen(28), np.random.default_rng(28)
+    tokens = [int(t) if s % 2 else 4 for s, t in enumerate(rng.integers(1, 33, 2000))]
+    keys = [t if s % 2 else 0 for s, t in enumerate(tokens)]
+    first, key = np.concatenate([[0], np.cumsum(tokens)]), np.concatenate([[0], np.cumsum(keys)])
+    q = normal(g, sum(tokens), 4, dim, dtype=dtype)
+    k, v = (normal(g, sum(keys), 1, dim, dtype=dtype) for _ in range(2))
+    at = starts(tokens), starts(keys)
+    want = ops.prompt_attention(q, k, v, *at)
+    hit, none = torch.zeros_like(want, dtype=torch.bool), torch.zeros(sum(tokens), dtype=torch.bool, device="cuda")
+    for s, t in enumerate(tokens):
+        if keys[s]:
+            i, c = int(rng.integers(t)), s % dim
+            v[int(key[s]) + i, 0, c] = math.inf
+            hit[int(first[s]) + i:int(first[s + 1]), :, c] = True
+        else:
+            none[int(first[s]):int(first[s + 1])] = True
+    for _ in range(20):
+        got = ops.prompt_attention(q, k, v, *at)
+        assert torch.equal(got.isinf(), hit) and torch.equal(got[~hit], want[~hit])
+        assert not got[none].any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_prompt_attention_of_stacked_views_and_a_given_scale(dtype):
     g = gen(10)
     stacked = normal(g, 300, 18, 64, dtype=dtype)
