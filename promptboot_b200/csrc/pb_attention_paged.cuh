@@ -82,6 +82,13 @@ __device__ __forceinline__ RowView row_view(const AttnArgs& a, const Sequence& s
   return {seen > s.t ? seen - s.t : 0, 0ull};
 }
 
+// The largest; not a number where one is not.
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
 __host__ __device__ __forceinline__ uint32_t ceil_div(uint32_t a, uint32_t b) { return (a + b - 1) / b; }
 
 // Segments (prompts) or key tiles (trees) of a sequence, per key head and in all.
@@ -270,7 +277,9 @@ __global__ void __launch_bounds__(kCombine) combine_kernel(const __grid_constant
       o.z = __fmul_rn(o.z, old); o.w = __fmul_rn(o.w, old);
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
-        if (mp[i] == -INFINITY) continue;  // no run, or one of which the row saw nothing
+        // no run, or one of which the row saw nothing (a score that is not a number makes
+        // the run's maximum one that is not)
+        if (mp[i] == -INFINITY) continue;
         const float w = exp2f(mp[i] - m);
         o.x = __fmaf_rn(w, op[i].x, o.x); o.y = __fmaf_rn(w, op[i].y, o.y);
         o.z = __fmaf_rn(w, op[i].z, o.z); o.w = __fmaf_rn(w, op[i].w, o.w);

@@ -183,11 +183,12 @@ __global__ void __launch_bounds__(kThreads, kTree ? Simt<kDim, kRpt>::kCtas : 1)
         for (int j = 0; j < kKpt; ++j) {
           const bool seen = !masked || view[i].sees(key0 + tx + 16 * j);
           sc[i][j] = seen ? __fmul_rn(sc[i][j], a.scale_log2) : -INFINITY;
-          top = fmaxf(top, sc[i][j]);
+          top = max_nan(top, sc[i][j], -INFINITY);
         }
 #pragma unroll
-        for (int d = 8; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        const float to = fmaxf(m[i], top);
+        for (int d = 8; d; d >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d), -INFINITY);
+        // Not a number where a score is not: then so are the row and what a join takes of it.
+        const float to = max_nan(m[i], top, -INFINITY);
         const float base = to == -INFINITY ? 0.f : to;
         const float keep = exp2f(m[i] - base);  // 0 from -inf
         m[i] = to;

@@ -85,13 +85,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// The largest; not a number where one is not.
-__device__ __forceinline__ float max_nan(float a, float b, float c) {
-  float y;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-  return y;
-}
-
 // Part `part` of kParts of value row `key` of a tile in shared memory (column blocks of
 // 128 bytes, kBlock apart, 128-byte swizzle): zeroed where it is past the keys; else
 // what is not finite is zeroed.  Whether there was any.

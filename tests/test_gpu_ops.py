@@ -529,6 +529,29 @@ def test_tree_attention_keeps_out_what_a_node_does_not_see(dtype, nodes):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,nodes,context", [(64, 1, 900), (64, 12, 200), (64, 48, 3000), (128, 12, 700)])
+def test_tree_attention_of_what_is_not_a_number_over_split_contexts(dtype, dim, nodes, context):
+    """A NaN in a query makes its row NaN and no other, NaN keys all rows that see them,
+    where whole runs of a split context have no score that is a number."""
+    g, rng = gen(29), np.random.default_rng(29)
+    cache, tables, keys, values = paged(g, rng, [context + nodes], 16, 2, dim, dtype)
+    q = normal(g, nodes, 8, dim, dtype=dtype)
+    visible = random_tree(rng, nodes)
+    args = (tables, i32([context]), starts([nodes]), masks(visible))
+    want = ops.tree_attention(q, cache, *args, layer=1)
+    bad = q.clone()
+    bad[nodes // 2, 3, 5] = NAN
+    got = ops.tree_attention(bad, cache, *args, layer=1)
+    assert got[nodes // 2, 3].isnan().all()
+    got[nodes // 2, 3] = want[nodes // 2, 3]
+    check_tree(got, q, [context], [nodes], visible, keys, values, dim ** -0.5, dtype)
+    at = torch.arange(64, 64 + context // 2, device="cuda")
+    cache.k[1][tables[0, at // 16].long(), 1, at % 16] = NAN
+    got = ops.tree_attention(q, cache, *args, layer=1)
+    assert torch.equal(got[:, :4], want[:, :4]) and got[:, 4:].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_tree_attention_tables_that_end_and_pages_outside_the_cache(dtype):
     """Positions past the table are not seen; a page id outside the cache is zeros."""
     g, rng = gen(22), np.random.default_rng(22)
