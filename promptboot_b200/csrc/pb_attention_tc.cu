@@ -579,7 +579,8 @@ attention_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       float part[4];
       unpk(l2[0], part[0], part[1]);
       unpk(l2[1], part[2], part[3]);
-      const float l = (part[0] + part[1]) + (part[2] + part[3]);
+      // No weight where every score is -inf: the polynomial gives those 2^-126 instead of none.
+      const float l = m == -INFINITY ? 0.f : (part[0] + part[1]) + (part[2] + part[3]);
       const float inv = l == 0.f ? 0.f : __frcp_rn(l);
       T* out = static_cast<T*>(a.out.data) + (uint64_t)(s.q0 + token) * a.out.row_stride +
                (uint64_t)head * a.out.head_stride;

@@ -417,6 +417,25 @@ def test_prompt_attention_large_scores_and_growing_maxima():
         check_heads(got, q, k * 0, v, causal(n, n), 0.125, dtype)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_of_scores_that_are_all_minus_infinity_is_zero(dtype, dim):
+    """As of a row that sees nothing, over tiles that every row sees whole too."""
+    g, rng = gen(32), np.random.default_rng(32)
+    q, k, v = (normal(g, 300, h, dim, dtype=dtype) for h in (4, 2, 2))
+    q[..., 0], k[:, 1, 0] = 1.0, -math.inf
+    got = ops.prompt_attention(q, k, v, starts([300]))
+    assert not got[:, 2:].any() and got[:, :2].any(-1).all()
+    for nodes in (1, 20, 60):
+        cache, tables, _, _ = paged(g, rng, [400 + nodes], 16, 2, dim, dtype)
+        cache.k[1][:, 1, :, 0] = -math.inf
+        q = normal(g, nodes, 4, dim, dtype=dtype)
+        q[..., 0] = 1.0
+        got = ops.tree_attention(q, cache, tables, i32([400]), starts([nodes]),
+                                 masks([1 << i for i in range(nodes)]), layer=1)
+        assert not got[:, 2:].any() and got[:, :2].any(-1).all()
+
+
 def masks(values):
     return torch.from_numpy(np.array(values, dtype=np.uint64).view(np.int64)).cuda()
 
