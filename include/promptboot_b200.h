@@ -301,7 +301,7 @@ PB_API uint32_t pb_expf_device(const uint32_t *x_device, uint64_t n, uint32_t *y
  * that point outside the buffers described here are ignored as each entry says,
  * never followed.  Operands may not overlap the outputs unless said so. */
 enum { PB_TYPE_F32 = 0, PB_TYPE_F16 = 1, PB_TYPE_BF16 = 2 };
-/* A position, slot or page id that stands for none. */
+/* A position, slot, page id or count of kept nodes that stands for none. */
 #define PB_NONE 0xffffffffu
 /* Sequences of one attention call. */
 #define PB_MAX_SEQS 2048u
@@ -420,7 +420,7 @@ PB_API uint32_t pb_cache_copy_pages_device(const pb_cache *cache, uint32_t n,
                                            const uint32_t *pairs_device, void *stream);
 /* Keeps the accepted nodes of drafted trees: for every layer, position contexts
  * [s] + nodes[s * nodes_width + i] moves to contexts[s] + i, for i < counts[s]
- * (cut at nodes_width).  nodes ascend within a sequence; an entry below its own
+ * (cut at nodes_width; PB_NONE: none).  nodes ascend within a sequence; an entry below its own
  * index, not above all those before it, or past the table, and a page id outside
  * the cache, is left out.  The pages that are written belong to one sequence each. */
 PB_API uint32_t pb_cache_keep_device(const pb_cache *cache, uint32_t seqs,

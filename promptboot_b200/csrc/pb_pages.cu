@@ -84,6 +84,7 @@ __global__ void __launch_bounds__(128) keep_kernel(const __grid_constant__ KeepA
     const int64_t n = i < a.nodes_width ? (int64_t)nodes[i] : -1;
     const uint64_t context = a.contexts[seq];
     count = a.counts[seq];
+    if (count == PB_NONE) count = 0;
     // the largest node before this one, over the warp and then the block
     int64_t before = n;
 #pragma unroll

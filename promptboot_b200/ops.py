@@ -5,7 +5,8 @@ page operations, and the host's book of pages.
 Each call checks its tensors, passes their addresses to the C ABI
 (include/promptboot_b200.h has the definitions) on the tensors' device and its
 current torch stream, and returns at once.  Index tensors are contiguous int32
-(or uint32), -1 standing for none; head tensors are [rows, heads, head_dim] of
+(or uint32); -1 stands for no position, slot, page or kept node, and is not an offset
+or a context length.  Head tensors are [rows, heads, head_dim] of
 float32, float16 or bfloat16 with a contiguous last dimension, any other strides a
 multiple of 16 bytes, so that views of a stacked q/k/v projection serve as they
 are.  Refused arguments raise OperatorError.  There are no gradients: a tensor that
@@ -130,7 +131,9 @@ class PageCache:
     def keep(self, tables, contexts, counts, nodes):
         """Moves the accepted nodes of each sequence's draft tree behind its
         context, in every layer: position contexts[s] + nodes[s, i] to contexts[s]
-        + i for i < counts[s].  tables [seqs, width] as in tree_attention."""
+        + i for i < counts[s] (-1: none).  The nodes ascend; an entry that does not is
+        left out.  tables [seqs, width] as in tree_attention; pages that are written
+        must belong to one sequence each."""
         device, seqs = self.device, contexts.shape[0]
         width, most = tables.shape[-1], nodes.shape[-1]
         a = _index(tables, (seqs, width), device, "tables")

@@ -750,6 +750,18 @@ def test_keep_of_long_rows_with_entries_that_stand_for_none():
     assert torch.equal(cache.k, want) and torch.equal(cache.v, want + 1)
 
 
+def test_keep_of_no_nodes_and_of_a_count_that_stands_for_none():
+    g = gen(33)
+    cache = ops.PageCache.empty(2, 12, 1, 16, 64, torch.float32)
+    cache.k.copy_(normal(g, *cache.k.shape))
+    cache.v.copy_(cache.k + 1)
+    want = cache.k.clone()
+    tables = torch.arange(12, dtype=torch.int32, device="cuda").view(3, 4)
+    cache.keep(tables, i32([5, 5, 5]), i32([-1, 0, 1]), i32([[2, 4], [3, 6], [3, 6]]))
+    want[:, 8, :, 5] = want[:, 8, :, 8]
+    assert torch.equal(cache.k, want) and torch.equal(cache.v, want + 1)
+
+
 # ------------------------------------------------------------- streams and graphs
 
 def test_operators_on_a_side_stream_and_in_graphs():
