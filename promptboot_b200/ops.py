@@ -10,7 +10,7 @@ or a context length.  Head tensors are [rows, heads, head_dim] of
 float32, float16 or bfloat16 with a contiguous last dimension, any other strides a
 multiple of 16 bytes, so that views of a stacked q/k/v projection serve as they
 are.  Refused arguments raise OperatorError.  There are no gradients: a tensor that
-asks for one is refused unless grad mode is off.
+asks for one, one of a cache too, is refused unless grad mode is off.
 """
 from __future__ import annotations
 
@@ -82,6 +82,12 @@ def _heads(t, dtype, device, name):
     return _Rows(t.data_ptr(), s[0], s[1])
 
 
+def _no_gradient(cache):
+    """Refuses a cache whose tensors ask for a gradient (they may since it was made)."""
+    if (cache.k.requires_grad or cache.v.requires_grad) and torch.is_grad_enabled():
+        raise OperatorError("the cache asks for a gradient, which the serving operators do not have")
+
+
 def _first(t, name):
     """(type, device) of the tensor that sets them for the others."""
     dtype, device = t.dtype, t.get_device()
@@ -124,6 +130,7 @@ class PageCache:
 
     def copy_pages(self, pairs):
         """Copies page pairs[i, 0] to page pairs[i, 1] in every layer."""
+        _no_gradient(self)
         n = pairs.shape[0]
         at = _index(pairs, (n, 2), self.device, "pairs")
         _call(self.device, _lib.load().pb_cache_copy_pages_device, _ref(self._c), n, at)
@@ -134,6 +141,7 @@ class PageCache:
         + i for i < counts[s] (-1: none).  The nodes ascend; an entry that does not is
         left out.  tables [seqs, width] as in tree_attention; pages that are written
         must belong to one sequence each."""
+        _no_gradient(self)
         device, seqs = self.device, contexts.shape[0]
         width, most = tables.shape[-1], nodes.shape[-1]
         a = _index(tables, (seqs, width), device, "tables")
@@ -188,6 +196,7 @@ class Rotary:
     def apply_to_cache(self, q, k, v, positions, cache, slots, layer=0, q_out=None):
         """q turned, as apply; k turned and v go to `layer` of the cache at
         slots[row] = page * page_size + slot in the page (-1: nowhere)."""
+        _no_gradient(cache)
         dtype, device = cache.dtype, cache.device
         q_in, k_in, v_in = (_heads(q, dtype, device, "q"), _heads(k, dtype, device, "k"),
                             _heads(v, dtype, device, "v"))
@@ -253,6 +262,7 @@ def tree_attention(q, cache, tables, contexts, offsets, visible, layer=0, scale=
     tables[s, p // page_size].  One node with visible 1 is plain decode.
     `workspace`: a uint8 tensor of tree_workspace_bytes, for calls that never
     overlap; by default one from torch's allocator."""
+    _no_gradient(cache)
     dtype, device = cache.dtype, cache.device
     q_in = _heads(q, dtype, device, "q")
     rows, heads, dim = q.shape

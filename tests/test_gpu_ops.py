@@ -1006,3 +1006,25 @@ def test_tensors_that_ask_for_gradients_are_refused_and_the_status_is_clean():
         assert not ops.prompt_attention(q, k, k, i32([0, 4])).any()
     ops.attention_status()
     ops.attention_status("cuda:0")
+
+
+def test_caches_that_ask_for_gradients_are_refused_by_every_call():
+    cache = ops.PageCache.empty(1, 4, 1, 16, 64, torch.float32)
+    cache.k.zero_()
+    cache.v.zero_()
+    q, k = torch.zeros(1, 2, 64, device="cuda"), torch.zeros(1, 1, 64, device="cuda")
+    one, plan = i32([1]), ops.Rotary(64)
+    calls = [lambda: ops.tree_attention(q, cache, i32([[0, 1]]), i32([9]), i32([0, 1]), masks([1])),
+             lambda: plan.apply_to_cache(q, k, k, one, cache, one),
+             lambda: cache.copy_pages(i32([[0, 1]])),
+             lambda: cache.keep(i32([[0, 1]]), i32([9]), one, i32([[1]]))]
+    for side in (cache.k, cache.v):
+        side.requires_grad_()
+        for call in calls:
+            with pytest.raises(ops.OperatorError, match="the cache asks for a gradient"):
+                call()
+            with torch.no_grad():
+                call()
+        side.requires_grad_(False)
+    for call in calls:
+        call()

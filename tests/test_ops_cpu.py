@@ -161,6 +161,16 @@ def test_wrappers_refuse_tensors_off_the_gpu():
         ops.Rotary(64, scaling="ntk")
 
 
+def test_a_cache_that_asks_for_gradients_is_refused_before_its_call():
+    cache = ops.PageCache.__new__(ops.PageCache)  # its calls look at the tensors before anything else
+    cache.k, cache.v = torch.zeros(1, 2, 1, 16, 64), torch.zeros(1, 2, 1, 16, 64, requires_grad=True)
+    for call in (lambda: cache.copy_pages(None), lambda: cache.keep(None, None, None, None),
+                 lambda: ops.tree_attention(None, cache, None, None, None, None),
+                 lambda: ops.Rotary(64).apply_to_cache(None, None, None, None, cache, None)):
+        with pytest.raises(ops.OperatorError, match="the cache asks for a gradient"):
+            call()
+
+
 # ---------------------------------------------------------------- the book of pages
 
 def test_pool_shares_pages_until_one_sequence_writes():
