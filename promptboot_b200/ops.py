@@ -10,7 +10,8 @@ or a context length.  Head tensors are [rows, heads, head_dim] of
 float32, float16 or bfloat16 with a contiguous last dimension, any other strides a
 multiple of 16 bytes, so that views of a stacked q/k/v projection serve as they
 are.  Refused arguments raise OperatorError.  There are no gradients: a tensor that
-asks for one, one of a cache too, is refused unless grad mode is off.
+asks for one, one of a cache too, is refused unless grad mode is off, and one that
+carries a forward-mode tangent always.
 """
 from __future__ import annotations
 
@@ -18,6 +19,7 @@ import ctypes
 import functools
 
 import torch
+import torch.autograd.forward_ad as _forward
 
 from . import _lib
 from .api import DeviceError
@@ -77,14 +79,21 @@ def _heads(t, dtype, device, name):
         raise OperatorError(f"{name} must be [rows, heads, head_dim] with a contiguous last dimension")
     if t.dtype is not dtype or t.get_device() != device:
         raise OperatorError(f"{name} has another type or device")
-    if t.requires_grad and torch.is_grad_enabled():
+    if t.requires_grad and torch.is_grad_enabled() or _forward._current_level >= 0 and _tangent(t):
         raise OperatorError(f"{name} asks for a gradient, which the serving operators do not have")
     return _Rows(t.data_ptr(), s[0], s[1])
 
 
+def _tangent(t):
+    """Whether t carries a tangent of the forward mode.  Callers look first whether a
+    level of it is open (_current_level), without which there are none."""
+    return _forward.unpack_dual(t).tangent is not None
+
+
 def _no_gradient(cache):
     """Refuses a cache whose tensors ask for a gradient (they may since it was made)."""
-    if (cache.k.requires_grad or cache.v.requires_grad) and torch.is_grad_enabled():
+    if (cache.k.requires_grad or cache.v.requires_grad) and torch.is_grad_enabled() \
+            or _forward._current_level >= 0 and (_tangent(cache.k) or _tangent(cache.v)):
         raise OperatorError("the cache asks for a gradient, which the serving operators do not have")
 
 

@@ -171,6 +171,30 @@ def test_a_cache_that_asks_for_gradients_is_refused_before_its_call():
             call()
 
 
+def test_tensors_with_a_tangent_are_refused():
+    import torch.autograd.forward_ad as forward
+    x = torch.zeros(4, 2, 64)
+    cache = ops.PageCache.__new__(ops.PageCache)
+    cache.k, cache.v = torch.zeros(1, 2, 1, 16, 64), torch.zeros(1, 2, 1, 16, 64)
+    with forward.dual_level():
+        dual = forward.make_dual(x, x + 1)
+        with torch.no_grad(), pytest.raises(ops.OperatorError, match="q asks for a gradient"):
+            ops._heads(dual, torch.float32, -1, "q")
+        ops._heads(x, torch.float32, -1, "q")
+        ops._no_gradient(cache)
+        cache.v = forward.make_dual(cache.v, cache.k)
+        with pytest.raises(ops.OperatorError, match="the cache asks for a gradient"):
+            ops._no_gradient(cache)
+
+    def use(t):
+        ops._heads(t, torch.float32, -1, "k")
+        return t
+    with pytest.raises(ops.OperatorError, match="k asks for a gradient"):
+        torch.func.jvp(use, (x,), (x,))
+    with pytest.raises(ops.OperatorError, match="k asks for a gradient"):
+        torch.func.grad(lambda t: use(t).sum())(x)
+
+
 # ---------------------------------------------------------------- the book of pages
 
 def test_pool_shares_pages_until_one_sequence_writes():
