@@ -31,6 +31,9 @@ _SCALINGS = {"none": 0, "linear": 1, "bands": 2, "yarn": 3}
 _ref = ctypes.byref
 _Rows = _lib.PbRows
 _empty_like = torch.empty_like
+# Tells autograd of tensors that a kernel has written: a backward pass that saved one
+# then raises an error instead of reading what is no longer there.
+_written = torch.autograd.graph.increment_version
 
 
 class OperatorError(ValueError):
@@ -143,6 +146,7 @@ class PageCache:
         n = pairs.shape[0]
         at = _index(pairs, (n, 2), self.device, "pairs")
         _call(self.device, _lib.load().pb_cache_copy_pages_device, _ref(self._c), n, at)
+        _written((self.k, self.v))
 
     def keep(self, tables, contexts, counts, nodes):
         """Moves the accepted nodes of each sequence's draft tree behind its
@@ -158,6 +162,7 @@ class PageCache:
         c = _index(counts, (seqs,), device, "counts")
         d = _index(nodes, (seqs, most), device, "nodes")
         _call(device, _lib.load().pb_cache_keep_device, _ref(self._c), seqs, a, width, b, c, d, most)
+        _written((self.k, self.v))
 
 
 class Rotary:
@@ -200,6 +205,7 @@ class Rotary:
         if rows:
             _call(device, _lib.load().pb_rotary_device, self._h, _TYPES[dtype], rows, at, heads, _ref(q_in), _ref(q_to),
                   k_heads, _ref(k_in), _ref(k_to))
+            _written((q_out, k_out))
         return q_out, k_out
 
     def apply_to_cache(self, q, k, v, positions, cache, slots, layer=0, q_out=None):
@@ -223,6 +229,7 @@ class Rotary:
         if rows:
             _call(device, _lib.load().pb_rotary_cache_device, self._h, rows, a, heads, _ref(q_in), _ref(q_to),
                   _ref(k_in), _ref(v_in), _ref(cache._c), layer, b)
+            _written((q_out, cache.k, cache.v))
         return q_out
 
 
@@ -246,6 +253,7 @@ def prompt_attention(q, k, v, offsets, kv_offsets=None, scale=None, out=None):
         raise OperatorError("out must have the shape of q")
     _call(device, _lib.load().pb_prompt_attention_device, _TYPES[dtype], dim, heads, k_heads, n - 1, rows, k_rows,
           _ref(q_in), _ref(k_in), _ref(v_in), _ref(to), a, b, dim ** -0.5 if scale is None else scale)
+    _written(out)
     return out
 
 
@@ -295,6 +303,7 @@ def tree_attention(q, cache, tables, contexts, offsets, visible, layer=0, scale=
         raise OperatorError("workspace must be a contiguous uint8 tensor on q's device")
     _call(device, _lib.load().pb_tree_attention_device, _ref(cache._c), layer, heads, seqs, rows, _ref(q_in),
           _ref(to), a, width, b, c, d, dim ** -0.5 if scale is None else scale, workspace.data_ptr(), workspace.numel())
+    _written(out)
     return out
 
 

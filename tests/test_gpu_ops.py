@@ -1028,3 +1028,37 @@ def test_caches_that_ask_for_gradients_are_refused_by_every_call():
         side.requires_grad_(False)
     for call in calls:
         call()
+
+
+def test_a_backward_pass_learns_that_a_tensor_it_saved_was_written():
+    g = gen(60)
+    q, k, one = normal(g, 1, 2, 64), normal(g, 1, 2, 64), i32([1])
+    cache = ops.PageCache(normal(g, 1, 4, 2, 16, 64), normal(g, 1, 4, 2, 16, 64))
+    plan, tree = ops.Rotary(64), (i32([[0, 1]]), i32([9]), i32([0, 1]), masks([1]))
+    calls = [(q, lambda: plan.apply(q, k, one, q_out=q)), (k, lambda: plan.apply(q, k, one, k_out=k)),
+             (q, lambda: plan.apply_to_cache(q, k, k, one, cache, one, q_out=q)),
+             (cache.k, lambda: plan.apply_to_cache(q, k, k, one, cache, one)),
+             (cache.v, lambda: plan.apply_to_cache(q, k, k, one, cache, one)),
+             (cache.k, lambda: cache.copy_pages(i32([[0, 1]]))), (cache.v, lambda: cache.copy_pages(i32([[0, 1]]))),
+             (cache.k, lambda: cache.keep(tree[0], tree[1], one, i32([[1]]))),
+             (cache.v, lambda: cache.keep(tree[0], tree[1], one, i32([[1]]))),
+             (q, lambda: ops.prompt_attention(k, k, k, i32([0, 1]), out=q)),
+             (q, lambda: ops.tree_attention(k, cache, *tree, out=q))]
+    for saved, call in calls:
+        w = torch.ones(64, device="cuda", requires_grad=True)
+        y = (saved * w).sum()
+        y.backward(retain_graph=True)
+        call()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    # what is only read keeps its version, and tensors of the inference mode have none
+    before = [t._version for t in (q, k, cache.k, cache.v)]
+    ops.prompt_attention(q, k, k, i32([0, 1]))
+    ops.tree_attention(q, cache, *tree)
+    plan.apply(q, k, one)
+    assert before == [t._version for t in (q, k, cache.k, cache.v)]
+    with torch.inference_mode():
+        q, k = normal(g, 1, 2, 64), normal(g, 1, 2, 64)
+        cache = ops.PageCache.empty(1, 4, 2, 16, 64, torch.float32)
+        assert plan.apply_to_cache(q, k, k, one, cache, one, q_out=q) is q
+        cache.copy_pages(i32([[0, 1]]))
