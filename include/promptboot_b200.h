@@ -292,11 +292,12 @@ PB_API uint32_t pb_expf_device(const uint32_t *x_device, uint64_t n, uint32_t *y
  * fp32_sse2.rs:1413-1672, inference.rs:2035-2052).
  *
  * All are asynchronous on `stream`, whose device must be the current one and
- * hold every pointer; none allocates device memory, waits or keeps state, so
- * they may be captured into a graph and called from any thread.  Arguments that
- * the host can see are checked first: PB_CAPACITY (a size, count or type that is
- * not supported), PB_ALIGNMENT (a pointer or stride), each with its text in
- * pb_last_error_string, and nothing is launched.  What device arrays hold
+ * hold every pointer; none allocates device memory, waits or keeps state (but the
+ * count of failures behind pb_attention_status), so they may be captured into a
+ * graph and called from any thread.  Arguments that the host can see are checked
+ * first: PB_CAPACITY (a size, count or type that is not supported), PB_ALIGNMENT
+ * (a pointer or stride), each with its text in pb_last_error_string, and nothing
+ * is launched.  What device arrays hold
  * (positions, offsets, page ids, slots, counts) cannot be checked there: values
  * that point outside the buffers described here are ignored as each entry says,
  * never followed.  Operands may not overlap the outputs unless said so. */
@@ -408,9 +409,10 @@ PB_API uint32_t pb_tree_attention_device(const pb_cache *cache, uint32_t layer, 
                                          const uint64_t *visible_device, float scale,
                                          void *workspace, uint64_t workspace_bytes, void *stream);
 
-/* Waits for `stream` and reports a prompt or tree attention whose kernel gave up
- * waiting for a copy or a product (PB_DEVICE, once; its outputs are not complete).
- * Not to be called while a graph is captured. */
+/* Waits for `stream` and reports whether any prompt or tree attention on the current
+ * device, on this stream or another, gave up waiting for a copy or a product since the
+ * calling host thread last asked (PB_DEVICE, once to each thread; the outputs of that
+ * attention are not complete).  Not to be called while a graph is captured. */
 PB_API uint32_t pb_attention_status(void *stream);
 
 /* Copies page pairs[2 i] to page pairs[2 i + 1] for i < n, keys and values of

@@ -2,6 +2,7 @@
 // kernel.
 #include "pb_attention_launch.h"
 #include "pb_common.cuh"
+#include "pb_told.h"
 
 #include <cmath>
 
@@ -156,9 +157,17 @@ uint32_t pb_tree_attention_device(const pb_cache* cache, uint32_t layer, uint32_
 }
 
 uint32_t pb_attention_status(void* stream) {
-  PB_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
-  const uint32_t a = pb::paged::tc_status(), b = pb::paged::few_status(), c = pb::paged::few32_status();
-  return a ? a : b ? b : c;
+  static thread_local pb::Told told;
+  const cudaStream_t s = (cudaStream_t)stream;
+  uint32_t st, count = 0;
+  if ((st = pb::paged::tc_timeouts(s, &count))) return st;
+  if ((st = pb::paged::few_timeouts(s, &count))) return st;
+  if ((st = pb::paged::few32_timeouts(s, &count))) return st;
+  int device = 0;
+  PB_CUDA(cudaGetDevice(&device));
+  if (!told.news(device, count)) return PB_OK;
+  pb::set_last_error("an attention pipeline timed out waiting for a copy or a product");
+  return PB_DEVICE;
 }
 
 }  // extern "C"

@@ -336,7 +336,7 @@ uint64_t few_tree_words(uint32_t head_dim, uint32_t tiles) {
   return tree_words((uint64_t)tree_ctas(ctas) * kWarps, 16 * tiles, head_dim);
 }
 
-uint32_t few_status() { return take_status(); }
+uint32_t few_timeouts(cudaStream_t s, uint32_t* count) { return add_timeouts(s, count); }
 
 uint32_t few_tree(const AttnArgs& a, uint32_t type, uint32_t head_dim, uint32_t tiles, cudaStream_t s) {
   return type == PB_TYPE_F16 ? by_size<__half>(a, head_dim, tiles, s)

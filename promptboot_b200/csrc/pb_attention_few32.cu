@@ -278,7 +278,7 @@ uint32_t few32_tree(const AttnArgs& a, uint32_t head_dim, uint32_t tile_rows, cu
   return tile_rows == 8 ? launch<128, 8>(a, s) : launch<128, 16>(a, s);
 }
 
-uint32_t few32_status() { return take_status(); }
+uint32_t few32_timeouts(cudaStream_t s, uint32_t* count) { return add_timeouts(s, count); }
 
 }  // namespace paged
 }  // namespace pb

@@ -697,7 +697,7 @@ uint32_t tc_tree(const AttnArgs& a, uint32_t type, uint32_t head_dim, cudaStream
   return head_dim == 64 ? launch<__nv_bfloat16, 64, true>(a, grid, s) : launch<__nv_bfloat16, 128, true>(a, grid, s);
 }
 
-uint32_t tc_status() { return take_status(); }
+uint32_t tc_timeouts(cudaStream_t s, uint32_t* count) { return add_timeouts(s, count); }
 
 }  // namespace paged
 }  // namespace pb

@@ -200,18 +200,17 @@ struct TileRing {
   }
 };
 
-// Set where a bounded wait of a kernel gave up (one word per source file).
-static __device__ unsigned int g_timeout;
-__device__ __forceinline__ void mark_timeout() { atomicOr(&g_timeout, 1u); }
-// Reads and clears it; PB_DEVICE with its text where it was set.
-static inline uint32_t take_status() {
-  unsigned int st = 0;
-  PB_CUDA(cudaMemcpyFromSymbol(&st, g_timeout, 4));
-  if (!st) return PB_OK;
-  const unsigned int zero = 0;
-  PB_CUDA(cudaMemcpyToSymbol(g_timeout, &zero, 4));
-  set_last_error("an attention pipeline timed out waiting for a copy or a product");
-  return PB_DEVICE;
+// CTAs in which a bounded wait gave up (one count per source file and device).  Never
+// cleared, so that whoever asks takes nothing from others who have still to ask.
+static __device__ unsigned int g_timeouts;
+__device__ __forceinline__ void mark_timeout() { atomicAdd(&g_timeouts, 1u); }
+// Adds it to *count, once `s` is done with what it has.
+static inline uint32_t add_timeouts(cudaStream_t s, uint32_t* count) {
+  unsigned int n = 0;
+  PB_CUDA(cudaMemcpyFromSymbolAsync(&n, g_timeouts, 4, 0, cudaMemcpyDeviceToHost, s));
+  PB_CUDA(cudaStreamSynchronize(s));
+  *count += n;
+  return PB_OK;
 }
 
 // --------------------------------------------------------------- tensor maps (host)

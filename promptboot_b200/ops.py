@@ -308,8 +308,9 @@ def tree_attention(q, cache, tables, contexts, offsets, visible, layer=0, scale=
 
 
 def attention_status(device=None):
-    """Waits for the device's current stream and raises DeviceError where an attention
-    on that device gave up waiting since the last call (its outputs are not complete)."""
+    """Waits for the device's current stream and raises DeviceError where an attention on
+    that device, on any stream, gave up waiting since this thread last asked (the outputs
+    of that attention are not complete)."""
     device = torch.cuda.current_device() if device is None else torch.device(device).index or 0
     _call(device, _lib.load().pb_attention_status)
 

@@ -195,6 +195,28 @@ def test_tensors_with_a_tangent_are_refused():
         torch.func.grad(lambda t: use(t).sum())(x)
 
 
+def test_every_thread_is_told_of_each_failure_once(tmp_path):
+    """What pb_attention_status says of a device's count, by host thread."""
+    import pathlib
+    import subprocess
+    import threading
+    csrc = pathlib.Path(_lib.__file__).parent / "csrc"
+    source, built = tmp_path / "told.cpp", tmp_path / "told.so"
+    source.write_text('#include "pb_told.h"\nextern "C" int news(int device, unsigned count) '
+                      '{ static thread_local pb::Told told; return told.news(device, count); }\n')
+    subprocess.run(["g++", "-std=c++17", "-shared", "-fPIC", "-I", str(csrc), str(source), "-o", str(built)], check=True)
+    news = ctypes.CDLL(str(built)).news
+    assert [news(0, n) for n in (0, 0, 2, 2, 3, 3)] == [0, 0, 1, 0, 1, 0]
+    assert [news(1, n) for n in (0, 1, 1)] == [0, 1, 0] and news(0, 3) == 0  # by device
+    other = []
+    thread = threading.Thread(target=lambda: other.extend(news(0, 3) for _ in range(2)))
+    thread.start()
+    thread.join()
+    assert other == [1, 0]  # what one thread asked takes nothing from another
+    assert news(0, 3) == 0 and news(0, 4) == 1
+    assert [news(64, 0), news(64, 2), news(64, 2), news(-1, 0)] == [0, 1, 1, 0]
+
+
 # ---------------------------------------------------------------- the book of pages
 
 def test_pool_shares_pages_until_one_sequence_writes():
