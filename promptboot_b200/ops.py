@@ -311,8 +311,10 @@ def attention_status(device=None):
     """Waits for the device's current stream and raises DeviceError where an attention on
     that device, on any stream, gave up waiting since this thread last asked (the outputs
     of that attention are not complete)."""
-    device = torch.cuda.current_device() if device is None else torch.device(device).index or 0
-    _call(device, _lib.load().pb_attention_status)
+    device = torch.device("cuda" if device is None else device)
+    if device.type != "cuda":
+        raise OperatorError(f"attention_status: {device} is not a CUDA device")
+    _call(torch.cuda.current_device() if device.index is None else device.index, _lib.load().pb_attention_status)
 
 
 class PagePool:

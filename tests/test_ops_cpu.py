@@ -195,6 +195,17 @@ def test_tensors_with_a_tangent_are_refused():
         torch.func.grad(lambda t: use(t).sum())(x)
 
 
+def test_attention_status_asks_the_device_that_is_meant(monkeypatch):
+    asked = []
+    monkeypatch.setattr(ops, "_call", lambda device, fn: asked.append(device))
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 3)
+    for device in (None, "cuda", torch.device("cuda"), "cuda:0", torch.device("cuda", 2), 1):
+        ops.attention_status(device)
+    assert asked == [3, 3, 3, 0, 2, 1]
+    with pytest.raises(ops.OperatorError, match="CUDA"):
+        ops.attention_status("cpu")
+
+
 def test_every_thread_is_told_of_each_failure_once(tmp_path):
     """What pb_attention_status says of a device's count, by host thread."""
     import pathlib
