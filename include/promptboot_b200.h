@@ -377,7 +377,8 @@ PB_API uint32_t pb_rotary_cache_device(const pb_rotary *rotary, uint32_t rows,
  * sees the first n - t + i + 1 of n keys.  A row that sees none is zero; rows
  * behind q_offsets[seqs] stay as they were.  Offsets ascend; they are cut at
  * q_rows and kv_rows.  Keys that a row does not see have no part in it whatever
- * they hold.  head_dim 64 or 128, seqs up to PB_MAX_SEQS. */
+ * they hold.  head_dim 64 or 128, seqs up to PB_MAX_SEQS, scale positive and scale
+ * log2(e) finite. */
 PB_API uint32_t pb_prompt_attention_device(uint32_t type, uint32_t head_dim, uint32_t q_heads,
                                            uint32_t kv_heads, uint32_t seqs, uint32_t q_rows,
                                            uint32_t kv_rows, const pb_rows *q, const pb_rows *k,

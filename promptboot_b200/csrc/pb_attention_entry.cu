@@ -30,9 +30,11 @@ uint32_t check_heads(const char* who, uint32_t type, uint32_t head_dim, uint32_t
   return PB_OK;
 }
 
+constexpr float kLog2E = 1.4426950408889634f;
+
 uint32_t check_scale(const char* who, float scale) {
-  if (!(scale > 0.f) || !std::isfinite(scale))
-    return refuse(PB_CAPACITY, who, "scale must be positive and finite");
+  if (!(scale > 0.f) || !std::isfinite(scale * kLog2E))
+    return refuse(PB_CAPACITY, who, "scale must be positive and scale * log2(e) finite");
   return PB_OK;
 }
 
@@ -50,8 +52,6 @@ uint32_t few32_rows(uint64_t rows, uint32_t seqs) {
   if (rows <= 8ull * seqs) return 8;
   return rows <= 16ull * seqs ? 16 : 0;
 }
-
-constexpr float kLog2E = 1.4426950408889634f;
 
 }  // namespace
 }  // namespace paged

@@ -128,6 +128,19 @@ def test_prompt_attention_refusals():
     assert prompt(n=0) == 0
 
 
+def test_attention_scales_whose_power_of_two_is_not_finite_are_refused():
+    """Weights are powers of two: scale log2(e) has to be finite too."""
+    lib, r = _lib.load(), rows()
+    for scale in (2.4e38, 3e38):
+        refused(lib.pb_prompt_attention_device(2, 64, 4, 2, 1, 8, 8, ref(r), ref(r), ref(r), ref(r), FAKE, FAKE, scale,
+                                               None), CAPACITY, "scale")
+        refused(lib.pb_tree_attention_device(ref(cache()), 0, 4, 1, 8, ref(r), ref(r), FAKE, 4, FAKE, FAKE, FAKE, scale,
+                                             FAKE, 1 << 40, None), CAPACITY, "scale")
+    # the next check speaks where the scale will do
+    refused(lib.pb_prompt_attention_device(2, 64, 4, 2, 1, 8, 1 << 30, ref(r), ref(r), ref(r), ref(r), FAKE, FAKE,
+                                           2.3e38, None), CAPACITY, "kv_rows")
+
+
 def test_tree_attention_refusals():
     lib = _lib.load()
 
