@@ -44,6 +44,13 @@ class OperatorError(ValueError):
         super().__init__(text)
 
 
+def _u32(x, name):
+    """x as the C ABI takes it, which would cut a larger number to 32 bits."""
+    if not 0 <= x < 1 << 32:
+        raise OperatorError(f"{name} is out of range")
+    return x
+
+
 def _check(status: int):
     if status == 0:
         return
@@ -174,8 +181,9 @@ class Rotary:
                  original_context=0, low=0.0, high=0.0, magnitude=0.0):
         if scaling not in _SCALINGS:
             raise OperatorError(f"scaling must be one of {', '.join(_SCALINGS)}")
-        config = _lib.PbRotaryConfig(head_dim, rotary_dim or head_dim, _LAYOUTS[bool(interleaved)],
-                                     _SCALINGS[scaling], theta, factor, original_context, low, high, magnitude)
+        rotary_dim = head_dim if rotary_dim is None else rotary_dim
+        config = _lib.PbRotaryConfig(_u32(head_dim, "head_dim"), _u32(rotary_dim, "rotary_dim"),
+                                     _LAYOUTS[bool(interleaved)], _SCALINGS[scaling], theta, factor, original_context, low, high, magnitude)
         self.head_dim = head_dim
         self._h = ctypes.c_void_p()
         _check(_lib.load().pb_rotary_create(_ref(config), _ref(self._h)))
@@ -228,7 +236,7 @@ class Rotary:
             raise OperatorError("q_out must have the shape of q")
         if rows:
             _call(device, _lib.load().pb_rotary_cache_device, self._h, rows, a, heads, _ref(q_in), _ref(q_to),
-                  _ref(k_in), _ref(v_in), _ref(cache._c), layer, b)
+                  _ref(k_in), _ref(v_in), _ref(cache._c), _u32(layer, "layer"), b)
             _written((q_out, cache.k, cache.v))
         return q_out
 
@@ -301,8 +309,8 @@ def tree_attention(q, cache, tables, contexts, offsets, visible, layer=0, scale=
         workspace = torch.empty(need, dtype=torch.uint8, device=cache.k.device)
     elif workspace.dtype is not torch.uint8 or workspace.get_device() != device or not workspace.is_contiguous():
         raise OperatorError("workspace must be a contiguous uint8 tensor on q's device")
-    _call(device, _lib.load().pb_tree_attention_device, _ref(cache._c), layer, heads, seqs, rows, _ref(q_in),
-          _ref(to), a, width, b, c, d, dim ** -0.5 if scale is None else scale, workspace.data_ptr(), workspace.numel())
+    _call(device, _lib.load().pb_tree_attention_device, _ref(cache._c), _u32(layer, "layer"), heads, seqs, rows,
+          _ref(q_in), _ref(to), a, width, b, c, d, dim ** -0.5 if scale is None else scale, workspace.data_ptr(), workspace.numel())
     _written(out)
     return out
 
@@ -323,7 +331,8 @@ class PagePool:
 
     def __init__(self, pages, page_size, max_seqs):
         self._h = ctypes.c_void_p()
-        _check(_lib.load().pb_pool_create(pages, page_size, max_seqs, _ref(self._h)))
+        _check(_lib.load().pb_pool_create(_u32(pages, "pages"), _u32(page_size, "page_size"),
+                                          _u32(max_seqs, "max_seqs"), _ref(self._h)))
         self.pages, self.page_size = pages, page_size
 
     def __del__(self):
@@ -343,22 +352,22 @@ class PagePool:
     def fork(self, seq):
         """A new sequence that shares every page of `seq`."""
         child = ctypes.c_uint32()
-        _check(_lib.load().pb_pool_fork(self._h, seq, _ref(child)))
+        _check(_lib.load().pb_pool_fork(self._h, _u32(seq, "seq"), _ref(child)))
         return child.value
 
     def extend(self, seq, tokens):
         """Room for `tokens` more; None, or the (from, to) pair of pages that
         PageCache.copy_pages has to copy before anything is written."""
         pair, needed = (ctypes.c_uint32 * 2)(), ctypes.c_uint32()
-        _check(_lib.load().pb_pool_extend(self._h, seq, tokens, pair, _ref(needed)))
+        _check(_lib.load().pb_pool_extend(self._h, _u32(seq, "seq"), _u32(tokens, "tokens"), pair, _ref(needed)))
         return None if pair[0] == 0xFFFFFFFF else (pair[0], pair[1])
 
     def truncate(self, seq, length):
         """Cuts a sequence to `length` tokens and frees the pages behind them."""
-        _check(_lib.load().pb_pool_truncate(self._h, seq, length))
+        _check(_lib.load().pb_pool_truncate(self._h, _u32(seq, "seq"), _u32(length, "length")))
 
     def free(self, seq):
-        _check(_lib.load().pb_pool_free(self._h, seq))
+        _check(_lib.load().pb_pool_free(self._h, _u32(seq, "seq")))
 
     def compact(self):
         """Moves the pages in use to the lowest ids: ([(from, to), ...] for
@@ -398,5 +407,5 @@ class PagePool:
         length, needed = ctypes.c_uint32(), ctypes.c_uint32()
         lib = _lib.load()
         table = (ctypes.c_uint32 * self.pages)()
-        _check(lib.pb_pool_table(self._h, seq, table, self.pages, _ref(length), _ref(needed)))
+        _check(lib.pb_pool_table(self._h, _u32(seq, "seq"), table, self.pages, _ref(length), _ref(needed)))
         return list(table[:needed.value]), length.value

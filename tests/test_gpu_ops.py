@@ -1062,3 +1062,13 @@ def test_a_backward_pass_learns_that_a_tensor_it_saved_was_written():
         cache = ops.PageCache.empty(1, 4, 2, 16, 64, torch.float32)
         assert plan.apply_to_cache(q, k, k, one, cache, one, q_out=q) is q
         cache.copy_pages(i32([[0, 1]]))
+
+
+def test_layers_past_32_bits_are_refused_not_cut():
+    q, k, one = torch.zeros(1, 2, 64, device="cuda"), torch.zeros(1, 1, 64, device="cuda"), i32([1])
+    cache = ops.PageCache.empty(1, 4, 1, 16, 64, torch.float32)
+    for layer in (1 << 32, -1):
+        with pytest.raises(ops.OperatorError, match="layer"):
+            ops.tree_attention(q, cache, i32([[0, 1]]), i32([9]), i32([0, 1]), masks([1]), layer=layer)
+        with pytest.raises(ops.OperatorError, match="layer"):
+            ops.Rotary(64).apply_to_cache(q, k, k, one, cache, one, layer=layer)

@@ -293,6 +293,22 @@ def test_pool_refusals_change_nothing():
             ops.PagePool(*bad)
 
 
+def test_numbers_past_32_bits_are_refused_not_cut():
+    pool, big = ops.PagePool(8, 16, 2), 1 << 32
+    a = pool.open()
+    pool.extend(a, 40)
+    for bad in (lambda: pool.extend(a, big + 5), lambda: pool.extend(a, -1), lambda: pool.truncate(a, big),
+                lambda: pool.truncate(a, big + 20), lambda: pool.fork(a + big), lambda: pool.free(a + big),
+                lambda: pool.pages_of(a + big), lambda: pool.length(a - big), lambda: ops.PagePool(big + 4, 16, 2),
+                lambda: ops.PagePool(4, big + 16, 2), lambda: ops.PagePool(4, 16, big + 2),
+                lambda: ops.Rotary(big + 64), lambda: ops.Rotary(64, big + 32), lambda: ops.Rotary(64, -big + 32)):
+        with pytest.raises(ops.OperatorError, match="out of range"):
+            bad()
+        assert pool.pages_of(a) == [0, 1, 2] and pool.length(a) == 40 and pool.free_pages() == 5
+    with pytest.raises(ops.OperatorError, match="rotary_dim"):
+        ops.Rotary(64, 0)  # no rotation is not the whole head
+
+
 def test_pool_short_arrays_are_refused_with_the_number_needed():
     lib, pool = _lib.load(), ops.PagePool(8, 16, 2)
     a, b = pool.open(), pool.open()
