@@ -183,7 +183,8 @@ class Rotary:
             raise OperatorError(f"scaling must be one of {', '.join(_SCALINGS)}")
         rotary_dim = head_dim if rotary_dim is None else rotary_dim
         config = _lib.PbRotaryConfig(_u32(head_dim, "head_dim"), _u32(rotary_dim, "rotary_dim"),
-                                     _LAYOUTS[bool(interleaved)], _SCALINGS[scaling], theta, factor, original_context, low, high, magnitude)
+                                     _LAYOUTS[bool(interleaved)], _SCALINGS[scaling], theta, factor,
+                                     original_context, low, high, magnitude)
         self.head_dim = head_dim
         self._h = ctypes.c_void_p()
         _check(_lib.load().pb_rotary_create(_ref(config), _ref(self._h)))
@@ -310,7 +311,8 @@ def tree_attention(q, cache, tables, contexts, offsets, visible, layer=0, scale=
     elif workspace.dtype is not torch.uint8 or workspace.get_device() != device or not workspace.is_contiguous():
         raise OperatorError("workspace must be a contiguous uint8 tensor on q's device")
     _call(device, _lib.load().pb_tree_attention_device, _ref(cache._c), _u32(layer, "layer"), heads, seqs, rows,
-          _ref(q_in), _ref(to), a, width, b, c, d, dim ** -0.5 if scale is None else scale, workspace.data_ptr(), workspace.numel())
+          _ref(q_in), _ref(to), a, width, b, c, d, dim ** -0.5 if scale is None else scale,
+          workspace.data_ptr(), workspace.numel())
     _written(out)
     return out
 

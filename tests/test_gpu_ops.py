@@ -812,6 +812,79 @@ def test_operators_on_a_side_stream_and_in_graphs():
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_operators_that_write_the_cache_on_a_side_stream_and_in_graphs(dtype):
+    """A drafting step with rows that go to their pages, a page that is copied and paths
+    that are kept: on a side stream while the default stream is held up, and from two
+    graphs on new inputs, it leaves the outputs and the cache that a plain call leaves."""
+    g, rng = gen(41), np.random.default_rng(41)
+    contexts, nodes, page = [500, 60], [6, 3], 16
+    cache, tables, _, _ = paged(g, rng, [c + t for c, t in zip(contexts, nodes)], page, 2, 64, dtype)
+    cache.k.copy_(normal(g, *cache.k.shape, dtype=dtype))
+    cache.v.copy_(normal(g, *cache.v.shape, dtype=dtype))
+    clean = cache.k.clone(), cache.v.clone()
+    table = tables.tolist()
+    spare = min(set(range(cache.pages)) - {p for row in table for p in row})
+    pairs = i32([[table[1][0], spare]])
+    at = [table[s][(c + j) // page] * page + (c + j) % page
+          for s, (c, t) in enumerate(zip(contexts, nodes)) for j in range(t)]
+    slots = i32(at)
+    counts, accepted = i32([2, 1]), i32([[1, 5], [2, 0]])
+    q, k, v = (normal(g, 9, h, 64, dtype=dtype) for h in (14, 2, 2))
+    plan, positions = ops.Rotary(64), i32(list(range(9)))
+    cs, offs, vis = i32(contexts), starts(nodes), masks([b for t in nodes for b in random_tree(rng, t)])
+
+    def reset():
+        cache.k.copy_(clean[0])
+        cache.v.copy_(clean[1])
+
+    def chain():
+        turned_q = plan.apply_to_cache(q, k, v, positions, cache, slots, layer=1)
+        tree = ops.tree_attention(turned_q, cache, tables, cs, offs, vis, layer=1)
+        packed = ops.prompt_attention(tree, k, v, offs)
+        cache.copy_pages(pairs)
+        cache.keep(tables, cs, counts, accepted)
+        return turned_q, tree, packed
+
+    def plain():
+        reset()
+        want = [x.clone() for x in (*chain(), cache.k, cache.v)]
+        for now, before in zip(want[3:], clean):  # each of the three has written
+            def row(x, i):
+                return x[1, at[i] // page, :, at[i] % page]
+            assert not torch.equal(row(now, 3), row(before, 3)) and torch.equal(row(now, 1), row(now, 5))
+            assert torch.equal(now[:, spare], now[:, table[1][0]]) and not torch.equal(now[:, spare], before[:, spare])
+        return want
+
+    def same(got, want):
+        return all(torch.equal(a, b) for a, b in zip((*got, cache.k, cache.v), want))
+    want = plain()
+    reset()
+    side, held = torch.cuda.Stream(), torch.cuda.Event()
+    side.wait_stream(torch.cuda.current_stream())
+    torch.cuda._sleep(400_000_000)  # some 0.2 s
+    held.record()
+    with torch.cuda.stream(side):
+        got = chain()
+    side.synchronize()
+    assert not held.query()  # the default stream was still at it
+    assert same(got, want)
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(chain())
+        graphs.append(graph)
+    for _ in range(2):
+        for x in (q, k, v):
+            x.copy_(normal(g, *x.shape, dtype=dtype))
+        want = plain()
+        for graph, out in zip(graphs, outs):
+            reset()
+            graph.replay()
+            assert same(out, want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_calls_on_two_streams_at_once_give_the_bits_of_calls_in_turn(dtype):
     g, rng = gen(26), np.random.default_rng(26)
     jobs = []
