@@ -156,10 +156,10 @@ struct pb_pool {
     uint32_t length = 0;
     std::vector<uint32_t> pages;
   };
-  uint32_t page_size = 0, free_count = 0;
+  uint32_t page_size = 0, free_count = 0, max_seqs = 0;
   std::vector<uint32_t> holders;  // sequences that hold each page
   std::vector<uint32_t> free_ids;  // the first free_count entries; sized for all pages
-  std::vector<Sequence> seqs;
+  std::vector<Sequence> seqs;  // as many as were ever open at once, max_seqs at most
 
   bool is_open(uint32_t s) const { return s < seqs.size() && seqs[s].open; }
   void drop(uint32_t page) {
@@ -246,9 +246,9 @@ uint32_t pb_pool_create(uint32_t pages, uint32_t page_size, uint32_t max_seqs, p
   if (!p) return no_memory(who);
   try {
     p->page_size = page_size;
+    p->max_seqs = max_seqs;
     p->holders.assign(pages, 0);
     p->free_ids.resize(pages);
-    p->seqs.resize(max_seqs);
   } catch (...) {
     delete p;
     return no_memory(who);
@@ -273,7 +273,15 @@ uint32_t pb_pool_open(pb_pool* p, uint32_t* seq) {
       *seq = s;
       return PB_OK;
     }
-  return pb::paged::refuse(PB_CAPACITY, who, "every sequence is open");
+  if (p->seqs.size() >= p->max_seqs) return pb::paged::refuse(PB_CAPACITY, who, "every sequence is open");
+  try {
+    p->seqs.emplace_back();
+  } catch (...) {
+    return no_memory(who);
+  }
+  p->seqs.back().open = true;
+  *seq = (uint32_t)p->seqs.size() - 1;
+  return PB_OK;
 }
 
 uint32_t pb_pool_fork(pb_pool* p, uint32_t seq, uint32_t* child) {

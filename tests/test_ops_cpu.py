@@ -309,6 +309,26 @@ def test_numbers_past_32_bits_are_refused_not_cut():
         ops.Rotary(64, 0)  # no rotation is not the whole head
 
 
+def test_a_pool_takes_memory_for_the_sequences_that_are_open_not_for_all_it_may_open():
+    import subprocess
+    import sys
+    code = """
+import ctypes, resource
+from promptboot_b200 import _lib
+lib, pool, seq, child = _lib.load(), ctypes.c_void_p(), ctypes.c_uint32(), ctypes.c_uint32()
+pair, needed = (ctypes.c_uint32 * 2)(), ctypes.c_uint32()
+size = int(open("/proc/self/statm").read().split()[0]) * resource.getpagesize()
+resource.setrlimit(resource.RLIMIT_AS, (size + (1 << 30),) * 2)
+assert lib.pb_pool_create(64, 16, 2**32 - 1, ctypes.byref(pool)) == 0, _lib.last_error()
+for want in range(1000):
+    assert lib.pb_pool_open(pool, ctypes.byref(seq)) == 0 and seq.value == want
+assert lib.pb_pool_extend(pool, 999, 40, pair, ctypes.byref(needed)) == 0
+assert lib.pb_pool_fork(pool, 999, ctypes.byref(child)) == 0 and child.value == 1000
+assert lib.pb_pool_free(pool, 7) == 0 and lib.pb_pool_open(pool, ctypes.byref(seq)) == 0 and seq.value == 7
+"""
+    assert subprocess.run([sys.executable, "-c", code], timeout=120).returncode == 0
+
+
 def test_pool_short_arrays_are_refused_with_the_number_needed():
     lib, pool = _lib.load(), ops.PagePool(8, 16, 2)
     a, b = pool.open(), pool.open()
