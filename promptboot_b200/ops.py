@@ -394,7 +394,8 @@ class PagePool:
         sequence's last page."""
         rows = [self.pages_of(s) for s in seqs]
         width = max([len(r) for r in rows] + [1])
-        return torch.tensor([r + [-1] * (width - len(r)) for r in rows], dtype=torch.int32, device=device)
+        rows = [r + [-1] * (width - len(r)) for r in rows]
+        return torch.tensor(rows, dtype=torch.int32, device=device).view(len(rows), width)
 
     def slots(self, seq, start, count, device="cuda"):
         """int32 cache slots of `count` positions from `start` on, for Rotary.apply_to_cache."""

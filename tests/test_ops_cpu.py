@@ -309,6 +309,15 @@ def test_numbers_past_32_bits_are_refused_not_cut():
         ops.Rotary(64, 0)  # no rotation is not the whole head
 
 
+def test_pool_tables_and_slots_of_nothing_keep_their_shapes():
+    pool = ops.PagePool(8, 16, 2)
+    assert pool.tables([], device="cpu").shape == (0, 1)
+    a = pool.open()
+    assert pool.tables([a], device="cpu").tolist() == [[-1]] and pool.slots(a, 0, 0, device="cpu").shape == (0,)
+    pool.extend(a, 17)
+    assert pool.tables([a, a], device="cpu").tolist() == [[0, 1], [0, 1]]
+
+
 def test_a_pool_takes_memory_for_the_sequences_that_are_open_not_for_all_it_may_open():
     import subprocess
     import sys
