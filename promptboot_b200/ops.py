@@ -269,15 +269,16 @@ def prompt_attention(q, k, v, offsets, kv_offsets=None, scale=None, out=None):
 @functools.lru_cache(maxsize=256)
 def _workspace_bytes(device, type_, dim, heads, kv_heads, seqs, rows):
     with torch.cuda.device(device):
-        return int(_lib.load().pb_tree_attention_workspace(type_, dim, heads, kv_heads, seqs, rows))
+        got = int(_lib.load().pb_tree_attention_workspace(type_, dim, heads, kv_heads, seqs, rows))
+    if not got:
+        raise OperatorError(_lib.last_error())  # (which is not cached)
+    return got
 
 
 def tree_workspace_bytes(cache, heads, seqs, rows):
     """Bytes of workspace that tree_attention needs for these sizes."""
-    got = _workspace_bytes(cache.device, _TYPES[cache.dtype], cache.head_dim, heads, cache.kv_heads, seqs, rows)
-    if not got:
-        raise OperatorError(_lib.last_error())
-    return got
+    return _workspace_bytes(cache.device, _TYPES[cache.dtype], cache.head_dim, _u32(heads, "heads"), cache.kv_heads,
+                            _u32(seqs, "seqs"), _u32(rows, "rows"))
 
 
 def tree_attention(q, cache, tables, contexts, offsets, visible, layer=0, scale=None, out=None, workspace=None):

@@ -141,6 +141,21 @@ def test_attention_scales_whose_power_of_two_is_not_finite_are_refused():
                                            2.3e38, None), CAPACITY, "kv_rows")
 
 
+def test_workspaces_refused_twice_say_why_twice(monkeypatch):
+    import contextlib
+    monkeypatch.setattr(torch.cuda, "device", lambda device: contextlib.nullcontext())
+    cache = ops.PageCache.__new__(ops.PageCache)
+    cache.device, cache.dtype, cache.head_dim, cache.kv_heads = 0, torch.bfloat16, 64, 2
+    for _ in range(2):
+        with pytest.raises(ops.OperatorError, match="multiple of kv_heads"):
+            ops.tree_workspace_bytes(cache, 3, 1, 8)
+        with pytest.raises(ops.OperatorError, match="sequences"):
+            ops.tree_workspace_bytes(cache, 4, 4096, 8)
+    assert ops.tree_workspace_bytes(cache, 4, 1, 8) == ops.tree_workspace_bytes(cache, 4, 1, 8) > 0
+    with pytest.raises(ops.OperatorError, match="out of range"):
+        ops.tree_workspace_bytes(cache, 4, 1, (1 << 32) + 8)
+
+
 def test_tree_attention_refusals():
     lib = _lib.load()
 
