@@ -509,6 +509,69 @@ def test_tree_attention_matches_the_definition(dtype, dim, heads, kv_heads, page
     check_tree(out, q, contexts, nodes, visible, keys, values, dim ** -0.5, dtype)
 
 
+def check_groups(got, q, keys, values, seen, dtype):
+    """check_heads for many heads: the heads that share a key head as rows of one."""
+    dim, group = q.shape[2], q.shape[1] // keys.shape[1]
+    rows = seen.repeat_interleave(group, 0)
+    for h in range(keys.shape[1]):
+        mine = slice(h * group, (h + 1) * group)
+        y, bound = attend(q[:, mine].reshape(-1, dim), keys[:, h], values[:, h], rows, dim ** -0.5, dtype)
+        assert_within(got[:, mine].reshape(-1, dim), y, bound)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 1024, 1), (128, 1024, 8), (64, 512, 512), (128, 129, 3)])
+def test_attention_of_the_most_heads(dtype, dim, heads, kv_heads):
+    g, rng = gen(34), np.random.default_rng(34)
+    tokens, keys = [3, 0, 1, 70], [3, 5, 130, 69]
+    q = normal(g, sum(tokens), heads, dim, dtype=dtype)
+    k, v = (normal(g, sum(keys), kv_heads, dim, dtype=dtype) for _ in range(2))
+    got = ops.prompt_attention(q, k, v, starts(tokens), kv_offsets=starts(keys))
+    at = kv_at = 0
+    for t, n in zip(tokens, keys):
+        check_groups(got[at:at + t], q[at:at + t], k[kv_at:kv_at + n], v[kv_at:kv_at + n], causal(t, n), dtype)
+        at, kv_at = at + t, kv_at + n
+    contexts, nodes = [40, 500, 0], [1, 3, 2]
+    cache, tables, keys, values = paged(g, rng, [c + t for c, t in zip(contexts, nodes)], 16, kv_heads, dim, dtype)
+    q = normal(g, sum(nodes), heads, dim, dtype=dtype)
+    got = ops.tree_attention(q, cache, tables, i32(contexts), starts(nodes), masks([1, 1, 2, 5, 1, 3]), layer=1)
+    at = 0
+    for s, (c, t, bits) in enumerate(zip(contexts, nodes, ([1], [1, 2, 5], [1, 3]))):
+        seen = torch.tensor([[j < c or b >> (j - c) & 1 == 1 for j in range(c + t)] for b in bits], device="cuda")
+        check_groups(got[at:at + t], q[at:at + t], keys[s], values[s], seen, dtype)
+        at += t
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_of_the_most_sequences(dtype):
+    """2048 of them, one with nearly all the rows; one more is refused."""
+    g, rng = gen(35), np.random.default_rng(35)
+    tokens = [1] * 2048
+    tokens[1000], tokens[1001], tokens[7] = 300, 0, 64
+    q, k, v = (normal(g, sum(tokens), h, 64, dtype=dtype) for h in (4, 1, 1))
+    got = ops.prompt_attention(q, k, v, starts(tokens))
+    first = np.concatenate([[0], np.cumsum(tokens)])
+    for s in (0, 7, 999, 1000, 1002, 2047):
+        rows = slice(int(first[s]), int(first[s + 1]))
+        check_heads(got[rows], q[rows], k[rows], v[rows], causal(tokens[s], tokens[s]), 0.125, dtype)
+    alone = torch.tensor([s not in (7, 1000) for s in np.repeat(np.arange(2048), tokens)], device="cuda")
+    assert torch.equal(got[alone], v[alone].expand(-1, 4, -1))  # one key: its value
+    contexts = [int(c) for c in rng.integers(0, 40, 2048)]
+    contexts[1000] = 5000
+    nodes = [min(t, 64) for t in tokens]
+    cache, tables, keys, values = paged(g, rng, [c + t for c, t in zip(contexts, nodes)], 16, 1, 64, dtype)
+    q = normal(g, sum(nodes), 4, 64, dtype=dtype)
+    visible = [b for t in nodes for b in random_tree(rng, t)]
+    got = ops.tree_attention(q, cache, tables, i32(contexts), starts(nodes), masks(visible), layer=1)
+    first = np.concatenate([[0], np.cumsum(nodes)])
+    for s in (0, 7, 999, 1000, 1002, 2047):
+        rows = slice(int(first[s]), int(first[s + 1]))
+        check_tree(got[rows], q[rows], contexts[s:s + 1], nodes[s:s + 1], visible[rows], keys[s:s + 1],
+                   values[s:s + 1], 0.125, dtype)
+    with pytest.raises(ops.OperatorError, match="sequences"):
+        ops.prompt_attention(q, q[:, :1], q[:, :1], i32([0] * 2050))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_tree_attention_rows_that_see_nothing_and_odd_masks(dtype):
     """Masks that leave a row empty without a context, that skip the row's own node,
