@@ -825,6 +825,47 @@ def test_keep_of_no_nodes_and_of_a_count_that_stands_for_none():
     assert torch.equal(cache.k, want) and torch.equal(cache.v, want + 1)
 
 
+@pytest.mark.parametrize("dtype,pages", [(torch.float32, 9000), (torch.bfloat16, 18000)])
+def test_places_past_32_bits(dtype, pages):
+    """A cache of more than 2^31 elements a side (2^32 in 16 bits), and packed rows as far
+    apart: every operator on the last of them."""
+    g, rng = gen(36), np.random.default_rng(36)
+    cache = ops.PageCache.empty(1, pages, 8, 256, 128, dtype)
+    assert cache.k.numel() * cache.k.itemsize > 1 << 33
+    tables = i32([[pages - 1, 2, pages - 3], [pages - 4, pages - 5, 1]])
+    contexts, nodes, lengths = [520, 300], [9, 2], [529, 302]
+    keys, values = [], []
+    for s, n in enumerate(lengths):
+        k, v = (normal(g, n, 8, 128, dtype=dtype) for _ in range(2))
+        at = torch.arange(n, device="cuda")
+        slots = tables[s][at // 256] * 256 + at.to(torch.int32) % 256
+        zero = torch.zeros(n, dtype=torch.int32, device="cuda")  # at position 0 nothing turns
+        ops.Rotary(128).apply_to_cache(k, k, v, zero, cache, slots.to(torch.int32))
+        keys.append(k)
+        values.append(v)
+    visible = [b for t in nodes for b in random_tree(rng, t)]
+    for heads in (8, 32):
+        q = normal(g, sum(nodes), heads, 128, dtype=dtype)
+        got = ops.tree_attention(q, cache, tables, i32(contexts), starts(nodes), masks(visible))
+        check_tree(got, q, contexts, nodes, visible, keys, values, 128 ** -0.5, dtype)
+    cache.copy_pages(i32([[pages - 1, pages - 2]]))
+    cache.keep(tables, i32(contexts), i32([2, 1]), i32([[3, 8], [1, 0]]))
+    for x, y in ((cache.k, keys), (cache.v, values)):
+        assert torch.equal(x[0, pages - 2].transpose(0, 1), y[0][:256])
+        assert torch.equal(x[0, pages - 3, :, 8:10].transpose(0, 1), y[0][[523, 528]])
+        assert torch.equal(x[0, pages - 5, :, 44], y[1][301])
+    apart = cache.k.view(-1)
+    far = apart.numel() // 3 // 64 * 64
+    q, k, v, out = (apart[i * 4096:].as_strided((3, h, 64), (far, 64, 1), i * 4096) for i, h in enumerate((4, 2, 2, 4)))
+    for x in (q, k, v):
+        x.copy_(normal(g, *x.shape, dtype=dtype))
+    want_q, want_k = ops.Rotary(64).apply(q.contiguous(), k.contiguous(), i32([7, 8, 9]))
+    ops.Rotary(64).apply(q, k, i32([7, 8, 9]), q_out=q, k_out=k)
+    assert torch.equal(q, want_q) and torch.equal(k, want_k)
+    ops.prompt_attention(q, k, v, i32([0, 3]), out=out)
+    assert torch.equal(out, ops.prompt_attention(want_q, want_k, v.contiguous(), i32([0, 3])))
+
+
 # ------------------------------------------------------------- streams and graphs
 
 def test_operators_on_a_side_stream_and_in_graphs():
