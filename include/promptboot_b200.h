@@ -374,8 +374,8 @@ PB_API uint32_t pb_rotary_cache_device(const pb_rotary *rotary, uint32_t rows,
  * head h reading key head h / (q_heads / kv_heads).  Sequence s has the q rows
  * [q_offsets[s], q_offsets[s + 1]) and the key rows [kv_offsets[s], kv_offsets
  * [s + 1]) (kv_offsets NULL: the same), both aligned at their ends: row i of t
- * sees the first n - t + i + 1 of n keys.  A row that sees none is zero; rows
- * behind q_offsets[seqs] stay as they were.  Offsets ascend; they are cut at
+ * sees the first n - t + i + 1 of n keys.  A row that sees none, or whose scores
+ * are all -inf, is zero; rows behind q_offsets[seqs] stay as they were.  Offsets ascend; they are cut at
  * q_rows and kv_rows.  Keys that a row does not see have no part in it whatever
  * they hold.  head_dim 64 or 128, seqs up to PB_MAX_SEQS, scale positive and scale
  * log2(e) finite. */

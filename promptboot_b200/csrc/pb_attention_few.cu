@@ -11,8 +11,9 @@
 // 37.6, for 256 single tokens over 512 to 1535 positions).  The legacy tensor path is the right one here: a tcgen05 tile has 128 rows, so that one
 // token of seven heads would pay for 18 times its products, and its scores would pass
 // through TMEM on the way.  Bound by memory and by the latency of a warp's chain
-// through a tile (some 1000 cycles), of which eight are under way on an SM; one warp
-// that fed all others was a bound of its own (a copy takes it some 100 cycles).
+// through a tile (some 1000 cycles), of which twelve are under way on an SM at heads of 64
+// with one row group and eight else; one warp that fed all others was a bound of its own
+// (a copy takes it some 100 cycles).
 #include "pb_attention_launch.h"
 #include "pb_attention_tma.cuh"
 

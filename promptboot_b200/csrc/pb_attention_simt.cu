@@ -9,7 +9,7 @@
 // The keys of the next tile are on their way while the weights are found and the values
 // added, its values while its scores are.  Bound by the latency of a warp's chain and
 // the reads of shared memory that feed its multiply-adds.  Row tiles of 32, four CTAs an
-// SM: a prompt of 2500 tokens, 14 heads of 64 to 2, takes 370 us, 30 TFLOP/s (tiles of 64:
+// SM (three of prompts at heads of 128, by their registers): a prompt of 2500 tokens, 14 heads of 64 to 2, takes 370 us, 30 TFLOP/s (tiles of 64:
 // 394, of 16: 492); 8 of 2500 in all 112 (139, 126); trees of 8 nodes over 32 x 3000
 // positions, 32 heads of 128 to 8, 438 us, 23 TFLOP/s (886 with tiles of 64, half empty).
 #include "pb_attention_launch.h"

@@ -20,12 +20,12 @@
 // Prompts: a CTA that is done cancels one that has not begun and takes its unit, so that
 // the start of a CTA is paid once an SM and the longest units do not end last.
 //
-// Bound by the softmax warps' instructions, 750 cycles per scheduler for 64 keys of a
-// row tile where the exponentials (16 a cycle and SM) need 512: measured with two, three
-// and four softmax warps per scheduler, the schedulers issue 0.55 instructions a cycle
-// and no more, since the packed products and the maxima share register ports (a pair of
-// them takes 3.25 cycles, each alone 2).  One prompt of 16384 (14 heads of 64): 0.61 ms
-// alone, 784 TFLOP/s; one of 4096 at 32 heads of 128: 125 us, 1100 TFLOP/s.  Three
+// Bound by the softmax warps, 750 cycles per scheduler for 64 keys of a row tile where
+// the exponentials (16 a cycle and SM) need 512.  No unit is full meanwhile (issue 47%,
+// exponential unit 60%, tensor pipe 33%, prompt of 8192 at heads of 64); two, three and
+// four softmax warps per scheduler measured the same, 0.47 to 0.55 instructions a cycle.
+// One prompt of 16384 (14 heads of 64): 0.61 ms alone, 784 TFLOP/s, 670 us where calls
+// follow one another; one of 4096 at 32 heads of 128: 125 us alone, 1100 TFLOP/s.  Three
 // row tiles a CTA that share the key tiles gained 5% there and lost as much on ragged
 // batches; four CTAs an SM with one score buffer each, and weights formed with the
 // maximum of the tile before, measured the same or worse.

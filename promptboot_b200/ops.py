@@ -9,7 +9,7 @@ current torch stream, and returns at once.  Index tensors are contiguous int32
 or a context length.  Head tensors are [rows, heads, head_dim] of
 float32, float16 or bfloat16 with a contiguous last dimension, any other strides a
 multiple of 16 bytes, so that views of a stacked q/k/v projection serve as they
-are.  Refused arguments raise OperatorError.  There are no gradients: a tensor that
+are.  An output shares no memory with an input unless its call says that it may.  Refused arguments raise OperatorError.  There are no gradients: a tensor that
 asks for one, one of a cache too, is refused unless grad mode is off, and one that
 carries a forward-mode tangent always.
 """
@@ -148,7 +148,8 @@ class PageCache:
                    torch.empty(shape, dtype=dtype, device=device))
 
     def copy_pages(self, pairs):
-        """Copies page pairs[i, 0] to page pairs[i, 1] in every layer."""
+        """Copies page pairs[i, 0] to page pairs[i, 1] in every layer.  A page may be the
+        source of several pairs, but the target of one only, and not a source then."""
         _no_gradient(self)
         n = pairs.shape[0]
         at = _index(pairs, (n, 2), self.device, "pairs")
@@ -198,7 +199,8 @@ class Rotary:
             pass
 
     def apply(self, q, k, positions, q_out=None, k_out=None):
-        """(q, k) turned, in new tensors or in q_out and k_out, which may be q and k."""
+        """(q, k) turned, in new tensors or in q_out and k_out, which may be q and k.  Rows
+        at position -1 stay as they were, unset in a new tensor."""
         dtype, device = _first(q, "q")
         q_in, k_in = _heads(q, dtype, device, "q"), _heads(k, dtype, device, "k")
         rows, heads, dim = q.shape
@@ -219,7 +221,8 @@ class Rotary:
 
     def apply_to_cache(self, q, k, v, positions, cache, slots, layer=0, q_out=None):
         """q turned, as apply; k turned and v go to `layer` of the cache at
-        slots[row] = page * page_size + slot in the page (-1: nowhere)."""
+        slots[row] = page * page_size + slot in the page (-1: nowhere).  Of rows with
+        the same slot it holds a mix."""
         _no_gradient(cache)
         dtype, device = cache.dtype, cache.device
         q_in, k_in, v_in = (_heads(q, dtype, device, "q"), _heads(k, dtype, device, "k"),
@@ -330,7 +333,7 @@ def attention_status(device=None):
 
 class PagePool:
     """The host's book of a cache's pages: which pages each sequence holds, shared
-    between forks until one of them writes."""
+    between forks until one of them writes.  One thread at a time."""
 
     def __init__(self, pages, page_size, max_seqs):
         self._h = ctypes.c_void_p()
