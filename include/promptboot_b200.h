@@ -309,7 +309,8 @@ enum { PB_TYPE_F32 = 0, PB_TYPE_F16 = 1, PB_TYPE_BF16 = 2 };
 
 /* Rows of heads on the device: element c of head h of row r is data[r *
  * row_stride + h * head_stride + c], strides in elements.  data is 16-byte
- * aligned and both strides are multiples of 16 bytes. */
+ * aligned and both strides are multiples of 16 bytes; those of an output that has
+ * several rows or heads are not 0. */
 typedef struct pb_rows {
     void *data;
     uint64_t row_stride, head_stride;

@@ -80,7 +80,7 @@ uint32_t pb_prompt_attention_device(uint32_t type, uint32_t head_dim, uint32_t q
   if (!kv_rows) k = v = q;  // not read: without key rows they may be NULL
   if ((st = pb::paged::check_rows(k, bytes, who, "k"))) return st;
   if ((st = pb::paged::check_rows(v, bytes, who, "v"))) return st;
-  if ((st = pb::paged::check_rows(out, bytes, who, "out"))) return st;
+  if ((st = pb::paged::check_output(out, bytes, q_rows, q_heads, who, "out"))) return st;
   if (kv_rows > 1 && (!k->row_stride || !v->row_stride))
     return refuse(PB_CAPACITY, who, "k and v need a row stride");
   pb::paged::AttnArgs a{};
@@ -123,7 +123,7 @@ uint32_t pb_tree_attention_device(const pb_cache* cache, uint32_t layer, uint32_
   if (!rows) return PB_OK;
   const uint32_t bytes = pb::paged::type_bytes(cache->type);
   if ((st = pb::paged::check_rows(q, bytes, who, "q"))) return st;
-  if ((st = pb::paged::check_rows(out, bytes, who, "out"))) return st;
+  if ((st = pb::paged::check_output(out, bytes, rows, q_heads, who, "out"))) return st;
   if (!tables || !table_width || !contexts || !offsets || !visible)
     return refuse(PB_CAPACITY, who, "an empty table or a NULL argument");
   // Key tiles are counted in 32 bits: of `least` keys or more, for row tiles of `least` or more.

@@ -38,6 +38,19 @@ inline uint32_t check_rows(const pb_rows* r, uint32_t bytes, const char* who, co
   return PB_OK;
 }
 
+// A pb_rows that is written: its rows and heads may not lie on one another (a stride of 0).
+inline uint32_t check_output(const pb_rows* r, uint32_t bytes, uint32_t rows, uint32_t heads, const char* who,
+                             const char* name) {
+  const uint32_t st = check_rows(r, bytes, who, name);
+  if (st) return st;
+  if ((rows > 1 && !r->row_stride) || (heads > 1 && !r->head_stride)) {
+    char text[160];
+    std::snprintf(text, sizeof text, "%s needs a row stride and a head stride", name);
+    return refuse(PB_CAPACITY, who, text);
+  }
+  return PB_OK;
+}
+
 inline uint32_t check_cache(const pb_cache* c, const char* who) {
   if (!c || !c->k || !c->v) return refuse(PB_CAPACITY, who, "the cache is NULL");
   const uint32_t bytes = type_bytes(c->type);

@@ -234,9 +234,9 @@ uint32_t pb_rotary_device(const pb_rotary* rotary, uint32_t type, uint32_t rows,
     return pb::paged::refuse(PB_CAPACITY, who, "rows, q_heads or k_heads out of range");
   uint32_t st;
   if ((st = pb::paged::check_rows(q, bytes, who, "q"))) return st;
-  if ((st = pb::paged::check_rows(q_out, bytes, who, "q_out"))) return st;
+  if ((st = pb::paged::check_output(q_out, bytes, rows, q_heads, who, "q_out"))) return st;
   if (k_heads && (st = pb::paged::check_rows(k, bytes, who, "k"))) return st;
-  if (k_heads && (st = pb::paged::check_rows(k_out, bytes, who, "k_out"))) return st;
+  if (k_heads && (st = pb::paged::check_output(k_out, bytes, rows, k_heads, who, "k_out"))) return st;
   if (!pb::same_or_apart(q, q_out) || (k_heads && !pb::same_or_apart(k, k_out)))
     return pb::paged::refuse(PB_CAPACITY, who, "an output in place needs its input's strides");
   pb::RotaryArgs a{};
@@ -262,7 +262,7 @@ uint32_t pb_rotary_cache_device(const pb_rotary* rotary, uint32_t rows, const ui
   if (cache->head_dim != rotary->config.head_dim)
     return pb::paged::refuse(PB_CAPACITY, who, "the cache has another head_dim");
   if ((st = pb::paged::check_rows(q, bytes, who, "q"))) return st;
-  if ((st = pb::paged::check_rows(q_out, bytes, who, "q_out"))) return st;
+  if ((st = pb::paged::check_output(q_out, bytes, rows, q_heads, who, "q_out"))) return st;
   if ((st = pb::paged::check_rows(k, bytes, who, "k"))) return st;
   if ((st = pb::paged::check_rows(v, bytes, who, "v"))) return st;
   if (!pb::same_or_apart(q, q_out))

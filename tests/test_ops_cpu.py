@@ -141,6 +141,24 @@ def test_attention_scales_whose_power_of_two_is_not_finite_are_refused():
                                            2.3e38, None), CAPACITY, "kv_rows")
 
 
+def test_outputs_whose_rows_or_heads_lie_on_one_another_are_refused():
+    lib, plan, r = _lib.load(), ops.Rotary(64), rows()
+    for bad in (rows(row=0), rows(head=0)):
+        refused(lib.pb_prompt_attention_device(2, 64, 4, 2, 1, 8, 8, ref(r), ref(r), ref(r), ref(bad), FAKE, FAKE, 1.0,
+                                               None), CAPACITY, "out needs a row stride")
+        refused(lib.pb_tree_attention_device(ref(cache()), 0, 4, 1, 8, ref(r), ref(bad), FAKE, 4, FAKE, FAKE, FAKE, 1.0,
+                                             FAKE, 1 << 40, None), CAPACITY, "out needs a row stride")
+        refused(lib.pb_rotary_device(plan._h, 0, 4, FAKE, 2, ref(bad), ref(bad), 0, None, None, None), CAPACITY,
+                "q_out needs a row stride")
+        refused(lib.pb_rotary_device(plan._h, 0, 4, FAKE, 2, ref(r), ref(r), 2, ref(r), ref(bad), None), CAPACITY,
+                "k_out needs a row stride")
+        refused(lib.pb_rotary_cache_device(plan._h, 4, FAKE, 2, ref(r), ref(bad), ref(r), ref(r), ref(cache()), 0, FAKE,
+                                           None), CAPACITY, "q_out needs a row stride")
+    # one row of one head has no strides to speak of: the next check speaks
+    refused(lib.pb_rotary_device(plan._h, 0, 1, FAKE, 1, ref(r), ref(rows(row=0, head=0)), 1, ref(r), None, None),
+            CAPACITY, "k_out is NULL")
+
+
 def test_workspaces_refused_twice_say_why_twice(monkeypatch):
     import contextlib
     monkeypatch.setattr(torch.cuda, "device", lambda device: contextlib.nullcontext())
