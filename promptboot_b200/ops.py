@@ -51,6 +51,22 @@ def _u32(x, name):
     return x
 
 
+class _Handle(ctypes.c_void_p):
+    """A handle of the C ABI, destroyed with its last holder: copies of an object share it."""
+
+    def __init__(self, destroy):
+        super().__init__()
+        self._destroy = destroy
+
+    def __del__(self):
+        try:
+            if self.value:
+                getattr(_lib.load(), self._destroy)(self)
+                self.value = None
+        except Exception:
+            pass
+
+
 def _check(status: int):
     if status == 0:
         return
@@ -187,16 +203,8 @@ class Rotary:
                                      _LAYOUTS[bool(interleaved)], _SCALINGS[scaling], theta, factor,
                                      original_context, low, high, magnitude)
         self.head_dim = head_dim
-        self._h = ctypes.c_void_p()
+        self._h = _Handle("pb_rotary_destroy")
         _check(_lib.load().pb_rotary_create(_ref(config), _ref(self._h)))
-
-    def __del__(self):
-        try:
-            if self._h:
-                _lib.load().pb_rotary_destroy(self._h)
-                self._h = None
-        except Exception:
-            pass
 
     def apply(self, q, k, positions, q_out=None, k_out=None):
         """(q, k) turned, in new tensors or in q_out and k_out, which may be q and k.  Rows
@@ -336,18 +344,10 @@ class PagePool:
     between forks until one of them writes.  One thread at a time."""
 
     def __init__(self, pages, page_size, max_seqs):
-        self._h = ctypes.c_void_p()
+        self._h = _Handle("pb_pool_destroy")
         _check(_lib.load().pb_pool_create(_u32(pages, "pages"), _u32(page_size, "page_size"),
                                           _u32(max_seqs, "max_seqs"), _ref(self._h)))
         self.pages, self.page_size = pages, page_size
-
-    def __del__(self):
-        try:
-            if self._h:
-                _lib.load().pb_pool_destroy(self._h)
-                self._h = None
-        except Exception:
-            pass
 
     def open(self):
         """A new sequence without tokens."""

@@ -342,6 +342,28 @@ def test_numbers_past_32_bits_are_refused_not_cut():
         ops.Rotary(64, 0)  # no rotation is not the whole head
 
 
+def test_copies_of_a_plan_or_a_pool_share_what_is_destroyed_once(monkeypatch):
+    import copy
+    lib, gone = _lib.load(), []
+
+    class Spy:
+        def __getattr__(self, name):
+            if name.endswith("_destroy"):
+                return lambda h: (gone.append(name), getattr(lib, name)(h))
+            return getattr(lib, name)
+    monkeypatch.setattr(ops._lib, "load", Spy)
+    pool, plan = ops.PagePool(8, 16, 2), ops.Rotary(64)
+    others = copy.copy(pool), copy.copy(plan)
+    del pool, plan
+    assert gone == []
+    assert others[0].extend(others[0].open(), 40) is None and others[0].free_pages() == 5
+    del others
+    assert sorted(gone) == ["pb_pool_destroy", "pb_rotary_destroy"]
+    with pytest.raises(ops.OperatorError):
+        ops.PagePool(0, 16, 2)  # nothing was made, nothing is destroyed
+    assert len(gone) == 2
+
+
 def test_pool_tables_and_slots_of_nothing_keep_their_shapes():
     pool = ops.PagePool(8, 16, 2)
     assert pool.tables([], device="cpu").shape == (0, 1)
