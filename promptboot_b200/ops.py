@@ -52,11 +52,15 @@ def _u32(x, name):
 
 
 class _Handle(ctypes.c_void_p):
-    """A handle of the C ABI, destroyed with its last holder: copies of an object share it."""
+    """A handle of the C ABI, destroyed with its last holder: copies of an object share it.
+    It is not copied itself, so its object cannot be pickled or copied deeply."""
 
     def __init__(self, destroy):
         super().__init__()
         self._destroy = destroy
+
+    def __reduce_ex__(self, protocol):
+        raise TypeError("handles of the C ABI cannot be pickled or copied")
 
     def __del__(self):
         try:

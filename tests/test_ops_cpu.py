@@ -344,6 +344,7 @@ def test_numbers_past_32_bits_are_refused_not_cut():
 
 def test_copies_of_a_plan_or_a_pool_share_what_is_destroyed_once(monkeypatch):
     import copy
+    import pickle
     lib, gone = _lib.load(), []
 
     class Spy:
@@ -353,6 +354,10 @@ def test_copies_of_a_plan_or_a_pool_share_what_is_destroyed_once(monkeypatch):
             return getattr(lib, name)
     monkeypatch.setattr(ops._lib, "load", Spy)
     pool, plan = ops.PagePool(8, 16, 2), ops.Rotary(64)
+    for x in (pool, plan):
+        for whole in (copy.deepcopy, pickle.dumps):
+            with pytest.raises(TypeError, match="copied"):
+                whole(x)
     others = copy.copy(pool), copy.copy(plan)
     del pool, plan
     assert gone == []
