@@ -413,8 +413,8 @@ PB_API uint32_t pb_tree_attention_device(const pb_cache *cache, uint32_t layer, 
 
 /* Waits for `stream` and reports whether any prompt or tree attention on the current
  * device, on this stream or another, gave up waiting for a copy or a product since the
- * calling host thread last asked (PB_DEVICE, once to each thread; the outputs of that
- * attention are not complete).  Not to be called while a graph is captured. */
+ * calling host thread last asked, or ever where it has not (PB_DEVICE, once to each
+ * thread; the outputs of that attention are not complete).  Not to be called while a graph is captured. */
 PB_API uint32_t pb_attention_status(void *stream);
 
 /* Copies page pairs[2 i] to page pairs[2 i + 1] for i < n, keys and values of
